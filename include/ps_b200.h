@@ -483,6 +483,79 @@ int ps_chunk_step_static(const ps_chunk_desc* chunks_host, uint32_t n_chunks, ui
                          const ps_segment* segs_host, uint32_t n_segs,
                          const ps_hyper_slot* slots_host, uint32_t n_slots, int skip, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * 8-bit products of a training step.  No counterpart in the reference.
+ *
+ * A matrix in 8-bit floating point carries one power-of-two scale for each
+ * block of 128: 1 x 128 ("row"), 128 x 1 ("col") or 128 x 128 ("tile").  Its
+ * values are row-major, each row starting a multiple of 16 bytes after the one
+ * before.  A scale 2^e is held as the byte e + 127.
+ *
+ * Scale bytes lie as the tensor core reads them.  For a contraction over L
+ * elements and O outer elements the array is
+ *     uint8 [ceil(L / 512)][ceil(O / 128)][32][4][4]
+ * and the byte of outer element o and contracted block kb = k / 128 is at
+ *     [kb / 4][o / 128][o % 32][(o % 128) / 32][kb % 4];
+ * places that stand for no element hold 0.
+ * ------------------------------------------------------------------------- */
+#define PS_DTYPE_F16 0
+#define PS_DTYPE_BF16 1
+#define PS_DTYPE_F32 2
+
+#define PS_FP8_E4M3 0 /* largest 448, no infinity   */
+#define PS_FP8_E5M2 1 /* largest 57344, infinities  */
+
+#define PS_BLOCKS_ROW 0     /* 1 x 128: contracted along a row                     */
+#define PS_BLOCKS_COL 1     /* 128 x 1: contracted along a column                  */
+#define PS_BLOCKS_ROW_COL 2 /* both of the above, two outputs from one read        */
+#define PS_BLOCKS_TILE 3    /* 128 x 128: one output, contracted either way        */
+
+/* Quantizes x[rows, cols] (row stride ld elements: any, rows may overlap; any
+ * alignment of the type):
+ *     amax = largest finite magnitude of the block = m 2^E, 1 <= m < 2
+ *     e    = E - top + (m > 1.75),  top = 8 (e4m3) or 15 (e5m2), e + 127 clamped to [1, 254]
+ *     q    = x 2^-e rounded to nearest even.
+ * A block whose amax is 0 or subnormal has the byte 1.  An element that is not
+ * finite becomes NaN (e4m3) or stays itself (e5m2).
+ *   q1, s1 : values and scales for a contraction over the columns (ROW, ROW_COL, TILE)
+ *   q0, s0 : values and scales for a contraction over the rows (COL, ROW_COL); TILE has the
+ *            values in q1 and both scale arrays
+ * Rows of q1 and q0 are ldq bytes (a multiple of 16, >= cols); the bytes behind
+ * the last column up to the next multiple of 8 are written with 0, further ones
+ * are left as they were.  colsum (ROW_COL only, may be NULL): float
+ * [ceil(rows / 128)][cols], the column sums of each run of 128 rows of x. */
+int ps_block_quantize(const void* x_dev, int dtype, uint64_t ld, uint32_t rows, uint32_t cols, int blocks, int fmt,
+                      void* q1_dev, void* s1_dev, void* q0_dev, void* s0_dev, uint64_t ldq, float* colsum_dev,
+                      void* stream);
+
+/* out[c] = sum over b of partial[b][c], in order and in 64 bits, rounded to `dtype`. */
+int ps_column_sum(const float* partial_dev, uint32_t blocks, uint32_t cols, void* out_dev, int dtype, void* stream);
+
+/* One operand of a product.  k_dim is the contracted dimension of the stored
+ * matrix: 1 = the columns ([outer, k]), 0 = the rows ([k, outer]); `scales` is
+ * the array for that contraction.  data, scales: 16-byte aligned; ld (bytes
+ * between rows): a multiple of 16. */
+typedef struct ps_block_operand {
+    const void* data;
+    const void* scales;
+    uint64_t ld;
+    int32_t fmt;
+    int32_t k_dim;
+} ps_block_operand;
+
+/* out[i, j] = sum_k a(i, k) b(j, k) (+ bias[j]) over the scaled values,
+ * accumulated in 32 bits, rounded once to out_dtype.  out is row-major with row
+ * stride ldo elements; elements behind column n are left as they were.  k == 0
+ * gives the bias, or zeros; m == 0 or n == 0 does nothing.  The operand structs
+ * are read before the call returns. */
+int ps_block_matmul(const ps_block_operand* a, const ps_block_operand* b, uint32_t m, uint32_t n, uint32_t k,
+                    const void* bias_dev, int bias_dtype, void* out_dev, int out_dtype, uint64_t ldo, void* stream);
+
+/* Number of thread blocks of ps_block_matmul on the current device that gave up
+ * a wait (2 s) since the library was loaded; such a block's part of the output
+ * is NaN.  0 unless the GPU is being held by something else.  Synchronises. */
+int ps_block_matmul_gave_up(uint32_t* count);
+
 /* Tuning knobs for measurements: "unroll" (1, 2, 4: 128-bit groups per thread
  * per tile of the step kernels), "scan_unroll" (1, 2, 4), "blocks_per_sm"
  * (0 = occupancy calculator), "bulk" (0, or 2..4 stages of the bulk-async

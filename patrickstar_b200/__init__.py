@@ -5,6 +5,10 @@ Public names mirror the reference's for this path:
     from patrickstar_b200 import FP16Adam, DynamicLossScaler, LossScaler, initialize_engine
     from patrickstar_b200 import cpu_adam_op      # create_adam / adam_update / destroy_adam
 
+Operators of the training step around it, which the reference leaves to torch:
+
+    from patrickstar_b200 import fp8_linear, Fp8Linear, block_quantize, block_matmul
+
 Everything that computes goes through ``libps_b200.so`` (hand-written sm_100a
 CUDA behind a C ABI, ``include/ps_b200.h``).  There is no CPU or PyTorch
 fallback: importing a compute name without the built library raises.
@@ -20,6 +24,12 @@ _LAZY = {
     "initialize_engine": ("engine", "initialize_engine"),
     "ChunkStepEngine": ("engine", "ChunkStepEngine"),
     "cpu_adam_op": ("cpu_adam_op", None),
+    "BlockQuantized": ("block_fp8", "BlockQuantized"),
+    "block_quantize": ("block_fp8", "block_quantize"),
+    "block_matmul": ("block_fp8", "block_matmul"),
+    "fp8_linear": ("block_fp8", "fp8_linear"),
+    "Fp8Linear": ("block_fp8", "Fp8Linear"),
+    "use_fp8_linears": ("block_fp8", "use_fp8_linears"),
 }
 
 

@@ -21,6 +21,10 @@ PS_ERR_CUDA = -4
 PS_ERR_TABLE = -5
 PS_ERR_LIMIT = -6
 
+PS_DTYPE_F16, PS_DTYPE_BF16, PS_DTYPE_F32 = 0, 1, 2
+PS_FP8_E4M3, PS_FP8_E5M2 = 0, 1
+PS_BLOCKS_ROW, PS_BLOCKS_COL, PS_BLOCKS_ROW_COL, PS_BLOCKS_TILE = 0, 1, 2, 3
+
 PS_MAX_GROUPS = 15
 PS_MAX_SLOTS = PS_MAX_GROUPS + 1
 PS_STATIC_MAX_CHUNKS = 256
@@ -82,6 +86,12 @@ class StepCtrl(C.Structure):
                 ("slots", HyperSlot * PS_MAX_SLOTS)]
 
 
+class BlockOperand(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("scales", C.c_void_p), ("ld", C.c_uint64), ("fmt", C.c_int32),
+                ("k_dim", C.c_int32)]
+
+
+assert C.sizeof(BlockOperand) == 32
 assert C.sizeof(StepPlan) == 512 and C.sizeof(ScalerState) == 64
 assert C.sizeof(HyperSlot) == 64 and C.sizeof(StepCtrl) == 48 + 64 * PS_MAX_SLOTS
 
@@ -132,6 +142,12 @@ SIGNATURES = {
     "ps_scaler_read": (C.c_int, [_p, C.POINTER(ScalerState), _p]),
     "ps_ctrl_read": (C.c_int, [_p, C.POINTER(StepCtrl), _p]),
     "ps_scale_loss": (C.c_int, [_p, _p, C.c_size_t, _p, _p]),
+    "ps_block_quantize": (C.c_int, [_p, C.c_int, C.c_uint64, C.c_uint32, C.c_uint32, C.c_int, C.c_int, _p, _p, _p, _p,
+                                    C.c_uint64, _p, _p]),
+    "ps_column_sum": (C.c_int, [_p, C.c_uint32, C.c_uint32, _p, C.c_int, _p]),
+    "ps_block_matmul": (C.c_int, [C.POINTER(BlockOperand), C.POINTER(BlockOperand), C.c_uint32, C.c_uint32,
+                                  C.c_uint32, _p, C.c_int, _p, C.c_int, C.c_uint64, _p]),
+    "ps_block_matmul_gave_up": (C.c_int, [C.POINTER(C.c_uint32)]),
 }
 
 

@@ -1,0 +1,352 @@
+"""8-bit matrix products of a training step, with one scale for each block of 128.
+
+The matrix products of a model's forward and backward pass on the tensor cores'
+8-bit path, next to the fp16 parameters and gradients the chunk step works on:
+
+  * ``block_quantize``  a matrix into e4m3 or e5m2 with a power-of-two scale for
+    each block of 1 x 128, 128 x 1 or 128 x 128 elements,
+  * ``block_matmul``    the product of two such matrices, accumulated in 32 bits,
+  * ``fp8_linear``, ``Fp8Linear``  the linear layer made of them, with its three
+    gradients, on ordinary fp16 / bf16 / fp32 tensors and parameters.
+
+The scales are powers of two like the loss scale: scaling is exact, and the
+tensor core applies them.  An element that is not finite stays visible (NaN in
+e4m3, itself in e5m2), so a gradient that overflowed still reaches the overflow
+test of the step.  No counterpart in the reference.
+"""
+import ctypes as C
+import math
+
+import torch
+
+from ._lib import (PS_BLOCKS_COL, PS_BLOCKS_ROW, PS_BLOCKS_ROW_COL, PS_BLOCKS_TILE, PS_DTYPE_BF16, PS_DTYPE_F16,
+                   PS_DTYPE_F32, PS_FP8_E4M3, PS_FP8_E5M2, BlockOperand, check, lib)
+
+BLOCK = 128
+
+_DTYPES = {torch.float16: PS_DTYPE_F16, torch.bfloat16: PS_DTYPE_BF16, torch.float32: PS_DTYPE_F32}
+_FORMATS = {"e4m3": (torch.float8_e4m3fn, PS_FP8_E4M3), "e5m2": (torch.float8_e5m2, PS_FP8_E5M2)}
+_FORMAT_OF = {dtype: code for dtype, code in _FORMATS.values()}
+_BLOCKS = {"row": PS_BLOCKS_ROW, "col": PS_BLOCKS_COL, "row+col": PS_BLOCKS_ROW_COL, "tile": PS_BLOCKS_TILE}
+
+
+def _stream_ptr(device):
+    return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def _scales_shape(outer, contracted):
+    return (-(-contracted // (4 * BLOCK)), -(-outer // BLOCK), 32, 4, 4)
+
+
+class BlockQuantized:
+    """A matrix [rows, cols] in 8-bit floating point with a scale for each block.
+
+    ``data``     float8_e4m3fn or float8_e5m2, rows a multiple of 16 bytes apart
+    ``blocks``   "row" (1 x 128), "col" (128 x 1) or "tile" (128 x 128)
+    ``scales1``  scale bytes for a contraction over dimension 1 ("row", "tile"), else None
+    ``scales0``  scale bytes for a contraction over dimension 0 ("col", "tile"), else None
+
+    A byte s stands for the scale 2^(s - 127).  For L contracted and O outer
+    elements the array is ``uint8[ceil(L / 512), ceil(O / 128), 32, 4, 4]`` and the
+    byte of outer element ``o`` and contracted block ``kb`` is at ``[kb // 4, o // 128,
+    o % 32, o % 128 // 32, kb % 4]``: the order in which the tensor core reads them.
+    """
+
+    __slots__ = ("data", "blocks", "scales1", "scales0")
+
+    def __init__(self, data, blocks, scales1=None, scales0=None):
+        if not isinstance(data, torch.Tensor) or data.dtype not in _FORMAT_OF:
+            raise TypeError("BlockQuantized needs float8_e4m3fn or float8_e5m2 values, got %s"
+                            % getattr(data, "dtype", type(data)))
+        if blocks not in ("row", "col", "tile"):
+            raise ValueError("blocks must be row, col or tile; got %r" % (blocks,))
+        if data.dim() != 2:
+            raise ValueError("BlockQuantized needs a matrix, got %d dimensions" % data.dim())
+        rows, cols = data.shape
+        if rows and cols:
+            if cols > 1 and data.stride(1) != 1:
+                raise ValueError("the values of a row must be adjacent")
+            if data.data_ptr() % 16 or (rows > 1 and (data.stride(0) % 16 or data.stride(0) < cols)):
+                raise ValueError("rows of values must start on 16-byte boundaries")
+        for name, scales, used, shape in (("scales1", scales1, blocks != "col", _scales_shape(rows, cols)),
+                                          ("scales0", scales0, blocks != "row", _scales_shape(cols, rows))):
+            if (scales is not None) != used:
+                raise ValueError("%s %s scales %s %s" % (blocks, "blocks need" if used else "blocks have no",
+                                                         "in", name))
+            if scales is None:
+                continue
+            if scales.dtype != torch.uint8 or tuple(scales.shape) != shape or not scales.is_contiguous():
+                raise ValueError("%s must be contiguous uint8 of shape %s; got %s of shape %s"
+                                 % (name, shape, scales.dtype, tuple(scales.shape)))
+            if scales.device != data.device:
+                raise ValueError("values on %s, %s on %s" % (data.device, name, scales.device))
+        self.data, self.blocks, self.scales1, self.scales0 = data, blocks, scales1, scales0
+
+    @classmethod
+    def _of(cls, data, blocks, scales1, scales0):
+        q = cls.__new__(cls)    # parts that this module allocated: nothing to check
+        q.data, q.blocks, q.scales1, q.scales0 = data, blocks, scales1, scales0
+        return q
+
+    @property
+    def shape(self):
+        return self.data.shape
+
+    @property
+    def device(self):
+        return self.data.device
+
+    @property
+    def dtype(self):
+        return self.data.dtype
+
+    def exponents(self):
+        """int32 exponents of the scales, one for each block: [rows, ceil(cols / 128)] for "row",
+        [ceil(rows / 128), cols] for "col", [ceil(rows / 128), ceil(cols / 128)] for "tile"."""
+        rows, cols = self.data.shape
+        s, outer, contracted = ((self.scales0, cols, rows) if self.blocks == "col" else (self.scales1, rows, cols))
+        groups, blocks = s.shape[:2]
+        flat = s.permute(1, 3, 2, 0, 4).reshape(blocks * BLOCK, groups * 4)[:outer, :-(-contracted // BLOCK)]
+        e = flat.to(torch.int32) - 127
+        return e.t() if self.blocks == "col" else e[::BLOCK] if self.blocks == "tile" else e
+
+    def dequantize(self, dtype=torch.float32):
+        """The values times their scales."""
+        rows, cols = self.data.shape
+        e = self.exponents()
+        if self.blocks != "row":
+            e = e.repeat_interleave(BLOCK, 0)[:rows]
+        if self.blocks != "col":
+            e = e.repeat_interleave(BLOCK, 1)[:, :cols]
+        return torch.ldexp(self.data.float(), e).to(dtype)
+
+    def _operand(self, dim):
+        scales = self.scales1 if dim else self.scales0
+        rows, cols = self.data.shape
+        ld = self.data.stride(0) if rows > 1 else -(-cols // 16) * 16
+        return BlockOperand(data=self.data.data_ptr(), scales=scales.data_ptr(), ld=ld,
+                            fmt=_FORMAT_OF[self.data.dtype], k_dim=dim)
+
+
+def _check_float(t, what):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in _DTYPES:
+        raise TypeError("%s must be a CUDA tensor of float16, bfloat16 or float32, got %s" % (
+            what, "%s on %s" % (t.dtype, t.device) if isinstance(t, torch.Tensor) else type(t).__name__))
+
+
+def _format(fmt):
+    if fmt not in _FORMATS:
+        raise ValueError("the format must be e4m3 or e5m2; got %r" % (fmt,))
+    return _FORMATS[fmt]
+
+
+def _quantize(x, blocks, fmt, sums=False):
+    """block_quantize for a checked matrix; with ``sums`` also the float32 column sums of each run of 128 rows."""
+    dtype, code = _FORMATS[fmt]
+    if x.stride(1) != 1 and x.shape[1] > 1:
+        x = x.contiguous()
+    rows, cols = x.shape
+    ldq = -(-cols // 16) * 16
+    dev = x.device
+    q1 = s1 = q0 = s0 = part = None
+    if blocks != "col":
+        q1 = torch.empty((rows, ldq), dtype=dtype, device=dev)
+        s1 = torch.empty(_scales_shape(rows, cols), dtype=torch.uint8, device=dev)
+    if blocks in ("col", "row+col"):
+        q0 = torch.empty((rows, ldq), dtype=dtype, device=dev)
+    if blocks != "row":
+        s0 = torch.empty(_scales_shape(cols, rows), dtype=torch.uint8, device=dev)
+    if sums:
+        part = torch.empty((-(-rows // BLOCK), cols), dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev):
+        check(lib.ps_block_quantize(
+            x.data_ptr(), _DTYPES[x.dtype], x.stride(0) if rows > 1 else cols, rows, cols, _BLOCKS[blocks], code,
+            q1.data_ptr() if q1 is not None else None, s1.data_ptr() if s1 is not None else None,
+            q0.data_ptr() if q0 is not None else None, s0.data_ptr() if s0 is not None else None, ldq,
+            part.data_ptr() if part is not None else None, _stream_ptr(dev)), "ps_block_quantize")
+    if cols != ldq:
+        q1 = q1 if q1 is None else q1[:, :cols]
+        q0 = q0 if q0 is None else q0[:, :cols]
+    if blocks == "tile":
+        return BlockQuantized._of(q1, "tile", s1, s0)
+    row = None if q1 is None else BlockQuantized._of(q1, "row", s1, None)
+    col = None if q0 is None else BlockQuantized._of(q0, "col", None, s0)
+    out = row if blocks == "row" else col if blocks == "col" else (row, col)
+    return (out, part) if sums else out
+
+
+def block_quantize(x, blocks="row", fmt="e4m3"):
+    """Quantizes the matrix ``x`` (CUDA, float16 / bfloat16 / float32) with a power-of-two scale for each block.
+
+    ``blocks``: "row" for 1 x 128 (to be contracted over dimension 1), "col" for 128 x 1 (over
+    dimension 0), "tile" for 128 x 128 (over either), "row+col" for a tuple of the first two
+    from one read.  The scale of a block is the smallest power of two that brings its largest
+    finite magnitude within the format's range (448 for ``fmt`` "e4m3", 57344 for "e5m2"), not
+    below 2^-126; values are rounded to nearest even.  Infinite and NaN elements become NaN in
+    e4m3 and stay themselves in e5m2.  No gradient flows through.
+    """
+    _check_float(x, "block_quantize: x")
+    if x.dim() != 2:
+        raise ValueError("block_quantize needs a matrix, got %d dimensions" % x.dim())
+    if blocks not in _BLOCKS:
+        raise ValueError("blocks must be row, col, row+col or tile; got %r" % (blocks,))
+    _format(fmt)
+    return _quantize(x.detach(), blocks, fmt)
+
+
+def _matmul(a, a_dim, b, b_dim, bias, out_dtype):
+    m, n, k = a.shape[1 - a_dim], b.shape[1 - b_dim], a.shape[a_dim]
+    out = torch.empty((m, n), dtype=out_dtype, device=a.device)
+    with torch.cuda.device(a.device):
+        check(lib.ps_block_matmul(
+            C.byref(a._operand(a_dim)), C.byref(b._operand(b_dim)), m, n, k,
+            bias.data_ptr() if bias is not None else None, _DTYPES[bias.dtype] if bias is not None else 0,
+            out.data_ptr(), _DTYPES[out_dtype], n, _stream_ptr(a.device)), "ps_block_matmul")
+    return out
+
+
+def _dim(q, dim, what):
+    if not isinstance(q, BlockQuantized):
+        raise TypeError("block_matmul: %s must be BlockQuantized, got %s" % (what, type(q).__name__))
+    if not q.data.is_cuda:
+        raise TypeError("block_matmul: %s must be on a CUDA device, got %s" % (what, q.device))
+    if dim is None:
+        dim = 0 if q.blocks == "col" else 1
+    if dim not in (0, 1) or (q.scales1 if dim else q.scales0) is None:
+        raise ValueError("block_matmul: %s has %s blocks: they cannot be contracted over dimension %r"
+                         % (what, q.blocks, dim))
+    return dim
+
+
+def block_matmul(a, b, a_dim=None, b_dim=None, bias=None, out_dtype=torch.float16):
+    """The product of two ``BlockQuantized`` matrices, contracted over dimension ``a_dim`` of ``a`` and
+    ``b_dim`` of ``b`` (each by default the one its blocks lie along; 1 for "tile" blocks).
+
+    Returns ``[outer size of a, outer size of b]`` in ``out_dtype`` (float16, bfloat16 or float32),
+    accumulated in 32 bits and rounded once, after ``bias`` (one value for each column) was added.
+    """
+    a_dim, b_dim = _dim(a, a_dim, "a"), _dim(b, b_dim, "b")
+    if a.device != b.device:
+        raise ValueError("block_matmul: a on %s, b on %s" % (a.device, b.device))
+    if a.shape[a_dim] != b.shape[b_dim]:
+        raise ValueError("block_matmul: contracted sizes differ: %d and %d" % (a.shape[a_dim], b.shape[b_dim]))
+    if out_dtype not in _DTYPES:
+        raise TypeError("block_matmul: out_dtype must be float16, bfloat16 or float32, got %s" % (out_dtype,))
+    if bias is not None:
+        _check_bias(bias, b.shape[1 - b_dim], a.device, "block_matmul")
+        bias = bias.detach().contiguous()
+    return _matmul(a, a_dim, b, b_dim, bias, out_dtype)
+
+
+def _check_bias(bias, n, device, where):
+    _check_float(bias, where + ": bias")
+    if tuple(bias.shape) != (n,):
+        raise ValueError("%s: bias must have shape (%d,), got %s" % (where, n, tuple(bias.shape)))
+    if bias.device != device:
+        raise ValueError("%s: bias on %s, the product on %s" % (where, bias.device, device))
+
+
+class _Fp8Linear(torch.autograd.Function):
+    """y = Q_row(x) Q_tile(w)^T + b;  dx = Q_row(dy) Q_tile(w);  dw = Q_col(dy)^T Q_col(x);  db = sum of dy."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, kept, grad_fmt):
+        x2 = x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
+        ctx.shape, ctx.grad_fmt = x.shape, grad_fmt
+        ctx.dtypes = (x.dtype, weight.dtype if weight is not None else None, bias.dtype if bias is not None else None)
+        xc = None
+        if ctx.needs_input_grad[1]:
+            xr, xc = _quantize(x2, "row+col", "e4m3")
+        else:
+            xr = _quantize(x2, "row", "e4m3")
+        w = kept if kept is not None else _quantize(weight, "tile", "e4m3")
+        wants_w = ctx.needs_input_grad[0]
+        ctx.save_for_backward(*(w.data, w.scales0) if wants_w else (None, None),
+                              *(xc.data, xc.scales0) if xc is not None else (None, None))
+        y = _matmul(xr, 1, w, 1, bias.contiguous() if bias is not None else None, x.dtype)
+        return y.view(x.shape[:-1] + (y.shape[1],))
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        wd, ws, xd, xs = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        x_dtype, w_dtype, b_dtype = ctx.dtypes
+        dx = dw = db = None
+        dy2 = dy.reshape(math.prod(dy.shape[:-1]), dy.shape[-1])
+        row = col = part = None
+        if need_b:
+            (row, col), part = _quantize(dy2, "row+col", ctx.grad_fmt, sums=True)
+        elif need_x and need_w:
+            row, col = _quantize(dy2, "row+col", ctx.grad_fmt)
+        elif need_x:
+            row = _quantize(dy2, "row", ctx.grad_fmt)
+        elif need_w:
+            col = _quantize(dy2, "col", ctx.grad_fmt)
+        if need_x:
+            dx = _matmul(row, 1, BlockQuantized._of(wd, "col", None, ws), 0, None, x_dtype).view(ctx.shape)
+        if need_w:
+            dw = _matmul(col, 0, BlockQuantized._of(xd, "col", None, xs), 0, None, w_dtype)
+        if need_b:
+            db = torch.empty(part.shape[1], dtype=b_dtype, device=part.device)
+            with torch.cuda.device(part.device):
+                check(lib.ps_column_sum(part.data_ptr(), part.shape[0], part.shape[1], db.data_ptr(), _DTYPES[b_dtype],
+                                        _stream_ptr(part.device)), "ps_column_sum")
+        return dx, dw, db, None, None
+
+
+def fp8_linear(x, weight, bias=None, grad_fmt="e4m3"):
+    """``x @ weight.T + bias`` on the 8-bit path; ``x`` [..., K], ``weight`` [N, K], ``bias`` [N].
+
+    ``x`` and ``weight`` are quantized to e4m3 within the call (1 x 128 and 128 x 128 blocks),
+    the incoming gradient in the backward pass to ``grad_fmt`` (1 x 128 and 128 x 1 blocks).
+    The result and the gradient of ``x`` have the type of ``x``, the gradients of ``weight`` and
+    ``bias`` theirs; the gradient of ``bias`` is summed from the unquantized gradient.  ``weight``
+    may also be a ``BlockQuantized`` with "tile" blocks, quantized once and kept; it has no
+    gradient then.  Between forward and backward the quantized ``x`` and ``weight`` are kept (one
+    byte an element), not the originals.
+    """
+    _check_float(x, "fp8_linear: x")
+    if x.dim() < 1:
+        raise ValueError("fp8_linear: x needs at least one dimension")
+    _format(grad_fmt)
+    kept = weight if isinstance(weight, BlockQuantized) else None
+    if kept is not None:
+        if kept.blocks != "tile":
+            raise ValueError("fp8_linear: a quantized weight needs tile blocks, got %s" % kept.blocks)
+    else:
+        _check_float(weight, "fp8_linear: weight")
+        if weight.dim() != 2:
+            raise ValueError("fp8_linear: weight must be a matrix, got %d dimensions" % weight.dim())
+    if weight.shape[1] != x.shape[-1]:
+        raise ValueError("fp8_linear: x has %d features, weight takes %d" % (x.shape[-1], weight.shape[1]))
+    if weight.device != x.device:
+        raise ValueError("fp8_linear: x on %s, weight on %s" % (x.device, weight.device))
+    if bias is not None:
+        _check_bias(bias, weight.shape[0], x.device, "fp8_linear")
+    return _Fp8Linear.apply(x, None if kept is not None else weight, bias, kept, grad_fmt)
+
+
+class Fp8Linear(torch.nn.Linear):
+    """``torch.nn.Linear`` whose products run through ``fp8_linear``; same parameters and state."""
+
+    grad_fmt = "e4m3"
+
+    def forward(self, x):
+        return fp8_linear(x, self.weight, self.bias, self.grad_fmt)
+
+    def extra_repr(self):
+        return super().extra_repr() + ", grad_fmt=%s" % self.grad_fmt
+
+
+def use_fp8_linears(module, grad_fmt="e4m3"):
+    """Makes every ``torch.nn.Linear`` of ``module`` (itself included; not subclasses) an ``Fp8Linear`` in
+    place: parameters, buffers, hooks and names stay.  Returns the number of layers changed."""
+    _format(grad_fmt)
+    n = 0
+    for m in module.modules():
+        if type(m) is torch.nn.Linear:
+            m.__class__ = Fp8Linear
+            m.grad_fmt = grad_fmt
+            n += 1
+    return n

@@ -1,7 +1,7 @@
 """In-tree build of the CUDA library: ``python -m patrickstar_b200.build``.
 
-One translation unit, nvcc, sm_100a only.  The output ``libps_b200.so`` sits
-beside the package so that it is found without installation.
+nvcc, sm_100a only.  The output ``libps_b200.so`` sits beside the package so
+that it is found without installation.
 """
 import os
 import subprocess
@@ -9,12 +9,14 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
-SOURCES = [os.path.join(HERE, "csrc", "ps_kernels.cu"), os.path.join(HERE, "csrc", "ps_offload.cu")]
-HEADER = os.path.join(ROOT, "include", "ps_b200.h")
+SOURCES = [os.path.join(HERE, "csrc", name) for name in (
+    "ps_kernels.cu", "ps_offload.cu", "ps_block_quantize.cu", "ps_block_matmul.cu")]
+HEADERS = [os.path.join(ROOT, "include", "ps_b200.h"), os.path.join(HERE, "csrc", "ps_internal.h"),
+           os.path.join(HERE, "csrc", "ps_tensor_core.cuh")]
 OUT = os.path.join(HERE, "libps_b200.so")
 
 NVCC_FLAGS = [
-    "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
+    "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "--threads", "0",
     # IEEE arithmetic on both sides: no fast-math on the device, no contraction on the host
     "-Xcompiler", "-fPIC,-ffp-contract=off", "-shared",
 ]
@@ -28,7 +30,7 @@ def _nvcc():
 
 def build(force=False, verbose=False):
     srcs = [s for s in SOURCES if os.path.exists(s)]
-    deps = srcs + [HEADER]
+    deps = srcs + HEADERS
     if not force and os.path.exists(OUT) and all(os.path.getmtime(OUT) >= os.path.getmtime(d) for d in deps):
         return OUT
     cmd = [_nvcc()] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + [

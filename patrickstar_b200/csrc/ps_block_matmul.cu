@@ -1,0 +1,374 @@
+// Product of two matrices held in 8-bit floating point with a power-of-two scale
+// for each block of 128 along the contracted dimension:
+//
+//   out[i, j] = sum_k a(i, k) 2^ea(i, k / 128) b(j, k) 2^eb(j, k / 128)  (+ bias[j])
+//
+// accumulated in 32 bits and rounded once to the output's type.  The scales are
+// powers of two, so the tensor core applies them itself (kind::mxf8f6f4: one
+// scale byte for 32 consecutive k; the four 32s of a block select the same
+// byte), and nothing between the first product and the output touches the
+// accumulator.
+//
+// Either operand may have the contracted dimension or the outer one contiguous
+// (the instruction descriptor's transpose bits): the weight that the forward
+// product reads is read as it lies by the input-gradient product, and the
+// weight gradient contracts over the rows of both operands.  Both forms use the
+// same 128 x 128-byte box with the 128-byte swizzle, with the coordinates
+// swapped.
+#include "ps_b200.h"
+
+#include "ps_internal.h"
+#include "ps_tensor_core.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstring>
+
+namespace {
+
+constexpr uint32_t kTile = 128;                   // rows of A, rows of B and k of one box
+constexpr uint32_t kBoxBytes = kTile * kTile;     // 16 KB
+constexpr uint32_t kScaleBytes = 512;             // scales of 128 outer elements, four k blocks
+
+__device__ unsigned int g_gave_up;  // CTAs that ran into the limit of a wait
+
+struct ProductArgs {
+    const void* bias;
+    void* out;
+    uint64_t ldo;
+    uint32_t m, n, n_kb;
+    uint32_t tiles_m, tiles_n;
+    uint32_t scale_blocks_a, scale_blocks_b;
+    uint32_t idesc;
+    int a_k_inner, b_k_inner;  // the contracted dimension is the contiguous one
+    int bias_dtype, out_dtype;
+    int vec;                   // output rows start on 16-byte boundaries
+};
+
+__device__ __forceinline__ float bias_at(const ProductArgs& p, uint32_t col)
+{
+    if (p.bias_dtype == PS_DTYPE_F16) return __half2float(reinterpret_cast<const __half*>(p.bias)[col]);
+    if (p.bias_dtype == PS_DTYPE_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.bias)[col]);
+    return reinterpret_cast<const float*>(p.bias)[col];
+}
+__device__ __forceinline__ uint32_t pack2(int dtype, float lo, float hi)
+{
+    if (dtype == PS_DTYPE_F16) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void store1(const ProductArgs& p, uint64_t at, float v)
+{
+    if (p.out_dtype == PS_DTYPE_F16)
+        reinterpret_cast<__half*>(p.out)[at] = __float2half_rn(v);
+    else if (p.out_dtype == PS_DTYPE_BF16)
+        reinterpret_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
+    else
+        reinterpret_cast<float*>(p.out)[at] = v;
+}
+
+// Shared-memory descriptor of the box at `addr`: k contiguous (8-row groups 1024 bytes apart), or the outer
+// dimension contiguous (groups of 8 k 1024 bytes apart).  The next 32 k are 32 bytes resp. 32 rows on.
+__device__ __forceinline__ uint64_t box_desc(uint32_t addr)
+{
+    return tc::matrix_desc(addr, 1024, 1024, tc::kSwizzle128);
+}
+__device__ __forceinline__ uint64_t scale_desc(uint32_t addr)
+{
+    return tc::matrix_desc(addr, 128, 128, tc::kSwizzleNone);
+}
+
+// ---------------------------------------------------------------------------
+// One 128 x 128 tile a cluster: its CTAs share the k blocks, and join their
+// partial sums over distributed shared memory in the order of their ranks.
+// ---------------------------------------------------------------------------
+constexpr int kSplitStages = 3;
+constexpr uint32_t kSplitStageBytes = 2 * kBoxBytes + 2 * kScaleBytes;
+constexpr uint32_t kSplitThreads = 192;  // warps 0-3 epilogue, 4 loads, 5 tensor core
+constexpr uint32_t kPartialPitch = 132;  // floats; 16-byte accesses of 8 rows fall into different banks
+constexpr uint32_t kSplitSmem = 1024 + kSplitStages * kSplitStageBytes;
+constexpr uint32_t kSplitColumns = 256;  // accumulator 128, scales behind it
+static_assert(kTile * kPartialPitch * 4 <= kSplitStages * kSplitStageBytes, "the partial tile lies over the stages");
+
+__global__ void __launch_bounds__(kSplitThreads)
+block_matmul_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                          const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_sb,
+                          const __grid_constant__ ProductArgs p, const uint32_t splits)
+{
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ uint64_t full[kSplitStages], empty[kSplitStages], done;
+    __shared__ uint32_t tmem_base;
+    __shared__ volatile int gave_up;
+
+    const uint32_t base = (tc::smem_u32(smem_raw) + 1023u) & ~1023u;
+    unsigned char* const base_ptr = smem_raw + (base - tc::smem_u32(smem_raw));
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = blockIdx.x % splits, tile = blockIdx.x / splits;
+    const uint32_t tm = tile % p.tiles_m, tn = tile / p.tiles_m;
+    const uint32_t kb0 = (uint32_t)((uint64_t)p.n_kb * rank / splits);
+    const uint32_t kb1 = (uint32_t)((uint64_t)p.n_kb * (rank + 1) / splits);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kSplitStages; ++s) tc::bar_init(&full[s], 1), tc::bar_init(&empty[s], 1);
+        tc::bar_init(&done, 1);
+        gave_up = 0;
+        tc::bar_init_fence();
+    }
+    if (warp == 5) tc::tmem_alloc<1>(&tmem_base, kSplitColumns);
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = tmem_base;
+
+    if (warp == 4 && lane == 0) {
+        uint32_t issued = 0;
+        for (uint32_t kb = kb0; kb < kb1; ++kb, ++issued) {
+            const uint32_t s = issued % kSplitStages, round = issued / kSplitStages;
+            if (round > 0 && !tc::bar_wait(&empty[s], (round - 1) & 1, &gave_up)) break;
+            const bool scales = kb == kb0 || (kb & 3) == 0;
+            const uint32_t at = base + s * kSplitStageBytes;
+            tc::bar_expect(&full[s], 2 * kBoxBytes + (scales ? 2 * kScaleBytes : 0));
+            const int k = (int)(kb * kTile), i = (int)(tm * kTile), j = (int)(tn * kTile);
+            tc::load_box(&map_a, at, &full[s], p.a_k_inner ? k : i, p.a_k_inner ? i : k);
+            tc::load_box(&map_b, at + kBoxBytes, &full[s], p.b_k_inner ? k : j, p.b_k_inner ? j : k);
+            if (scales) {
+                tc::load_box(&map_sa, at + 2 * kBoxBytes, &full[s], 0, (int)((kb >> 2) * p.scale_blocks_a + tm));
+                tc::load_box(&map_sb, at + 2 * kBoxBytes + kScaleBytes, &full[s], 0,
+                             (int)((kb >> 2) * p.scale_blocks_b + tn));
+            }
+        }
+        if (gave_up) {
+            // copies may still be landing in this CTA's memory: the stages in flight, each waited for with the
+            // same limit
+            int ignore = 0;
+            for (uint32_t i = issued < kSplitStages ? 0 : issued - kSplitStages; i < issued; ++i)
+                tc::bar_wait(&full[i % kSplitStages], (i / kSplitStages) & 1, &ignore);
+        }
+    } else if (warp == 5 && lane == 0) {
+        const uint32_t a_step = p.a_k_inner ? 32 : 32 * kTile, b_step = p.b_k_inner ? 32 : 32 * kTile;
+        uint32_t used = 0, groups = 0;
+        for (uint32_t kb = kb0; kb < kb1; ++kb, ++used) {
+            const uint32_t s = used % kSplitStages;
+            if (!tc::bar_wait(&full[s], (used / kSplitStages) & 1, &gave_up)) break;
+            tc::fence_after();
+            const uint32_t at = base + s * kSplitStageBytes;
+            if (kb == kb0 || (kb & 3) == 0) {
+                ++groups;
+                const uint32_t sf = tmem + kTile + (groups & 1) * 8;
+                tc::scale_copy<1>(sf, scale_desc(at + 2 * kBoxBytes));
+                tc::scale_copy<1>(sf + 4, scale_desc(at + 2 * kBoxBytes + kScaleBytes));
+            }
+            const uint32_t sf = tmem + kTile + (groups & 1) * 8;
+            const uint32_t idesc = tc::mx_idesc_select(p.idesc, kb & 3);
+#pragma unroll
+            for (uint32_t q = 0; q < 4; ++q)
+                tc::mx_mma<1>(tmem, box_desc(at + q * a_step), box_desc(at + kBoxBytes + q * b_step), idesc, sf, sf + 4,
+                              used > 0 || q > 0);
+            tc::mma_commit<1>(&empty[s]);
+        }
+        tc::mma_commit<1>(&done);
+        if (gave_up) {
+            int ignore = 0;
+            tc::bar_wait(&done, 0, &ignore);
+        }
+    } else if (warp < 4) {
+        // this CTA's partial tile into shared memory, over the stages (all of them are read by now)
+        const bool ok = tc::bar_wait(&done, 0, &gave_up);
+        tc::fence_after();
+        float* row = reinterpret_cast<float*>(base_ptr) + (size_t)(warp * 32 + lane) * kPartialPitch;
+        const bool good = ok && !gave_up;
+        for (uint32_t c = 0; c < kTile; c += 32) {
+            uint32_t v[32];
+            if (kb0 < kb1) {
+                tc::tmem_ld32(tmem + (warp << 21) + c, v);
+                tc::tmem_ld_wait();
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float4 f = make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]),
+                                       __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
+                if (kb0 >= kb1) f = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (!good) f.x = f.y = f.z = f.w = __int_as_float(0x7fffffff);
+                *reinterpret_cast<float4*>(row + c + 4 * i) = f;
+            }
+        }
+        tc::fence_before();
+    }
+
+    __syncthreads();
+    if (warp == 5) tc::tmem_free<1>(tmem, kSplitColumns);
+    if (splits > 1) tc::cluster_sync();
+
+    // rows [lo, hi) of the tile: the sum of the partial tiles, one row a warp
+    const uint32_t lo = rank * kTile / splits, hi = (rank + 1) * kTile / splits;
+    for (uint32_t r = lo + warp; r < hi; r += kSplitThreads / 32) {
+        const uint32_t i = tm * kTile + r, j = tn * kTile + lane * 4;
+        if (i >= p.m) break;
+        const uint32_t at = base + (r * kPartialPitch + lane * 4) * 4;
+        float4 t = tc::ld_cluster_f4(at, 0);
+        for (uint32_t s = 1; s < splits; ++s) {
+            const float4 u = tc::ld_cluster_f4(at, s);
+            t.x += u.x, t.y += u.y, t.z += u.z, t.w += u.w;
+        }
+        if (p.bias != nullptr) {
+            if (j < p.n) t.x += bias_at(p, j);
+            if (j + 1 < p.n) t.y += bias_at(p, j + 1);
+            if (j + 2 < p.n) t.z += bias_at(p, j + 2);
+            if (j + 3 < p.n) t.w += bias_at(p, j + 3);
+        }
+        const uint64_t o = (uint64_t)i * p.ldo + j;
+        if (p.vec && j + 4 <= p.n) {
+            if (p.out_dtype == PS_DTYPE_F32)
+                *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + o) = t;
+            else
+                *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.out) + o) =
+                    make_uint2(pack2(p.out_dtype, t.x, t.y), pack2(p.out_dtype, t.z, t.w));
+        } else {
+            const float f[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (j + q < p.n) store1(p, o + q, f[q]);
+        }
+    }
+    if (splits > 1) tc::cluster_sync();  // no CTA leaves while its partial tile is read
+    if (threadIdx.x == 0 && gave_up) atomicAdd(&g_gave_up, 1u);
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encoder()
+{
+    static const EncodeTiled fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &q);
+        if (e != cudaSuccess || q != cudaDriverEntryPointSuccess) {
+            ps_internal::set_cuda_error((int)e);
+            cudaGetLastError();
+            f = nullptr;
+        }
+        return (EncodeTiled)f;
+    }();
+    return fn;
+}
+
+int encode(CUtensorMap* m, CUtensorMapDataType type, const void* p, uint64_t inner, uint64_t rows, uint64_t row_bytes,
+           uint32_t box_inner, uint32_t box_rows, CUtensorMapSwizzle swizzle)
+{
+    const EncodeTiled fn = encoder();
+    if (fn == nullptr) return PS_ERR_CUDA;
+    const cuuint64_t dims[2] = {inner, rows}, strides[1] = {row_bytes};
+    const cuuint32_t box[2] = {box_inner, box_rows}, step[2] = {1, 1};
+    const CUresult r = fn(m, type, 2, const_cast<void*>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? PS_OK : PS_ERR_INVALID;
+}
+
+int check_operand(const ps_block_operand* o, uint64_t outer, uint64_t k)
+{
+    if (o == nullptr || o->data == nullptr || o->scales == nullptr) return PS_ERR_INVALID;
+    if (o->fmt != PS_FP8_E4M3 && o->fmt != PS_FP8_E5M2) return PS_ERR_INVALID;
+    if (o->k_dim != 0 && o->k_dim != 1) return PS_ERR_INVALID;
+    if (o->ld < (o->k_dim ? k : outer)) return PS_ERR_INVALID;
+    if (o->ld % 16 || (uintptr_t)o->data % 16 || (uintptr_t)o->scales % 16) return PS_ERR_ALIGN;
+    return PS_OK;
+}
+
+int encode_operand(const ps_block_operand* o, uint64_t outer, uint64_t k, uint32_t blocks, CUtensorMap* data,
+                   CUtensorMap* scales)
+{
+    int rc = encode(data, CU_TENSOR_MAP_DATA_TYPE_UINT8, o->data, o->k_dim ? k : outer, o->k_dim ? outer : k, o->ld,
+                    kTile, kTile, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc != PS_OK) return rc;
+    return encode(scales, CU_TENSOR_MAP_DATA_TYPE_INT32, o->scales, kScaleBytes / 4, (uint64_t)((k + 511) / 512) * blocks,
+                  kScaleBytes, kScaleBytes / 4, 1, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
+
+}  // namespace
+
+extern "C" {
+
+int ps_block_matmul(const ps_block_operand* a, const ps_block_operand* b, uint32_t m, uint32_t n, uint32_t k,
+                    const void* bias_dev, int bias_dtype, void* out_dev, int out_dtype, uint64_t ldo, void* stream)
+{
+    if (out_dtype < PS_DTYPE_F16 || out_dtype > PS_DTYPE_F32) return PS_ERR_INVALID;
+    if (bias_dev != nullptr && (bias_dtype < PS_DTYPE_F16 || bias_dtype > PS_DTYPE_F32)) return PS_ERR_INVALID;
+    if (m == 0 || n == 0) return PS_OK;
+    if (out_dev == nullptr || ldo < n) return PS_ERR_INVALID;
+    if (m > 0x7fffff00u || n > 0x7fffff00u || k > 0x7fffff00u) return PS_ERR_LIMIT;
+    const uint64_t osize = out_dtype == PS_DTYPE_F32 ? 4 : 2;
+    if ((uintptr_t)out_dev % osize) return PS_ERR_ALIGN;
+    ProductArgs p;
+    memset(&p, 0, sizeof(p));
+    CUtensorMap maps[4];
+    memset(maps, 0, sizeof(maps));
+    p.scale_blocks_a = ceil_div(m, kTile), p.scale_blocks_b = ceil_div(n, kTile);
+    if (k > 0) {
+        int rc = check_operand(a, m, k);
+        if (rc == PS_OK) rc = check_operand(b, n, k);
+        if (rc != PS_OK) return rc;
+        if ((uint64_t)ceil_div(k, 512) * (p.scale_blocks_a > p.scale_blocks_b ? p.scale_blocks_a : p.scale_blocks_b) >
+            0x7fffffffull)
+            return PS_ERR_LIMIT;
+        rc = encode_operand(a, m, k, p.scale_blocks_a, &maps[0], &maps[2]);
+        if (rc == PS_OK) rc = encode_operand(b, n, k, p.scale_blocks_b, &maps[1], &maps[3]);
+        if (rc != PS_OK) return rc;
+        p.a_k_inner = a->k_dim, p.b_k_inner = b->k_dim;
+    }
+    p.bias = bias_dev, p.bias_dtype = bias_dtype, p.out = out_dev, p.out_dtype = out_dtype, p.ldo = ldo;
+    p.m = m, p.n = n, p.n_kb = ceil_div(k, kTile);
+    p.vec = (uintptr_t)out_dev % 16 == 0 && (ldo * osize) % 16 == 0;
+    const int sms = ps_internal::sm_count();
+    if (sms < 0) return sms;
+
+    p.tiles_m = ceil_div(m, kTile), p.tiles_n = ceil_div(n, kTile);
+    if (k > 0) p.idesc = tc::mx_idesc(128, 128, a->fmt, b->fmt, !a->k_dim, !b->k_dim);
+    const uint64_t tiles = (uint64_t)p.tiles_m * p.tiles_n;
+    uint32_t splits = 1;
+    while (splits < 8 && tiles * splits < (uint64_t)sms && splits * 4 <= p.n_kb) splits *= 2;
+    if (tiles * splits > 0x7fffffffull) return PS_ERR_LIMIT;
+    static const cudaError_t attr =
+        cudaFuncSetAttribute(block_matmul_split_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSplitSmem);
+    if (attr != cudaSuccess) {
+        ps_internal::set_cuda_error((int)attr);
+        return PS_ERR_CUDA;
+    }
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3((uint32_t)(tiles * splits));
+    cfg.blockDim = dim3(kSplitThreads);
+    cfg.dynamicSmemBytes = kSplitSmem;
+    cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = splits, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, block_matmul_split_kernel, maps[0], maps[1], maps[2], maps[3], p, splits);
+    return ps_internal::after_launch();
+}
+
+int ps_block_matmul_gave_up(uint32_t* count)
+{
+    if (count == nullptr) return PS_ERR_INVALID;
+    const cudaError_t e = cudaMemcpyFromSymbol(count, g_gave_up, sizeof(*count));
+    if (e != cudaSuccess) {
+        ps_internal::set_cuda_error((int)e);
+        cudaGetLastError();
+        return PS_ERR_CUDA;
+    }
+    return PS_OK;
+}
+
+}  // extern "C"

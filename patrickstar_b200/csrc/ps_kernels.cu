@@ -13,6 +13,8 @@
 // core work.
 #include "ps_b200.h"
 
+#include "ps_internal.h"
+
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -1631,6 +1633,17 @@ int static_scratch_address(unsigned char** out)
 }
 
 }  // namespace
+
+namespace ps_internal {
+void set_cuda_error(int e) { g_last_cuda_error = e; }
+int after_launch() { return ::after_launch(); }
+int sm_count()
+{
+    DeviceInfo info;
+    const int rc = device_info(&info);
+    return rc == PS_OK ? info.sm_count : rc;
+}
+}  // namespace ps_internal
 
 // ---------------------------------------------------------------------------
 // C ABI
