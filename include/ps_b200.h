@@ -556,6 +556,64 @@ int ps_block_matmul(const ps_block_operand* a, const ps_block_operand* b, uint32
  * is NaN.  0 unless the GPU is being held by something else.  Synchronises. */
 int ps_block_matmul_gave_up(uint32_t* count);
 
+/* ---------------------------------------------------------------------------
+ * Distillation from a teacher's top entries.  No counterpart in the reference.
+ *
+ * For a row z of student logits, q = softmax(z / temperature) over the
+ * vocabulary; the teacher gives k entries (index, value):
+ *   PS_TAIL_DROP    p = softmax(value / temperature) over the listed entries
+ *                   (values: logits or log-probabilities)
+ *   PS_TAIL_BUCKET  p = exp(value) (values: log-probabilities at this temperature), and the
+ *                   rest p_r = max(0, 1 - sum p) against q_r, the student's mass outside of
+ *                   the listed indices (no rest where every index is listed)
+ *   row loss = weight temperature^2 (sum_j p_j (log p_j - log q_idx_j) + p_r (log p_r - log q_r))
+ * An index of -1 lists nothing; any other index outside of the vocabulary makes
+ * the row's loss and gradient NaN.  The same index may be listed more than once.
+ * An entry of probability 0 adds nothing; a row that lists nothing has loss 0
+ * and gradient 0.
+ * Rows whose mask byte is 0 have loss 0 and gradient 0 and are not read.
+ * ------------------------------------------------------------------------- */
+#define PS_TAIL_DROP 0
+#define PS_TAIL_BUCKET 1
+
+#define PS_REDUCE_NONE 0
+#define PS_REDUCE_SUM 1
+#define PS_REDUCE_MEAN 2 /* over the rows that the mask keeps, or 1 if it keeps none */
+
+#define PS_DISTILL_MAX_VOCAB (1u << 20)
+#define PS_DISTILL_MAX_K 1024
+
+typedef struct ps_distill_problem {
+    const void* logits;  /* [rows, vocab], dtype; row stride in elements, any alignment of the type */
+    const void* indices; /* [rows, k], int32 or int64 */
+    const void* teacher; /* [rows, k], teacher_dtype */
+    const void* mask;    /* uint8 [rows], or NULL: all rows */
+    uint64_t ld_logits, ld_indices, ld_teacher;
+    uint32_t rows, vocab, k;
+    int32_t dtype, index_bytes, teacher_dtype, tail, reduction;
+    float temperature, weight;
+} ps_distill_problem;
+
+/* Losses of the rows (row_loss, float [rows]) and, unless reduction is NONE,
+ * their sum or mean (loss).  stats: float [rows][4], 16-byte aligned, what the
+ * backward call needs.  inv_n: one float, written; needed for MEAN with a mask.
+ *
+ * With grad != NULL (reduction SUM or MEAN) the gradient of loss * scale with
+ * respect to the logits is written as well (same dtype, row stride ld_grad;
+ * elements behind the vocabulary are left as they were), scale being the
+ * scaler's current one, which is left in used_scale (one float). */
+int ps_distill_forward(const ps_distill_problem* problem, float* loss_dev, float* row_loss_dev, void* stats_dev,
+                       float* inv_n_dev, const ps_scaler_state* scaler_dev, void* grad_dev, uint64_t ld_grad,
+                       float* used_scale_dev, void* stream);
+
+/* Gradient of the loss times grad_out: one float (stride 0), or with reduction
+ * NONE one for each row.  With used_scale != NULL, grad holds the gradient that
+ * the forward call wrote for that scale, and the call leaves it when grad_out
+ * equals it; the result is the same bits either way. */
+int ps_distill_backward(const ps_distill_problem* problem, const void* stats_dev, const float* inv_n_dev,
+                        const float* grad_out_dev, uint32_t grad_out_stride, const float* used_scale_dev,
+                        void* grad_dev, uint64_t ld_grad, void* stream);
+
 /* Tuning knobs for measurements: "unroll" (1, 2, 4: 128-bit groups per thread
  * per tile of the step kernels), "scan_unroll" (1, 2, 4), "blocks_per_sm"
  * (0 = occupancy calculator), "bulk" (0, or 2..4 stages of the bulk-async

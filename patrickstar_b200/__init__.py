@@ -8,6 +8,7 @@ Public names mirror the reference's for this path:
 Operators of the training step around it, which the reference leaves to torch:
 
     from patrickstar_b200 import fp8_linear, Fp8Linear, block_quantize, block_matmul
+    from patrickstar_b200 import distillation_loss, DistillationLoss
 
 Everything that computes goes through ``libps_b200.so`` (hand-written sm_100a
 CUDA behind a C ABI, ``include/ps_b200.h``).  There is no CPU or PyTorch
@@ -30,6 +31,8 @@ _LAZY = {
     "fp8_linear": ("block_fp8", "fp8_linear"),
     "Fp8Linear": ("block_fp8", "Fp8Linear"),
     "use_fp8_linears": ("block_fp8", "use_fp8_linears"),
+    "distillation_loss": ("distill_loss", "distillation_loss"),
+    "DistillationLoss": ("distill_loss", "DistillationLoss"),
 }
 
 

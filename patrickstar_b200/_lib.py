@@ -23,6 +23,9 @@ PS_ERR_LIMIT = -6
 
 PS_DTYPE_F16, PS_DTYPE_BF16, PS_DTYPE_F32 = 0, 1, 2
 PS_FP8_E4M3, PS_FP8_E5M2 = 0, 1
+PS_TAIL_DROP, PS_TAIL_BUCKET = 0, 1
+PS_REDUCE_NONE, PS_REDUCE_SUM, PS_REDUCE_MEAN = 0, 1, 2
+PS_DISTILL_MAX_VOCAB, PS_DISTILL_MAX_K = 1 << 20, 1024
 PS_BLOCKS_ROW, PS_BLOCKS_COL, PS_BLOCKS_ROW_COL, PS_BLOCKS_TILE = 0, 1, 2, 3
 
 PS_MAX_GROUPS = 15
@@ -91,7 +94,15 @@ class BlockOperand(C.Structure):
                 ("k_dim", C.c_int32)]
 
 
-assert C.sizeof(BlockOperand) == 32
+class DistillProblem(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("indices", C.c_void_p), ("teacher", C.c_void_p), ("mask", C.c_void_p),
+                ("ld_logits", C.c_uint64), ("ld_indices", C.c_uint64), ("ld_teacher", C.c_uint64),
+                ("rows", C.c_uint32), ("vocab", C.c_uint32), ("k", C.c_uint32), ("dtype", C.c_int32),
+                ("index_bytes", C.c_int32), ("teacher_dtype", C.c_int32), ("tail", C.c_int32),
+                ("reduction", C.c_int32), ("temperature", C.c_float), ("weight", C.c_float)]
+
+
+assert C.sizeof(BlockOperand) == 32 and C.sizeof(DistillProblem) == 96
 assert C.sizeof(StepPlan) == 512 and C.sizeof(ScalerState) == 64
 assert C.sizeof(HyperSlot) == 64 and C.sizeof(StepCtrl) == 48 + 64 * PS_MAX_SLOTS
 
@@ -147,6 +158,8 @@ SIGNATURES = {
     "ps_column_sum": (C.c_int, [_p, C.c_uint32, C.c_uint32, _p, C.c_int, _p]),
     "ps_block_matmul": (C.c_int, [C.POINTER(BlockOperand), C.POINTER(BlockOperand), C.c_uint32, C.c_uint32,
                                   C.c_uint32, _p, C.c_int, _p, C.c_int, C.c_uint64, _p]),
+    "ps_distill_forward": (C.c_int, [C.POINTER(DistillProblem), _p, _p, _p, _p, _p, _p, C.c_uint64, _p, _p]),
+    "ps_distill_backward": (C.c_int, [C.POINTER(DistillProblem), _p, _p, _p, C.c_uint32, _p, _p, C.c_uint64, _p]),
     "ps_block_matmul_gave_up": (C.c_int, [C.POINTER(C.c_uint32)]),
 }
 

@@ -246,22 +246,31 @@ def _check_bias(bias, n, device, where):
         raise ValueError("%s: bias on %s, the product on %s" % (where, bias.device, device))
 
 
+def _aligned(data):
+    """Values whose rows start on 16-byte boundaries: ``data``, or a copy where a saved tensor came back packed."""
+    if data.data_ptr() % 16 == 0 and (data.shape[0] < 2 or data.stride(0) % 16 == 0) and data.stride(1) == 1:
+        return data
+    out = torch.empty((data.shape[0], -(-data.shape[1] // 16) * 16), dtype=data.dtype, device=data.device)
+    out = out[:, :data.shape[1]]
+    out.view(torch.uint8).copy_(data.view(torch.uint8))
+    return out
+
+
 class _Fp8Linear(torch.autograd.Function):
     """y = Q_row(x) Q_tile(w)^T + b;  dx = Q_row(dy) Q_tile(w);  dw = Q_col(dy)^T Q_col(x);  db = sum of dy."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, kept, grad_fmt):
+    def forward(ctx, x, weight, bias, kept, grad_fmt, grads):
         x2 = x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
         ctx.shape, ctx.grad_fmt = x.shape, grad_fmt
         ctx.dtypes = (x.dtype, weight.dtype if weight is not None else None, bias.dtype if bias is not None else None)
         xc = None
-        if ctx.needs_input_grad[1]:
+        if grads and ctx.needs_input_grad[1]:
             xr, xc = _quantize(x2, "row+col", "e4m3")
         else:
             xr = _quantize(x2, "row", "e4m3")
         w = kept if kept is not None else _quantize(weight, "tile", "e4m3")
-        wants_w = ctx.needs_input_grad[0]
-        ctx.save_for_backward(*(w.data, w.scales0) if wants_w else (None, None),
+        ctx.save_for_backward(*(w.data, w.scales0) if ctx.needs_input_grad[0] else (None, None),
                               *(xc.data, xc.scales0) if xc is not None else (None, None))
         y = _matmul(xr, 1, w, 1, bias.contiguous() if bias is not None else None, x.dtype)
         return y.view(x.shape[:-1] + (y.shape[1],))
@@ -284,15 +293,15 @@ class _Fp8Linear(torch.autograd.Function):
         elif need_w:
             col = _quantize(dy2, "col", ctx.grad_fmt)
         if need_x:
-            dx = _matmul(row, 1, BlockQuantized._of(wd, "col", None, ws), 0, None, x_dtype).view(ctx.shape)
+            dx = _matmul(row, 1, BlockQuantized._of(_aligned(wd), "col", None, ws), 0, None, x_dtype).view(ctx.shape)
         if need_w:
-            dw = _matmul(col, 0, BlockQuantized._of(xd, "col", None, xs), 0, None, w_dtype)
+            dw = _matmul(col, 0, BlockQuantized._of(_aligned(xd), "col", None, xs), 0, None, w_dtype)
         if need_b:
             db = torch.empty(part.shape[1], dtype=b_dtype, device=part.device)
             with torch.cuda.device(part.device):
                 check(lib.ps_column_sum(part.data_ptr(), part.shape[0], part.shape[1], db.data_ptr(), _DTYPES[b_dtype],
                                         _stream_ptr(part.device)), "ps_column_sum")
-        return dx, dw, db, None, None
+        return dx, dw, db, None, None, None
 
 
 def fp8_linear(x, weight, bias=None, grad_fmt="e4m3"):
@@ -324,7 +333,8 @@ def fp8_linear(x, weight, bias=None, grad_fmt="e4m3"):
         raise ValueError("fp8_linear: x on %s, weight on %s" % (x.device, weight.device))
     if bias is not None:
         _check_bias(bias, weight.shape[0], x.device, "fp8_linear")
-    return _Fp8Linear.apply(x, None if kept is not None else weight, bias, kept, grad_fmt)
+    return _Fp8Linear.apply(x, None if kept is not None else weight, bias, kept, grad_fmt,
+                            torch.is_grad_enabled())
 
 
 class Fp8Linear(torch.nn.Linear):

@@ -26,11 +26,22 @@ the gather over NVSwitch multicast memory or peer mappings; ``"staged"`` /
 ``"copy"``: the pipelined two-kernel and copy-engine forms of the same exchange;
 ``"auto"`` (default): p2p for 2-3 ranks, multimem for more, nccl when symmetric
 memory cannot be set up.
+
+Two top-level keys are added for the operators around the step, both absent by
+default:
+  * ``fp8`` — ``{"enabled": True, "grad_format": "e4m3"}``: the model's
+    ``torch.nn.Linear`` layers run their three products in 8 bits
+    (``Fp8Linear``); parameters, gradients and the step stay as they are.
+    ``grad_format`` ("e4m3" or "e5m2") is what incoming gradients are quantized to.
+  * ``distillation`` — ``{"temperature": 1.0, "tail": "drop", "weight": 1.0}``:
+    the settings of ``ChunkStepEngine.distillation_loss``.
 """
 import torch
 
+from .block_fp8 import use_fp8_linears
 from .chunk_list import DEFAULT_CHUNK_SIZE
 from .client import ChunkClient
+from .distill_loss import distillation_loss
 from .fp16_adam import FP16Adam
 from .loss_scaler import DynamicLossScaler, LossScaler
 
@@ -40,12 +51,16 @@ _DEFAULT_OPTIM = {
 }
 
 
+_DEFAULT_DISTILLATION = {"temperature": 1.0, "tail": "drop", "weight": 1.0}
+
+
 def parse_config(config):
     """engine.py:53-105 as a pure function.  Returns a dict with optim_type,
     optim_params, scaler ("none" | ("static", scale) | ("dynamic", kwargs)),
-    gradient_clipping, default_chunk_size."""
+    gradient_clipping, default_chunk_size, fp8 (None | the gradients' format), distillation."""
     out = {"default_chunk_size": DEFAULT_CHUNK_SIZE, "gradient_clipping": -1, "scaler": "none",
            "fused_collectives": "auto"}
+    out["fp8"], out["distillation"] = None, dict(_DEFAULT_DISTILLATION)
     if config is None:
         out["optim_type"] = _DEFAULT_OPTIM["type"]
         out["optim_params"] = dict(_DEFAULT_OPTIM["params"])
@@ -81,6 +96,17 @@ def parse_config(config):
         raise ValueError("client.opts.fused_collectives must be auto, nccl, multimem, p2p, staged or copy; "
                          "got %r" % (mode,))
     out["fused_collectives"] = mode
+    fp8 = config.get("fp8") or {}
+    if fp8.get("enabled", False):
+        out["fp8"] = fp8.get("grad_format", "e4m3")
+        if out["fp8"] not in ("e4m3", "e5m2"):
+            raise ValueError("fp8.grad_format must be e4m3 or e5m2; got %r" % (out["fp8"],))
+    for key, val in (config.get("distillation") or {}).items():
+        if key not in _DEFAULT_DISTILLATION:
+            raise ValueError("distillation takes %s; got %r" % (", ".join(_DEFAULT_DISTILLATION), key))
+        out["distillation"][key] = val
+    if out["distillation"]["tail"] not in ("drop", "bucket"):
+        raise ValueError("distillation.tail must be drop or bucket; got %r" % (out["distillation"]["tail"],))
     return out
 
 
@@ -116,6 +142,9 @@ class ChunkStepEngine(torch.nn.Module):
         self.module = model
         self.client = client
         parsed = parse_config(config)
+        if parsed["fp8"] is not None:
+            use_fp8_linears(self.module, parsed["fp8"])
+        self._distillation = parsed["distillation"]
         self.loss_scaler = build_loss_scaler(parsed, client.device)
         self.gradient_clipping = parsed["gradient_clipping"]
         op = parsed["optim_params"]
@@ -142,6 +171,12 @@ class ChunkStepEngine(torch.nn.Module):
 
     def forward(self, *inputs, **kwargs):
         return self.module(*inputs, **kwargs)
+
+    def distillation_loss(self, logits, indices, teacher, mask=None, reduction="mean"):
+        """``distillation_loss`` with the config's settings and this engine's loss scaler: handed to
+        ``backward`` next, its gradient is written once, already scaled."""
+        return distillation_loss(logits, indices, teacher, mask=mask, reduction=reduction,
+                                 scaler=None if reduction == "none" else self.loss_scaler, **self._distillation)
 
     def backward(self, loss):
         """engine.py:206-224 + hook.py:212-216: scaled backward, per-parameter
