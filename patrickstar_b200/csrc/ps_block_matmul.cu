@@ -124,7 +124,7 @@ block_matmul_split_kernel(const __grid_constant__ CUtensorMap map_a, const __gri
     tc::fence_after();
     const uint32_t tmem = tmem_base;
 
-    if (warp == 4 && lane == 0) {
+    if (warp == 4 && tc::elect_one()) {
         uint32_t issued = 0;
         for (uint32_t kb = kb0; kb < kb1; ++kb, ++issued) {
             const uint32_t s = issued % kSplitStages, round = issued / kSplitStages;
@@ -148,7 +148,7 @@ block_matmul_split_kernel(const __grid_constant__ CUtensorMap map_a, const __gri
             for (uint32_t i = issued < kSplitStages ? 0 : issued - kSplitStages; i < issued; ++i)
                 tc::bar_wait(&full[i % kSplitStages], (i / kSplitStages) & 1, &ignore);
         }
-    } else if (warp == 5 && lane == 0) {
+    } else if (warp == 5 && tc::elect_one()) {
         const uint32_t a_step = p.a_k_inner ? 32 : 32 * kTile, b_step = p.b_k_inner ? 32 : 32 * kTile;
         uint32_t used = 0, groups = 0;
         for (uint32_t kb = kb0; kb < kb1; ++kb, ++used) {
@@ -199,6 +199,7 @@ block_matmul_split_kernel(const __grid_constant__ CUtensorMap map_a, const __gri
         tc::fence_before();
     }
 
+    __syncwarp();
     __syncthreads();
     if (warp == 5) tc::tmem_free<1>(tmem, kSplitColumns);
     if (splits > 1) tc::cluster_sync();
@@ -235,6 +236,246 @@ block_matmul_split_kernel(const __grid_constant__ CUtensorMap map_a, const __gri
         }
     }
     if (splits > 1) tc::cluster_sync();  // no CTA leaves while its partial tile is read
+    if (threadIdx.x == 0 && gave_up) atomicAdd(&g_gave_up, 1u);
+}
+
+// ---------------------------------------------------------------------------
+// 256 x 256 tiles, one after another on each pair of SMs: the pair's tensor
+// cores work as one (cta_group::2), each CTA holding 128 rows of A, 128 rows of
+// B and 128 rows of the accumulator.
+//
+// Two accumulators of 256 columns and the scales do not fit into 512 columns of
+// tensor memory, so the accumulators overlap in 32 columns: the epilogue reads
+// those first, and the next tile starts as soon as they are out.
+// ---------------------------------------------------------------------------
+constexpr uint32_t kPairTile = 256;
+constexpr int kPairStages = 5;
+constexpr uint32_t kPairStageBytes = 2 * kBoxBytes + 4 * kScaleBytes;  // scales: 1 of A, 2 of B, 1 unused
+constexpr uint32_t kPairThreads = 192;                                 // warps 0-3 epilogue, 4 loads, 5 tensor core
+constexpr uint32_t kStoreBytes = 32 * 128;                             // 32 rows of 128 bytes a warp
+constexpr uint32_t kPairSmem = 1024 + kPairStages * kPairStageBytes + 4 * 2 * kStoreBytes;
+constexpr uint32_t kAccStride = 224;
+constexpr uint32_t kScaleColumn = kAccStride + kPairTile;  // 480: twice 4 columns of A and 8 of B
+static_assert(kScaleColumn + 2 * 12 <= 512, "tensor memory");
+static_assert(kPairSmem <= 227 * 1024, "shared memory");
+static_assert(kPairStages >= 5 && kPairStageBytes % 1024 == 0, "scale columns, swizzled boxes");
+constexpr uint32_t kGroupRows = 8;  // tiles of A that are worked on together
+
+__device__ __forceinline__ void tile_at(const ProductArgs& p, uint32_t t, uint32_t* tm, uint32_t* tn)
+{
+    const uint32_t per = kGroupRows * p.tiles_n, g = t / per, r = t % per;
+    const uint32_t first = g * kGroupRows, rows = min(kGroupRows, p.tiles_m - first);
+    *tm = first + r % rows, *tn = r / rows;
+}
+
+// 128 bytes of an output row from the accumulator's values; kOut is its type.
+template <int kOut>
+__device__ __forceinline__ void stage_row(unsigned char* buf, uint32_t row, const ProductArgs& p, uint32_t col,
+                                          uint32_t tmem, bool good, bool* loaded, uint64_t* drained)
+{
+    constexpr uint32_t kCols = kOut == PS_DTYPE_F32 ? 32 : 64;
+    uint32_t v[kCols / 32][32];
+#pragma unroll
+    for (uint32_t h = 0; h < kCols / 32; ++h) tc::tmem_ld32(tmem + 32 * h, v[h]);
+    tc::tmem_ld_wait();
+    if (!*loaded) {
+        *loaded = true;
+        tc::fence_before();
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) tc::bar_arrive_at(drained, 0);
+    }
+#pragma unroll
+    for (uint32_t q = 0; q < 8; ++q) {  // 16 bytes each, swizzled as the store's map says
+        uint4 w;
+        if constexpr (kOut == PS_DTYPE_F32) {
+            float f[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                f[i] = __uint_as_float(v[0][4 * q + i]);
+                if (p.bias != nullptr && col + 4 * q + i < p.n) f[i] += bias_at(p, col + 4 * q + i);
+                if (!good) f[i] = __int_as_float(0x7fffffff);
+            }
+            w = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+        } else {
+            float f[8];
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+                f[i] = __uint_as_float(v[q / 4][8 * (q & 3) + i]);
+                if (p.bias != nullptr && col + 8 * q + i < p.n) f[i] += bias_at(p, col + 8 * q + i);
+                if (!good) f[i] = __int_as_float(0x7fffffff);
+            }
+            w = make_uint4(pack2(kOut, f[0], f[1]), pack2(kOut, f[2], f[3]), pack2(kOut, f[4], f[5]), pack2(kOut, f[6], f[7]));
+        }
+        *reinterpret_cast<uint4*>(buf + row * 128 + ((q ^ (row & 7)) << 4)) = w;
+    }
+}
+
+template <int kOut>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads)
+block_matmul_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                         const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_sb,
+                         const __grid_constant__ CUtensorMap map_out, const __grid_constant__ ProductArgs p)
+{
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ uint64_t full[kPairStages], empty[kPairStages], done, drained, ended;
+    __shared__ uint32_t tmem_base;
+    __shared__ volatile int gave_up;
+
+    const uint32_t base = (tc::smem_u32(smem_raw) + 1023u) & ~1023u;
+    unsigned char* const base_ptr = smem_raw + (base - tc::smem_u32(smem_raw));
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = tc::cluster_rank();
+    const uint32_t tiles = p.tiles_m * p.tiles_n, first = blockIdx.x / 2, step = gridDim.x / 2;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kPairStages; ++s) tc::bar_init(&full[s], 1), tc::bar_init(&empty[s], 1);
+        tc::bar_init(&done, 1);
+        tc::bar_init(&drained, 8);  // the four epilogue warps of both CTAs
+        tc::bar_init(&ended, 1);
+        gave_up = 0;
+        tc::bar_init_fence();
+    }
+    if (warp == 5) tc::tmem_alloc<2>(&tmem_base, 512);
+    tc::fence_before();
+    __syncthreads();
+    tc::cluster_sync();
+    tc::fence_after();
+    const uint32_t tmem = tmem_base;
+
+    if (warp == 4 && tc::elect_one()) {
+        uint32_t issued = 0;
+        bool ok = true;
+        for (uint32_t t = first; t < tiles && ok; t += step) {
+            uint32_t tm, tn;
+            tile_at(p, t, &tm, &tn);
+            const int i = (int)(tm * kPairTile + rank * kTile), j = (int)(tn * kPairTile + rank * kTile);
+            for (uint32_t kb = 0; kb < p.n_kb; ++kb, ++issued) {
+                const uint32_t s = issued % kPairStages, round = issued / kPairStages;
+                if (round > 0 && !tc::bar_wait(&empty[s], (round - 1) & 1, &gave_up)) {
+                    ok = false;
+                    break;
+                }
+                const bool scales = (kb & 3) == 0;
+                const uint32_t at = base + s * kPairStageBytes;
+                if (rank == 0) tc::bar_expect(&full[s], 2 * (2 * kBoxBytes + (scales ? 3 * kScaleBytes : 0)));
+                const uint32_t bar = tc::cluster_addr(&full[s], 0);
+                const int k = (int)(kb * kTile);
+                tc::load_box_pair(&map_a, at, bar, p.a_k_inner ? k : i, p.a_k_inner ? i : k);
+                tc::load_box_pair(&map_b, at + kBoxBytes, bar, p.b_k_inner ? k : j, p.b_k_inner ? j : k);
+                if (scales) {
+                    // of A those of this CTA's rows, of B those of both CTAs'
+                    const uint32_t sf = at + 2 * kBoxBytes;
+                    tc::load_box_pair(&map_sa, sf, bar, 0, (int)((kb >> 2) * p.scale_blocks_a + 2 * tm + rank));
+                    const int y = (int)((kb >> 2) * p.scale_blocks_b + 2 * tn);
+                    tc::load_box_pair(&map_sb, sf + kScaleBytes, bar, 0, y);
+                    tc::load_box_pair(&map_sb, sf + 2 * kScaleBytes, bar, 0, y + 1);
+                }
+            }
+        }
+        if (gave_up && rank == 0) {
+            // copies may still be landing: the stages in flight, each waited for with the same limit (the barriers
+            // of both CTAs' copies are this CTA's; the other stays until the cluster's barrier below)
+            int ignore = 0;
+            for (uint32_t i = issued < kPairStages ? 0 : issued - kPairStages; i < issued; ++i)
+                tc::bar_wait(&full[i % kPairStages], (i / kPairStages) & 1, &ignore);
+        }
+    } else if (warp == 5 && rank == 0 && tc::elect_one()) {
+        const uint32_t a_step = p.a_k_inner ? 32 : 32 * kTile, b_step = p.b_k_inner ? 32 : 32 * kTile;
+        uint32_t used = 0, groups = 0, it = 0;
+        bool ok = true;
+        for (uint32_t t = first; t < tiles && ok; t += step, ++it) {
+            if (it > 0 && !tc::bar_wait(&drained, (it - 1) & 1, &gave_up)) break;
+            tc::fence_after();
+            const uint32_t acc = tmem + (it & 1) * kAccStride;
+            for (uint32_t kb = 0; kb < p.n_kb; ++kb, ++used) {
+                const uint32_t s = used % kPairStages;
+                if (!tc::bar_wait(&full[s], (used / kPairStages) & 1, &gave_up)) {
+                    ok = false;
+                    break;
+                }
+                tc::fence_after();
+                const uint32_t at = base + s * kPairStageBytes;
+                if ((kb & 3) == 0) {
+                    // into the columns of the group before the last: its products are done, since this stage's
+                    // load waited for those five k blocks back, and a tile's first one for the tile before
+                    ++groups;
+                    const uint32_t sf = tmem + kScaleColumn + (groups & 1) * 12, from = at + 2 * kBoxBytes;
+                    tc::scale_copy<2>(sf, scale_desc(from));
+                    tc::scale_copy<2>(sf + 4, scale_desc(from + kScaleBytes));
+                    tc::scale_copy<2>(sf + 8, scale_desc(from + 2 * kScaleBytes));
+                }
+                const uint32_t sf = tmem + kScaleColumn + (groups & 1) * 12;
+                const uint32_t idesc = tc::mx_idesc_select(p.idesc, kb & 3);
+#pragma unroll
+                for (uint32_t q = 0; q < 4; ++q)
+                    tc::mx_mma<2>(acc, box_desc(at + q * a_step), box_desc(at + kBoxBytes + q * b_step), idesc, sf,
+                                  sf + 4, kb > 0 || q > 0);
+                tc::mma_commit<2>(&empty[s]);
+            }
+            tc::mma_commit<2>(&done);
+        }
+        if (gave_up) {
+            // the tensor cores may still be at work
+            tc::mma_commit<2>(&ended);
+            int ignore = 0;
+            tc::bar_wait(&ended, 0, &ignore);
+        }
+    } else if (warp < 4) {
+        constexpr uint32_t kCols = kOut == PS_DTYPE_F32 ? 32 : 64, kChunks = kPairTile / kCols;
+        unsigned char* const bufs = base_ptr + kPairStages * kPairStageBytes + warp * 2 * kStoreBytes;
+        uint32_t it = 0, n = 0;
+        bool good = true;
+        for (uint32_t t = first; t < tiles; t += step, ++it) {
+            uint32_t tm, tn;
+            tile_at(p, t, &tm, &tn);
+            good = good && tc::bar_wait(&done, it & 1, &gave_up);
+            good = __all_sync(0xffffffffu, good);
+            tc::fence_after();
+            const uint32_t acc = tmem + (it & 1) * kAccStride + (warp << 21);
+            const uint32_t row0 = tm * kPairTile + rank * kTile + warp * 32;
+            bool loaded = false;
+            for (uint32_t c = 0; c < kChunks; ++c, ++n) {
+                // the overlapping columns first: the last ones of the lower accumulator, the first of the upper
+                const uint32_t chunk = (it & 1) ? c : (c == 0 ? kChunks - 1 : c - 1);
+                const uint32_t col = tn * kPairTile + chunk * kCols;
+                unsigned char* const buf = bufs + (n & 1) * kStoreBytes;
+                if (p.vec) {
+                    if (lane == 0) tc::store_wait_read<1>();
+                    __syncwarp();
+                }
+                stage_row<kOut>(buf, lane, p, col, acc + chunk * kCols, good, &loaded, &drained);
+                if (p.vec) tc::fence_to_async();
+                __syncwarp();
+                if (row0 >= p.m || col >= p.n) {
+                    if (p.vec && lane == 0) tc::store_none();
+                    continue;
+                }
+                if (p.vec) {
+                    if (lane == 0) tc::store_box(&map_out, tc::smem_u32(buf), (int)col, (int)row0);
+                } else {
+                    const uint32_t rows = min(32u, p.m - row0), cols = min(kCols, p.n - col);
+                    for (uint32_t r = 0; r < rows; ++r) {
+                        const uint64_t o = (uint64_t)(row0 + r) * p.ldo + col;
+                        for (uint32_t e = lane; e < cols; e += 32) {
+                            constexpr uint32_t kPer = kOut == PS_DTYPE_F32 ? 4 : 8;
+                            const unsigned char* at = buf + r * 128 + (((e / kPer) ^ (r & 7)) << 4);
+                            if constexpr (kOut == PS_DTYPE_F32)
+                                reinterpret_cast<float*>(p.out)[o + e] = reinterpret_cast<const float*>(at)[e % kPer];
+                            else
+                                reinterpret_cast<uint16_t*>(p.out)[o + e] = reinterpret_cast<const uint16_t*>(at)[e % kPer];
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+        if (lane == 0) tc::store_wait_read<0>();
+        tc::fence_before();
+    }
+    __syncwarp();
+    __syncthreads();
+    tc::cluster_sync();
+    if (warp == 5) tc::tmem_free<2>(tmem, 512);
     if (threadIdx.x == 0 && gave_up) atomicAdd(&g_gave_up, 1u);
 }
 
@@ -295,6 +536,81 @@ int encode_operand(const ps_block_operand* o, uint64_t outer, uint64_t k, uint32
 
 uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 
+// 256 x 256 tiles where they fill the pairs of SMs.
+bool use_pairs(uint32_t m, uint32_t n, uint32_t n_kb, int sms)
+{
+    return n_kb > 0 && (uint64_t)ceil_div(m, kPairTile) * ceil_div(n, kPairTile) >= (uint64_t)sms / 2;
+}
+
+template <typename F>
+int allow_smem(F kernel, uint32_t bytes)
+{
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess) return PS_OK;
+    ps_internal::set_cuda_error((int)e);
+    cudaGetLastError();
+    return PS_ERR_CUDA;
+}
+
+template <int kOut>
+int launch_pairs_as(const ProductArgs& p, const CUtensorMap* maps, const CUtensorMap& out, uint32_t grid, cudaStream_t st)
+{
+    const int rc = allow_smem(block_matmul_pair_kernel<kOut>, kPairSmem);
+    if (rc != PS_OK) return rc;
+    block_matmul_pair_kernel<kOut><<<grid, kPairThreads, kPairSmem, st>>>(maps[0], maps[1], maps[2], maps[3], out, p);
+    return ps_internal::after_launch();
+}
+
+int launch_pairs(ProductArgs& p, const CUtensorMap* maps, const ps_block_operand* a, const ps_block_operand* b,
+                 uint64_t osize, int sms, cudaStream_t st)
+{
+    p.tiles_m = ceil_div(p.m, kPairTile), p.tiles_n = ceil_div(p.n, kPairTile);
+    p.idesc = tc::mx_idesc(256, 256, a->fmt, b->fmt, !a->k_dim, !b->k_dim);
+    const uint64_t tiles = (uint64_t)p.tiles_m * p.tiles_n;
+    if (tiles > 0x7fffffffull) return PS_ERR_LIMIT;
+    CUtensorMap out;
+    memset(&out, 0, sizeof(out));
+    if (p.vec) {
+        const CUtensorMapDataType type = p.out_dtype == PS_DTYPE_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                         : p.out_dtype == PS_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                       : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+        const int rc = encode(&out, type, p.out, p.n, p.m, p.ldo * osize, (uint32_t)(128 / osize), 32,
+                              CU_TENSOR_MAP_SWIZZLE_128B);
+        if (rc != PS_OK) return rc;
+    }
+    const uint64_t pairs = (uint64_t)sms / 2;
+    const uint32_t grid = 2 * (uint32_t)(tiles < pairs ? tiles : pairs);
+    if (p.out_dtype == PS_DTYPE_F16) return launch_pairs_as<PS_DTYPE_F16>(p, maps, out, grid, st);
+    if (p.out_dtype == PS_DTYPE_BF16) return launch_pairs_as<PS_DTYPE_BF16>(p, maps, out, grid, st);
+    return launch_pairs_as<PS_DTYPE_F32>(p, maps, out, grid, st);
+}
+
+int launch_split(ProductArgs& p, const CUtensorMap* maps, const ps_block_operand* a, const ps_block_operand* b, int sms,
+                 cudaStream_t st)
+{
+    p.tiles_m = ceil_div(p.m, kTile), p.tiles_n = ceil_div(p.n, kTile);
+    if (p.n_kb > 0) p.idesc = tc::mx_idesc(128, 128, a->fmt, b->fmt, !a->k_dim, !b->k_dim);
+    const uint64_t tiles = (uint64_t)p.tiles_m * p.tiles_n;
+    uint32_t splits = 1;
+    while (splits < 8 && tiles * splits < (uint64_t)sms && splits * 4 <= p.n_kb) splits *= 2;
+    if (tiles * splits > 0x7fffffffull) return PS_ERR_LIMIT;
+    const int rc = allow_smem(block_matmul_split_kernel, kSplitSmem);
+    if (rc != PS_OK) return rc;
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3((uint32_t)(tiles * splits));
+    cfg.blockDim = dim3(kSplitThreads);
+    cfg.dynamicSmemBytes = kSplitSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = splits, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, block_matmul_split_kernel, maps[0], maps[1], maps[2], maps[3], p, splits);
+    return ps_internal::after_launch();
+}
+
 }  // namespace
 
 extern "C" {
@@ -332,31 +648,8 @@ int ps_block_matmul(const ps_block_operand* a, const ps_block_operand* b, uint32
     const int sms = ps_internal::sm_count();
     if (sms < 0) return sms;
 
-    p.tiles_m = ceil_div(m, kTile), p.tiles_n = ceil_div(n, kTile);
-    if (k > 0) p.idesc = tc::mx_idesc(128, 128, a->fmt, b->fmt, !a->k_dim, !b->k_dim);
-    const uint64_t tiles = (uint64_t)p.tiles_m * p.tiles_n;
-    uint32_t splits = 1;
-    while (splits < 8 && tiles * splits < (uint64_t)sms && splits * 4 <= p.n_kb) splits *= 2;
-    if (tiles * splits > 0x7fffffffull) return PS_ERR_LIMIT;
-    static const cudaError_t attr =
-        cudaFuncSetAttribute(block_matmul_split_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSplitSmem);
-    if (attr != cudaSuccess) {
-        ps_internal::set_cuda_error((int)attr);
-        return PS_ERR_CUDA;
-    }
-    cudaLaunchConfig_t cfg;
-    memset(&cfg, 0, sizeof(cfg));
-    cfg.gridDim = dim3((uint32_t)(tiles * splits));
-    cfg.blockDim = dim3(kSplitThreads);
-    cfg.dynamicSmemBytes = kSplitSmem;
-    cfg.stream = (cudaStream_t)stream;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = splits, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, block_matmul_split_kernel, maps[0], maps[1], maps[2], maps[3], p, splits);
-    return ps_internal::after_launch();
+    if (use_pairs(m, n, p.n_kb, sms)) return launch_pairs(p, maps, a, b, osize, sms, (cudaStream_t)stream);
+    return launch_split(p, maps, a, b, sms, (cudaStream_t)stream);
 }
 
 int ps_block_matmul_gave_up(uint32_t* count)

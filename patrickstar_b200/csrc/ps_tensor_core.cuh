@@ -36,7 +36,7 @@ __device__ __forceinline__ void bar_arrive_at(uint64_t* bar, uint32_t rank)
         "{\n"
         ".reg .b32 r;\n"
         "mapa.shared::cluster.u32 r, %0, %1;\n"
-        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [r];\n"
+        "mbarrier.arrive.shared::cluster.b64 _, [r];\n"
         "}\n" ::"r"(smem_u32(bar)),
         "r"(rank)
         : "memory");
@@ -47,13 +47,22 @@ __device__ __forceinline__ bool bar_try(uint32_t addr, uint32_t parity)
     asm volatile(
         "{\n"
         ".reg .pred p;\n"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
         "selp.u32 %0, 1, 0, p;\n"
         "}\n"
         : "=r"(done)
         : "r"(addr), "r"(parity)
         : "memory");
     return done != 0;
+}
+// True in one lane of a converged warp.  A branch on it tells the compiler that a single thread runs what is
+// inside, so that descriptors and addresses of tcgen05 and of tensor-map copies stay in uniform registers;
+// a branch on the lane's number makes it loop over lanes before each of them (product 8192^3: 458 us, not 390).
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t one;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(one));
+    return one != 0;
 }
 __device__ __forceinline__ uint64_t now_ns()
 {
@@ -126,15 +135,41 @@ __device__ __forceinline__ void load_box(const CUtensorMap* m, uint32_t dst, uin
         "l"(m), "r"(smem_u32(bar)), "r"(x), "r"(y)
         : "memory");
 }
-// A CTA of a pair loads into its own memory; completion counts on the barrier of the pair's even CTA.
-__device__ __forceinline__ void load_box_pair(const CUtensorMap* m, uint32_t dst, uint64_t* bar, int x, int y)
+// Address of `p` in CTA `rank`'s shared memory
+__device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank)
+{
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+    return r;
+}
+// A CTA of a pair loads into its own memory; completion counts on a barrier of either (cluster_addr).
+__device__ __forceinline__ void load_box_pair(const CUtensorMap* m, uint32_t dst, uint32_t bar, int x, int y)
 {
     asm volatile(
         "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
         "%4}], [%2];" ::"r"(dst),
-        "l"(m), "r"(smem_u32(bar) & 0xFEFFFFFFu), "r"(x), "r"(y)
+        "l"(m), "r"(bar), "r"(x), "r"(y)
         : "memory");
 }
+
+// A box of shared memory to global memory; boxes reach over the matrix's end without writing there.
+__device__ __forceinline__ void store_box(const CUtensorMap* m, uint32_t src, int x, int y)
+{
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(m), "r"(src),
+                 "r"(x), "r"(y)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// Stands for a store that was left out.
+__device__ __forceinline__ void store_none() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// Until at most `kLeft` of this thread's stores still read shared memory.
+template <int kLeft>
+__device__ __forceinline__ void store_wait_read()
+{
+    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kLeft) : "memory");
+}
+// What this thread wrote to shared memory is seen by the copies it issues from now on.
+__device__ __forceinline__ void fence_to_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // ---------------------------------------------------------------------------
 // tensor memory

@@ -38,7 +38,7 @@ def integer_operand(rows, cols, blocks, fmt, gen):
 
 
 SHAPES = [(1, 16, 16), (1, 1, 1), (128, 128, 128), (128, 128, 512), (7, 250, 129), (130, 129, 640), (257, 384, 1000),
-          (300, 17, 1537), (64, 1600, 800), (513, 1025, 300), (640, 640, 2100), (1, 4096, 1024)]
+          (300, 17, 1537), (64, 1600, 800), (513, 1025, 300), (640, 640, 2100), (1, 4096, 1024), (2300, 2090, 1100), (2560, 2304, 128), (1281, 4099, 257)]
 
 
 @pytest.mark.parametrize("form", sorted(FORMS))
