@@ -551,6 +551,41 @@ typedef struct ps_block_operand {
 int ps_block_matmul(const ps_block_operand* a, const ps_block_operand* b, uint32_t m, uint32_t n, uint32_t k,
                     const void* bias_dev, int bias_dtype, void* out_dev, int out_dtype, uint64_t ldo, void* stream);
 
+/* A linear layer made of the calls above: y = Q_row(x) Q_tile(weight)^T + bias,
+ * dx = Q_row(dy) Q_tile(weight), dw = Q_col(dy)^T Q_col(x), db = column sums of dy.
+ * x and y [tokens, k] and [tokens, n] of x_dtype; weight [n, k] of weight_dtype,
+ * or, quantized before, kept_data with both scale arrays of tile blocks (weight
+ * is then not read).  Row strides in elements (ld_kept: bytes); y, dx, dw, db
+ * are contiguous, dx of x_dtype, dw of weight_dtype, db of bias_dtype.
+ *
+ * keep says what the backward call will want: PS_KEEP_INPUT for dw,
+ * PS_KEEP_WEIGHT for dx.  ps_fp8_linear_sizes gives the bytes of the buffers that
+ * the caller provides (256-byte aligned): sizes[0] `saved`, kept from the forward
+ * call to the backward one, sizes[1] and sizes[2] the scratch of the two.  The
+ * backward call takes the same struct and keep (x, weight and bias are not read)
+ * and skips the gradients whose pointer is NULL. */
+#define PS_KEEP_INPUT 1
+#define PS_KEEP_WEIGHT 2
+
+typedef struct ps_fp8_linear {
+    const void* x;
+    const void* weight;
+    const void* bias;      /* [n] or NULL */
+    const void* kept_data; /* or NULL */
+    const void* kept_scales1;
+    const void* kept_scales0;
+    uint64_t ld_x, ld_weight, ld_kept;
+    uint32_t tokens, k, n;
+    int32_t x_dtype, weight_dtype, bias_dtype, kept_fmt;
+    int32_t reserved;
+} ps_fp8_linear;
+
+int ps_fp8_linear_sizes(const ps_fp8_linear* layer, int keep, uint64_t* sizes);
+int ps_fp8_linear_forward(const ps_fp8_linear* layer, int keep, void* y_dev, void* saved_dev, void* scratch_dev,
+                          void* stream);
+int ps_fp8_linear_backward(const ps_fp8_linear* layer, int keep, const void* saved_dev, const void* dy_dev, uint64_t ld_dy,
+                           int grad_fmt, void* dx_dev, void* dw_dev, void* db_dev, void* scratch_dev, void* stream);
+
 /* Number of thread blocks of ps_block_matmul on the current device that gave up
  * a wait (2 s) since the library was loaded; such a block's part of the output
  * is NaN.  0 unless the GPU is being held by something else.  Synchronises. */

@@ -23,6 +23,7 @@ PS_ERR_LIMIT = -6
 
 PS_DTYPE_F16, PS_DTYPE_BF16, PS_DTYPE_F32 = 0, 1, 2
 PS_FP8_E4M3, PS_FP8_E5M2 = 0, 1
+PS_KEEP_INPUT, PS_KEEP_WEIGHT = 1, 2
 PS_TAIL_DROP, PS_TAIL_BUCKET = 0, 1
 PS_REDUCE_NONE, PS_REDUCE_SUM, PS_REDUCE_MEAN = 0, 1, 2
 PS_DISTILL_MAX_VOCAB, PS_DISTILL_MAX_K = 1 << 20, 1024
@@ -94,6 +95,14 @@ class BlockOperand(C.Structure):
                 ("k_dim", C.c_int32)]
 
 
+class Fp8LinearLayer(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p), ("kept_data", C.c_void_p),
+                ("kept_scales1", C.c_void_p), ("kept_scales0", C.c_void_p), ("ld_x", C.c_uint64),
+                ("ld_weight", C.c_uint64), ("ld_kept", C.c_uint64), ("tokens", C.c_uint32), ("k", C.c_uint32),
+                ("n", C.c_uint32), ("x_dtype", C.c_int32), ("weight_dtype", C.c_int32), ("bias_dtype", C.c_int32),
+                ("kept_fmt", C.c_int32), ("reserved", C.c_int32)]
+
+
 class DistillProblem(C.Structure):
     _fields_ = [("logits", C.c_void_p), ("indices", C.c_void_p), ("teacher", C.c_void_p), ("mask", C.c_void_p),
                 ("ld_logits", C.c_uint64), ("ld_indices", C.c_uint64), ("ld_teacher", C.c_uint64),
@@ -102,7 +111,7 @@ class DistillProblem(C.Structure):
                 ("reduction", C.c_int32), ("temperature", C.c_float), ("weight", C.c_float)]
 
 
-assert C.sizeof(BlockOperand) == 32 and C.sizeof(DistillProblem) == 96
+assert C.sizeof(BlockOperand) == 32 and C.sizeof(DistillProblem) == 96 and C.sizeof(Fp8LinearLayer) == 104
 assert C.sizeof(StepPlan) == 512 and C.sizeof(ScalerState) == 64
 assert C.sizeof(HyperSlot) == 64 and C.sizeof(StepCtrl) == 48 + 64 * PS_MAX_SLOTS
 
@@ -160,6 +169,10 @@ SIGNATURES = {
                                   C.c_uint32, _p, C.c_int, _p, C.c_int, C.c_uint64, _p]),
     "ps_distill_forward": (C.c_int, [C.POINTER(DistillProblem), _p, _p, _p, _p, _p, _p, C.c_uint64, _p, _p]),
     "ps_distill_backward": (C.c_int, [C.POINTER(DistillProblem), _p, _p, _p, C.c_uint32, _p, _p, C.c_uint64, _p]),
+    "ps_fp8_linear_sizes": (C.c_int, [C.POINTER(Fp8LinearLayer), C.c_int, C.POINTER(C.c_uint64)]),
+    "ps_fp8_linear_forward": (C.c_int, [C.POINTER(Fp8LinearLayer), C.c_int, _p, _p, _p, _p]),
+    "ps_fp8_linear_backward": (C.c_int, [C.POINTER(Fp8LinearLayer), C.c_int, _p, _p, C.c_uint64, C.c_int, _p, _p, _p,
+                                         _p, _p]),
     "ps_block_matmul_gave_up": (C.c_int, [C.POINTER(C.c_uint32)]),
 }
 

@@ -14,13 +14,16 @@ tensor core applies them.  An element that is not finite stays visible (NaN in
 e4m3, itself in e5m2), so a gradient that overflowed still reaches the overflow
 test of the step.  No counterpart in the reference.
 """
+import contextlib
 import ctypes as C
+import functools
 import math
 
 import torch
 
 from ._lib import (PS_BLOCKS_COL, PS_BLOCKS_ROW, PS_BLOCKS_ROW_COL, PS_BLOCKS_TILE, PS_DTYPE_BF16, PS_DTYPE_F16,
-                   PS_DTYPE_F32, PS_FP8_E4M3, PS_FP8_E5M2, BlockOperand, check, lib)
+                   PS_DTYPE_F32, PS_FP8_E4M3, PS_FP8_E5M2, PS_KEEP_INPUT, PS_KEEP_WEIGHT, BlockOperand, Fp8LinearLayer,
+                   check, lib)
 
 BLOCK = 128
 
@@ -31,7 +34,15 @@ _BLOCKS = {"row": PS_BLOCKS_ROW, "col": PS_BLOCKS_COL, "row+col": PS_BLOCKS_ROW_
 
 
 def _stream_ptr(device):
-    return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    return torch._C._cuda_getCurrentRawStream(device.index)   # current_stream(device).cuda_stream, without the object
+
+
+_NO_SWITCH = contextlib.nullcontext()
+
+
+def _on(device):
+    """``torch.cuda.device(device)`` where that is not the current one already."""
+    return _NO_SWITCH if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _scales_shape(outer, contracted):
@@ -140,15 +151,14 @@ def _format(fmt):
     return _FORMATS[fmt]
 
 
-def _quantize(x, blocks, fmt, sums=False):
-    """block_quantize for a checked matrix; with ``sums`` also the float32 column sums of each run of 128 rows."""
+def _quantize(x, blocks, fmt):
+    """block_quantize for a checked matrix."""
     dtype, code = _FORMATS[fmt]
-    if x.stride(1) != 1 and x.shape[1] > 1:
-        x = x.contiguous()
+    x = _adjacent(x)
     rows, cols = x.shape
     ldq = -(-cols // 16) * 16
     dev = x.device
-    q1 = s1 = q0 = s0 = part = None
+    q1 = s1 = q0 = s0 = None
     if blocks != "col":
         q1 = torch.empty((rows, ldq), dtype=dtype, device=dev)
         s1 = torch.empty(_scales_shape(rows, cols), dtype=torch.uint8, device=dev)
@@ -156,14 +166,12 @@ def _quantize(x, blocks, fmt, sums=False):
         q0 = torch.empty((rows, ldq), dtype=dtype, device=dev)
     if blocks != "row":
         s0 = torch.empty(_scales_shape(cols, rows), dtype=torch.uint8, device=dev)
-    if sums:
-        part = torch.empty((-(-rows // BLOCK), cols), dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
+    with _on(dev):
         check(lib.ps_block_quantize(
             x.data_ptr(), _DTYPES[x.dtype], x.stride(0) if rows > 1 else cols, rows, cols, _BLOCKS[blocks], code,
             q1.data_ptr() if q1 is not None else None, s1.data_ptr() if s1 is not None else None,
             q0.data_ptr() if q0 is not None else None, s0.data_ptr() if s0 is not None else None, ldq,
-            part.data_ptr() if part is not None else None, _stream_ptr(dev)), "ps_block_quantize")
+            None, _stream_ptr(dev)), "ps_block_quantize")
     if cols != ldq:
         q1 = q1 if q1 is None else q1[:, :cols]
         q0 = q0 if q0 is None else q0[:, :cols]
@@ -171,8 +179,7 @@ def _quantize(x, blocks, fmt, sums=False):
         return BlockQuantized._of(q1, "tile", s1, s0)
     row = None if q1 is None else BlockQuantized._of(q1, "row", s1, None)
     col = None if q0 is None else BlockQuantized._of(q0, "col", None, s0)
-    out = row if blocks == "row" else col if blocks == "col" else (row, col)
-    return (out, part) if sums else out
+    return row if blocks == "row" else col if blocks == "col" else (row, col)
 
 
 def block_quantize(x, blocks="row", fmt="e4m3"):
@@ -197,7 +204,7 @@ def block_quantize(x, blocks="row", fmt="e4m3"):
 def _matmul(a, a_dim, b, b_dim, bias, out_dtype):
     m, n, k = a.shape[1 - a_dim], b.shape[1 - b_dim], a.shape[a_dim]
     out = torch.empty((m, n), dtype=out_dtype, device=a.device)
-    with torch.cuda.device(a.device):
+    with _on(a.device):
         check(lib.ps_block_matmul(
             C.byref(a._operand(a_dim)), C.byref(b._operand(b_dim)), m, n, k,
             bias.data_ptr() if bias is not None else None, _DTYPES[bias.dtype] if bias is not None else 0,
@@ -246,9 +253,55 @@ def _check_bias(bias, n, device, where):
         raise ValueError("%s: bias on %s, the product on %s" % (where, bias.device, device))
 
 
+@functools.lru_cache(maxsize=4096)
+def _layer_bytes(tokens, k, n, kept, keep):
+    """Bytes of the buffers of ps_fp8_linear_forward and _backward: (saved, forward scratch, backward scratch)."""
+    sizes = (C.c_uint64 * 3)()
+    check(lib.ps_fp8_linear_sizes(C.byref(Fp8LinearLayer(kept_data=1 if kept else None, tokens=tokens, k=k, n=n)), keep,
+                                  sizes), "ps_fp8_linear_sizes")
+    return tuple(sizes)
+
+
+def _layer(x, weight, bias, kept, tokens, k, n):
+    """The C struct of a layer.  ``x``, ``weight`` and ``bias`` have adjacent elements."""
+    if kept is None:
+        return Fp8LinearLayer(x.data_ptr(), weight.data_ptr(), None if bias is None else bias.data_ptr(), None, None,
+                              None, x.stride(0) if tokens > 1 else k, weight.stride(0) if n > 1 else k, 0, tokens, k, n,
+                              _DTYPES[x.dtype], _DTYPES[weight.dtype], 0 if bias is None else _DTYPES[bias.dtype], 0, 0)
+    op = kept._operand(1)
+    return Fp8LinearLayer(x.data_ptr(), None, None if bias is None else bias.data_ptr(), op.data, op.scales,
+                          kept.scales0.data_ptr(), x.stride(0) if tokens > 1 else k, 0, op.ld, tokens, k, n,
+                          _DTYPES[x.dtype], 0, 0 if bias is None else _DTYPES[bias.dtype], op.fmt, 0)
+
+
+def _adjacent(t):
+    return t if t.shape[1] == 1 or t.stride(1) == 1 else t.contiguous()
+
+
+def _linear_forward(x, weight, bias, kept, keep):
+    """(y, saved buffer or None, layer struct) of matrices that are checked."""
+    tokens, k = x.shape
+    n = (weight if kept is None else kept).shape[0]
+    x = _adjacent(x)
+    if kept is None:
+        weight = _adjacent(weight)
+    if bias is not None:
+        bias = bias.contiguous()
+    dev = x.device
+    saved_bytes, scratch_bytes, _ = _layer_bytes(tokens, k, n, kept is not None, keep)
+    y = torch.empty((tokens, n), dtype=x.dtype, device=dev)
+    saved = torch.empty(saved_bytes, dtype=torch.uint8, device=dev) if saved_bytes else None
+    scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=dev)
+    layer = _layer(x, weight, bias, kept, tokens, k, n)
+    with _on(dev):
+        check(lib.ps_fp8_linear_forward(C.byref(layer), keep, y.data_ptr(), None if saved is None else saved.data_ptr(),
+                                        scratch.data_ptr(), _stream_ptr(dev)), "ps_fp8_linear_forward")
+    return y, saved, layer
+
+
 def _aligned(data):
-    """Values whose rows start on 16-byte boundaries: ``data``, or a copy where a saved tensor came back packed."""
-    if data.data_ptr() % 16 == 0 and (data.shape[0] < 2 or data.stride(0) % 16 == 0) and data.stride(1) == 1:
+    """8-bit values whose rows start on 16-byte boundaries: ``data``, or a copy where a saved tensor came back packed."""
+    if data.data_ptr() % 16 == 0 and (data.shape[0] < 2 or data.stride(0) % 16 == 0):
         return data
     out = torch.empty((data.shape[0], -(-data.shape[1] // 16) * 16), dtype=data.dtype, device=data.device)
     out = out[:, :data.shape[1]]
@@ -260,48 +313,39 @@ class _Fp8Linear(torch.autograd.Function):
     """y = Q_row(x) Q_tile(w)^T + b;  dx = Q_row(dy) Q_tile(w);  dw = Q_col(dy)^T Q_col(x);  db = sum of dy."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, kept, grad_fmt, grads):
-        x2 = x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
-        ctx.shape, ctx.grad_fmt = x.shape, grad_fmt
-        ctx.dtypes = (x.dtype, weight.dtype if weight is not None else None, bias.dtype if bias is not None else None)
-        xc = None
-        if grads and ctx.needs_input_grad[1]:
-            xr, xc = _quantize(x2, "row+col", "e4m3")
-        else:
-            xr = _quantize(x2, "row", "e4m3")
-        w = kept if kept is not None else _quantize(weight, "tile", "e4m3")
-        ctx.save_for_backward(*(w.data, w.scales0) if ctx.needs_input_grad[0] else (None, None),
-                              *(xc.data, xc.scales0) if xc is not None else (None, None))
-        y = _matmul(xr, 1, w, 1, bias.contiguous() if bias is not None else None, x.dtype)
-        return y.view(x.shape[:-1] + (y.shape[1],))
+    def forward(ctx, x, weight, bias, kept, grad_fmt):
+        need_x, need_w = ctx.needs_input_grad[:2]
+        keep = (PS_KEEP_WEIGHT if need_x else 0) | (PS_KEEP_INPUT if need_w else 0)
+        y, saved, ctx.layer = _linear_forward(x, weight, bias, kept, keep)
+        ctx.keep, ctx.grad_fmt, ctx.x_dtype = keep, grad_fmt, x.dtype
+        ctx.w_dtype = None if weight is None else weight.dtype
+        ctx.b_dtype = None if bias is None else bias.dtype
+        ctx.save_for_backward(saved, *((kept.data, kept.scales1, kept.scales0) if kept is not None and need_x else ()))
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        wd, ws, xd, xs = ctx.saved_tensors
+        saved, *kept = ctx.saved_tensors
+        layer, dev = ctx.layer, dy.device
+        if kept:    # saved tensors may come back elsewhere
+            kept[0] = _aligned(kept[0])
+            op = BlockQuantized._of(kept[0], "tile", kept[1], kept[2])._operand(0)
+            layer.kept_data, layer.kept_scales0, layer.ld_kept = op.data, op.scales, op.ld
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        x_dtype, w_dtype, b_dtype = ctx.dtypes
-        dx = dw = db = None
-        dy2 = dy.reshape(math.prod(dy.shape[:-1]), dy.shape[-1])
-        row = col = part = None
-        if need_b:
-            (row, col), part = _quantize(dy2, "row+col", ctx.grad_fmt, sums=True)
-        elif need_x and need_w:
-            row, col = _quantize(dy2, "row+col", ctx.grad_fmt)
-        elif need_x:
-            row = _quantize(dy2, "row", ctx.grad_fmt)
-        elif need_w:
-            col = _quantize(dy2, "col", ctx.grad_fmt)
-        if need_x:
-            dx = _matmul(row, 1, BlockQuantized._of(_aligned(wd), "col", None, ws), 0, None, x_dtype).view(ctx.shape)
-        if need_w:
-            dw = _matmul(col, 0, BlockQuantized._of(_aligned(xd), "col", None, xs), 0, None, w_dtype)
-        if need_b:
-            db = torch.empty(part.shape[1], dtype=b_dtype, device=part.device)
-            with torch.cuda.device(part.device):
-                check(lib.ps_column_sum(part.data_ptr(), part.shape[0], part.shape[1], db.data_ptr(), _DTYPES[b_dtype],
-                                        _stream_ptr(part.device)), "ps_column_sum")
-        return dx, dw, db, None, None, None
+        dy = _adjacent(dy)
+        tokens, k, n = layer.tokens, layer.k, layer.n
+        dx = torch.empty((tokens, k), dtype=ctx.x_dtype, device=dev) if need_x else None
+        dw = torch.empty((n, k), dtype=ctx.w_dtype, device=dev) if need_w else None
+        db = torch.empty(n, dtype=ctx.b_dtype, device=dev) if need_b else None
+        scratch = torch.empty(_layer_bytes(tokens, k, n, bool(layer.kept_data), ctx.keep)[2], dtype=torch.uint8, device=dev)
+        with _on(dev):
+            check(lib.ps_fp8_linear_backward(
+                C.byref(layer), ctx.keep, None if saved is None else saved.data_ptr(), dy.data_ptr(),
+                dy.stride(0) if tokens > 1 else n, _FORMATS[ctx.grad_fmt][1], dx.data_ptr() if need_x else None,
+                dw.data_ptr() if need_w else None, db.data_ptr() if need_b else None, scratch.data_ptr(),
+                _stream_ptr(dev)), "ps_fp8_linear_backward")
+        return dx, dw, db, None, None
 
 
 def fp8_linear(x, weight, bias=None, grad_fmt="e4m3"):
@@ -319,22 +363,31 @@ def fp8_linear(x, weight, bias=None, grad_fmt="e4m3"):
     if x.dim() < 1:
         raise ValueError("fp8_linear: x needs at least one dimension")
     _format(grad_fmt)
-    kept = weight if isinstance(weight, BlockQuantized) else None
-    if kept is not None:
+    kept = None
+    if isinstance(weight, BlockQuantized):
+        kept, weight = weight, None
         if kept.blocks != "tile":
             raise ValueError("fp8_linear: a quantized weight needs tile blocks, got %s" % kept.blocks)
+        (n, k), dev = kept.shape, kept.device
     else:
         _check_float(weight, "fp8_linear: weight")
         if weight.dim() != 2:
             raise ValueError("fp8_linear: weight must be a matrix, got %d dimensions" % weight.dim())
-    if weight.shape[1] != x.shape[-1]:
-        raise ValueError("fp8_linear: x has %d features, weight takes %d" % (x.shape[-1], weight.shape[1]))
-    if weight.device != x.device:
-        raise ValueError("fp8_linear: x on %s, weight on %s" % (x.device, weight.device))
+        (n, k), dev = weight.shape, weight.device
+    shape = x.shape
+    if shape[-1] != k:
+        raise ValueError("fp8_linear: x has %d features, weight takes %d" % (shape[-1], k))
+    if dev != x.device:
+        raise ValueError("fp8_linear: x on %s, weight on %s" % (x.device, dev))
     if bias is not None:
-        _check_bias(bias, weight.shape[0], x.device, "fp8_linear")
-    return _Fp8Linear.apply(x, None if kept is not None else weight, bias, kept, grad_fmt,
-                            torch.is_grad_enabled())
+        _check_bias(bias, n, dev, "fp8_linear")
+    x2 = x if len(shape) == 2 else x.reshape(math.prod(shape[:-1]), k)
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
+                                    (bias is not None and bias.requires_grad)):
+        y = _Fp8Linear.apply(x2, weight, bias, kept, grad_fmt)
+    else:
+        y = _linear_forward(x2, weight, bias, kept, 0)[0]
+    return y if len(shape) == 2 else y.view(shape[:-1] + (n,))
 
 
 class Fp8Linear(torch.nn.Linear):

@@ -23,6 +23,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
 #include <cstring>
 
 namespace {
@@ -123,6 +124,7 @@ block_matmul_split_kernel(const __grid_constant__ CUtensorMap map_a, const __gri
     __syncthreads();
     tc::fence_after();
     const uint32_t tmem = tmem_base;
+    cudaGridDependencySynchronize();  // up to here nothing that another kernel writes was touched
 
     if (warp == 4 && tc::elect_one()) {
         uint32_t issued = 0;
@@ -311,7 +313,7 @@ __device__ __forceinline__ void stage_row(unsigned char* buf, uint32_t row, cons
 }
 
 template <int kOut>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads)
+__global__ void __launch_bounds__(kPairThreads)
 block_matmul_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                          const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_sb,
                          const __grid_constant__ CUtensorMap map_out, const __grid_constant__ ProductArgs p)
@@ -341,6 +343,7 @@ block_matmul_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     tc::cluster_sync();
     tc::fence_after();
     const uint32_t tmem = tmem_base;
+    cudaGridDependencySynchronize();  // up to here nothing that another kernel writes was touched
 
     if (warp == 4 && tc::elect_one()) {
         uint32_t issued = 0;
@@ -542,22 +545,54 @@ bool use_pairs(uint32_t m, uint32_t n, uint32_t n_kb, int sms)
     return n_kb > 0 && (uint64_t)ceil_div(m, kPairTile) * ceil_div(n, kPairTile) >= (uint64_t)sms / 2;
 }
 
+// Lets a kernel have that much shared memory; `seen`: the devices on which that is done.
 template <typename F>
-int allow_smem(F kernel, uint32_t bytes)
+int allow_smem(F kernel, uint32_t bytes, std::atomic<uint64_t>& seen)
 {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    if (e == cudaSuccess) return PS_OK;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    const uint64_t bit = 1ull << (dev & 63);
+    if (e == cudaSuccess && dev < 64 && (seen.load(std::memory_order_relaxed) & bit)) return PS_OK;
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess) {
+        seen.fetch_or(bit, std::memory_order_relaxed);
+        return PS_OK;
+    }
     ps_internal::set_cuda_error((int)e);
     cudaGetLastError();
     return PS_ERR_CUDA;
 }
 
+// The kernel's set-up may run while the kernel before it in the stream finishes (the quantizer lets it).
+template <typename K, typename... Args>
+void launch_in_clusters(K kernel, uint32_t grid, uint32_t threads, uint32_t smem, uint32_t cluster, cudaStream_t st,
+                        const Args&... args)
+{
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    memset(at, 0, sizeof(at));
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cluster, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 template <int kOut>
 int launch_pairs_as(const ProductArgs& p, const CUtensorMap* maps, const CUtensorMap& out, uint32_t grid, cudaStream_t st)
 {
-    const int rc = allow_smem(block_matmul_pair_kernel<kOut>, kPairSmem);
+    static std::atomic<uint64_t> seen{0};
+    const int rc = allow_smem(block_matmul_pair_kernel<kOut>, kPairSmem, seen);
     if (rc != PS_OK) return rc;
-    block_matmul_pair_kernel<kOut><<<grid, kPairThreads, kPairSmem, st>>>(maps[0], maps[1], maps[2], maps[3], out, p);
+    launch_in_clusters(block_matmul_pair_kernel<kOut>, grid, kPairThreads, kPairSmem, 2, st, maps[0], maps[1], maps[2],
+                       maps[3], out, p);
     return ps_internal::after_launch();
 }
 
@@ -594,20 +629,11 @@ int launch_split(ProductArgs& p, const CUtensorMap* maps, const ps_block_operand
     uint32_t splits = 1;
     while (splits < 8 && tiles * splits < (uint64_t)sms && splits * 4 <= p.n_kb) splits *= 2;
     if (tiles * splits > 0x7fffffffull) return PS_ERR_LIMIT;
-    const int rc = allow_smem(block_matmul_split_kernel, kSplitSmem);
+    static std::atomic<uint64_t> seen{0};
+    const int rc = allow_smem(block_matmul_split_kernel, kSplitSmem, seen);
     if (rc != PS_OK) return rc;
-    cudaLaunchConfig_t cfg;
-    memset(&cfg, 0, sizeof(cfg));
-    cfg.gridDim = dim3((uint32_t)(tiles * splits));
-    cfg.blockDim = dim3(kSplitThreads);
-    cfg.dynamicSmemBytes = kSplitSmem;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = splits, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, block_matmul_split_kernel, maps[0], maps[1], maps[2], maps[3], p, splits);
+    launch_in_clusters(block_matmul_split_kernel, (uint32_t)(tiles * splits), kSplitThreads, kSplitSmem, splits, st, maps[0],
+                       maps[1], maps[2], maps[3], p, splits);
     return ps_internal::after_launch();
 }
 

@@ -171,14 +171,16 @@ struct QuantArgs {
 __host__ __device__ constexpr bool has_row(int mode) { return mode == PS_BLOCKS_ROW || mode == PS_BLOCKS_ROW_COL; }
 __host__ __device__ constexpr bool has_col(int mode) { return mode == PS_BLOCKS_COL || mode == PS_BLOCKS_ROW_COL; }
 
+struct Shared {
+    uint32_t key[kWarps][16][8];
+    float sum[kWarps][kBlock];
+};
+
 template <typename T, int kMode, int kFmt, bool kSum>
-__global__ void __launch_bounds__(kThreads) block_quantize_kernel(const QuantArgs a)
+__device__ __forceinline__ void quantize_tile(const QuantArgs& a, uint32_t tile, Shared& sh)
 {
     using V = Vec8<T>;
-    __shared__ uint32_t s_key[kWarps][16][V::kWords];
-    __shared__ float s_sum[kSum ? kWarps : 1][kBlock];
-
-    const uint32_t cb = blockIdx.x % a.col_blocks, rb = blockIdx.x / a.col_blocks;
+    const uint32_t cb = tile % a.col_blocks, rb = tile / a.col_blocks;
     const uint32_t cg = threadIdx.x & 15, rg = threadIdx.x >> 4;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t c0 = cb * kBlock + cg * 8, r0 = rb * kBlock + rg;
@@ -290,7 +292,7 @@ __global__ void __launch_bounds__(kThreads) block_quantize_kernel(const QuantArg
         }
         if (lane < 16) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s_sum[warp][cg * 8 + j] = cs[j];
+            for (int j = 0; j < 8; ++j) sh.sum[warp][cg * 8 + j] = cs[j];
         }
     }
 
@@ -298,13 +300,13 @@ __global__ void __launch_bounds__(kThreads) block_quantize_kernel(const QuantArg
 #pragma unroll
         for (int k = 0; k < V::kWords; ++k) {
             ck[k] = key_max<T>(ck[k], __shfl_xor_sync(0xffffffffu, ck[k], 16));
-            if (lane < 16) s_key[warp][cg][k] = ck[k];
+            if (lane < 16) sh.key[warp][cg][k] = ck[k];
         }
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < V::kWords; ++k) {
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) ck[k] = key_max<T>(ck[k], s_key[w][cg][k]);
+            for (int w = 0; w < kWarps; ++w) ck[k] = key_max<T>(ck[k], sh.key[w][cg][k]);
         }
         float inv[8];
         uint32_t byte[8];
@@ -326,10 +328,10 @@ __global__ void __launch_bounds__(kThreads) block_quantize_kernel(const QuantArg
 #pragma unroll
         for (int k = 0; k < V::kWords; ++k) key = key_max<T>(key, ck[k]);
         key = __reduce_max_sync(0xffffffffu, key_fold<T>(key));
-        if (lane == 0) s_key[warp][0][0] = key;
+        if (lane == 0) sh.key[warp][0][0] = key;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) key = max(key, s_key[w][0][0]);
+        for (int w = 0; w < kWarps; ++w) key = max(key, sh.key[w][0][0]);
         const uint32_t byte = scale_byte<kFmt>(key_float<T>(key));
         const float inv = scale_inverse(byte);
 #pragma unroll
@@ -347,10 +349,30 @@ __global__ void __launch_bounds__(kThreads) block_quantize_kernel(const QuantArg
             const uint32_t c = cb * kBlock + threadIdx.x;
             float t = 0.f;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) t += s_sum[w][threadIdx.x];
+            for (int w = 0; w < kWarps; ++w) t += sh.sum[w][threadIdx.x];
             if (c < a.cols) a.colsum[(size_t)rb * a.cols + c] = t;
         }
     }
+}
+
+template <typename T, int kMode, int kFmt, bool kSum>
+__global__ void __launch_bounds__(kThreads) block_quantize_kernel(const QuantArgs a)
+{
+    __shared__ Shared sh;
+    cudaTriggerProgrammaticLaunchCompletion();
+    quantize_tile<T, kMode, kFmt, kSum>(a, blockIdx.x, sh);
+}
+
+// Two matrices in one launch: the input of a layer (kMode) and, behind its `split` tiles, the weight.
+template <typename T, int kMode>
+__global__ void __launch_bounds__(kThreads) quantize_layer_kernel(const QuantArgs x, const QuantArgs w, uint32_t split)
+{
+    __shared__ Shared sh;
+    cudaTriggerProgrammaticLaunchCompletion();
+    if (blockIdx.x < split)
+        quantize_tile<T, kMode, PS_FP8_E4M3, false>(x, blockIdx.x, sh);
+    else
+        quantize_tile<T, PS_BLOCKS_TILE, PS_FP8_E4M3, false>(w, blockIdx.x - split, sh);
 }
 
 // Sums of a column's blocks, in order, in 64 bits: one thread a column.
@@ -388,7 +410,84 @@ void launch(int fmt, int mode, const QuantArgs& a, uint32_t tiles, cudaStream_t 
         launch<T, PS_FP8_E5M2>(mode, a, tiles, st);
 }
 
+// Checks a job and makes its arguments; *tiles is 0 where there is nothing to do.
+int prepare(const ps_internal::QuantizeJob& j, QuantArgs* a, uint32_t* tiles)
+{
+    *tiles = 0;
+    if (j.dtype < PS_DTYPE_F16 || j.dtype > PS_DTYPE_F32 || j.blocks < PS_BLOCKS_ROW || j.blocks > PS_BLOCKS_TILE)
+        return PS_ERR_INVALID;
+    if (j.fmt != PS_FP8_E4M3 && j.fmt != PS_FP8_E5M2) return PS_ERR_INVALID;
+    if (j.colsum != nullptr && j.blocks != PS_BLOCKS_ROW_COL) return PS_ERR_INVALID;
+    if (j.rows == 0 || j.cols == 0) return PS_OK;
+    const bool row = has_row(j.blocks) || j.blocks == PS_BLOCKS_TILE, col = has_col(j.blocks);
+    if (j.x == nullptr || (row && (j.q1 == nullptr || j.s1 == nullptr)) || (col && (j.q0 == nullptr || j.s0 == nullptr)) ||
+        (j.blocks == PS_BLOCKS_TILE && j.s0 == nullptr))
+        return PS_ERR_INVALID;
+    if (j.ldq < j.cols) return PS_ERR_INVALID;
+    const uint64_t esize = j.dtype == PS_DTYPE_F32 ? 4 : 2;
+    if ((uintptr_t)j.x % esize || j.ldq % 16 || (row && (uintptr_t)j.q1 % 16) || (col && (uintptr_t)j.q0 % 16))
+        return PS_ERR_ALIGN;
+    a->x = j.x, a->ld = j.ld, a->ldq = j.ldq, a->rows = j.rows, a->cols = j.cols;
+    a->row_blocks = (uint32_t)(((uint64_t)j.rows + kBlock - 1) / kBlock);
+    a->col_blocks = (uint32_t)(((uint64_t)j.cols + kBlock - 1) / kBlock);
+    a->q1 = (uint8_t*)j.q1, a->q0 = (uint8_t*)j.q0, a->s1 = (uint8_t*)j.s1, a->s0 = (uint8_t*)j.s0;
+    a->colsum = j.colsum;
+    a->vec = (uintptr_t)j.x % 16 == 0 && (j.ld * esize) % 16 == 0;
+    const uint64_t n = (uint64_t)a->row_blocks * a->col_blocks;
+    if (n > 0x7fffffffull || j.cols > 0xffffff00u || j.rows > 0xffffff00u) return PS_ERR_LIMIT;
+    *tiles = (uint32_t)n;
+    return PS_OK;
+}
+
+template <typename T>
+void launch_layer(int mode, const QuantArgs& x, uint32_t x_tiles, const QuantArgs& w, uint32_t w_tiles, cudaStream_t st)
+{
+    if (mode == PS_BLOCKS_ROW)
+        quantize_layer_kernel<T, PS_BLOCKS_ROW><<<x_tiles + w_tiles, kThreads, 0, st>>>(x, w, x_tiles);
+    else
+        quantize_layer_kernel<T, PS_BLOCKS_ROW_COL><<<x_tiles + w_tiles, kThreads, 0, st>>>(x, w, x_tiles);
+}
+
 }  // namespace
+
+namespace ps_internal {
+
+int quantize(const QuantizeJob& j, cudaStream_t st)
+{
+    QuantArgs a;
+    uint32_t tiles;
+    const int rc = prepare(j, &a, &tiles);
+    if (rc != PS_OK || tiles == 0) return rc;
+    if (j.dtype == PS_DTYPE_F16)
+        launch<__half>(j.fmt, j.blocks, a, tiles, st);
+    else if (j.dtype == PS_DTYPE_BF16)
+        launch<__nv_bfloat16>(j.fmt, j.blocks, a, tiles, st);
+    else
+        launch<float>(j.fmt, j.blocks, a, tiles, st);
+    return after_launch();
+}
+
+int quantize_layer(const QuantizeJob& x, const QuantizeJob& w, cudaStream_t st)
+{
+    QuantArgs ax, aw;
+    uint32_t x_tiles, w_tiles;
+    int rc = prepare(x, &ax, &x_tiles);
+    if (rc == PS_OK) rc = prepare(w, &aw, &w_tiles);
+    if (rc != PS_OK) return rc;
+    if (x_tiles == 0 || w_tiles == 0 || x.dtype != w.dtype || (uint64_t)x_tiles + w_tiles > 0x7fffffffull) {
+        rc = quantize(x, st);
+        return rc == PS_OK ? quantize(w, st) : rc;
+    }
+    if (x.dtype == PS_DTYPE_F16)
+        launch_layer<__half>(x.blocks, ax, x_tiles, aw, w_tiles, st);
+    else if (x.dtype == PS_DTYPE_BF16)
+        launch_layer<__nv_bfloat16>(x.blocks, ax, x_tiles, aw, w_tiles, st);
+    else
+        launch_layer<float>(x.blocks, ax, x_tiles, aw, w_tiles, st);
+    return after_launch();
+}
+
+}  // namespace ps_internal
 
 extern "C" {
 
@@ -396,36 +495,8 @@ int ps_block_quantize(const void* x_dev, int dtype, uint64_t ld, uint32_t rows, 
                       void* q1_dev, void* s1_dev, void* q0_dev, void* s0_dev, uint64_t ldq, float* colsum_dev,
                       void* stream)
 {
-    if (dtype < PS_DTYPE_F16 || dtype > PS_DTYPE_F32 || blocks < PS_BLOCKS_ROW || blocks > PS_BLOCKS_TILE)
-        return PS_ERR_INVALID;
-    if (fmt != PS_FP8_E4M3 && fmt != PS_FP8_E5M2) return PS_ERR_INVALID;
-    if (colsum_dev != nullptr && blocks != PS_BLOCKS_ROW_COL) return PS_ERR_INVALID;
-    if (rows == 0 || cols == 0) return PS_OK;
-    const bool row = has_row(blocks) || blocks == PS_BLOCKS_TILE, col = has_col(blocks);
-    if (x_dev == nullptr || (row && (q1_dev == nullptr || s1_dev == nullptr)) ||
-        (col && (q0_dev == nullptr || s0_dev == nullptr)) || (blocks == PS_BLOCKS_TILE && s0_dev == nullptr))
-        return PS_ERR_INVALID;
-    if (ldq < cols) return PS_ERR_INVALID;
-    const uint64_t esize = dtype == PS_DTYPE_F32 ? 4 : 2;
-    if ((uintptr_t)x_dev % esize || ldq % 16 || (row && (uintptr_t)q1_dev % 16) || (col && (uintptr_t)q0_dev % 16))
-        return PS_ERR_ALIGN;
-    QuantArgs a;
-    a.x = x_dev, a.ld = ld, a.ldq = ldq, a.rows = rows, a.cols = cols;
-    a.row_blocks = (uint32_t)(((uint64_t)rows + kBlock - 1) / kBlock);
-    a.col_blocks = (uint32_t)(((uint64_t)cols + kBlock - 1) / kBlock);
-    a.q1 = (uint8_t*)q1_dev, a.q0 = (uint8_t*)q0_dev, a.s1 = (uint8_t*)s1_dev, a.s0 = (uint8_t*)s0_dev;
-    a.colsum = colsum_dev;
-    a.vec = (uintptr_t)x_dev % 16 == 0 && (ld * esize) % 16 == 0;
-    const uint64_t tiles = (uint64_t)a.row_blocks * a.col_blocks;
-    if (tiles > 0x7fffffffull || cols > 0xffffff00u || rows > 0xffffff00u) return PS_ERR_LIMIT;
-    cudaStream_t st = (cudaStream_t)stream;
-    if (dtype == PS_DTYPE_F16)
-        launch<__half>(fmt, blocks, a, (uint32_t)tiles, st);
-    else if (dtype == PS_DTYPE_BF16)
-        launch<__nv_bfloat16>(fmt, blocks, a, (uint32_t)tiles, st);
-    else
-        launch<float>(fmt, blocks, a, (uint32_t)tiles, st);
-    return ps_internal::after_launch();
+    return ps_internal::quantize({x_dev, dtype, ld, rows, cols, blocks, fmt, q1_dev, s1_dev, q0_dev, s0_dev, ldq, colsum_dev},
+                                 (cudaStream_t)stream);
 }
 
 int ps_column_sum(const float* partial_dev, uint32_t blocks, uint32_t cols, void* out_dev, int dtype, void* stream)

@@ -12,17 +12,12 @@ import math
 
 import torch
 
-from ._lib import (PS_DISTILL_MAX_K, PS_DISTILL_MAX_VOCAB, PS_DTYPE_BF16, PS_DTYPE_F16, PS_DTYPE_F32,
-                   PS_REDUCE_MEAN, PS_REDUCE_NONE, PS_REDUCE_SUM, PS_TAIL_BUCKET, PS_TAIL_DROP, DistillProblem,
-                   check, lib)
+from ._lib import (PS_DISTILL_MAX_K, PS_DISTILL_MAX_VOCAB, PS_REDUCE_MEAN, PS_REDUCE_NONE, PS_REDUCE_SUM,
+                   PS_TAIL_BUCKET, PS_TAIL_DROP, DistillProblem, check, lib)
+from .block_fp8 import _DTYPES, _on, _stream_ptr
 
-_DTYPES = {torch.float16: PS_DTYPE_F16, torch.bfloat16: PS_DTYPE_BF16, torch.float32: PS_DTYPE_F32}
 _TAILS = {"drop": PS_TAIL_DROP, "bucket": PS_TAIL_BUCKET}
 _REDUCTIONS = {"none": PS_REDUCE_NONE, "sum": PS_REDUCE_SUM, "mean": PS_REDUCE_MEAN}
-
-
-def _stream_ptr(device):
-    return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
 def _like_rows(z):
@@ -44,53 +39,58 @@ def _point(problem, z, idx, teacher, mask):
     return problem
 
 
+def _forward(z, idx, teacher, mask, problem, scaler):
+    """(loss or row losses, buffer of what backward needs, gradient or None).  The buffer's floats: 1 / rows kept,
+    the scale of the gradient, two unused ones, four for each row."""
+    dev, rows = z.device, z.shape[0]
+    reduce = problem.reduction != PS_REDUCE_NONE
+    out = torch.empty(() if reduce else rows, dtype=torch.float32, device=dev)
+    buf = torch.empty(4 + (5 if reduce else 4) * rows, dtype=torch.float32, device=dev)
+    grad = _like_rows(z) if scaler is not None and rows else None
+    at, o = buf.data_ptr(), out.data_ptr()
+    _point(problem, z, idx, teacher, mask)
+    with _on(dev):
+        check(lib.ps_distill_forward(
+            C.byref(problem), o if reduce else None, at + 16 + 16 * rows if reduce else o, at + 16, at,
+            scaler.state_ptr if grad is not None else None, grad.data_ptr() if grad is not None else None,
+            grad.stride(0) if grad is not None and rows > 1 else z.shape[1], at + 4, _stream_ptr(dev)),
+            "ps_distill_forward")
+    return out, buf, grad
+
+
 class _Distill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, z, idx, teacher, mask, problem, scaler):
-        dev, rows = z.device, z.shape[0]
-        _point(problem, z, idx, teacher, mask)
-        f32 = dict(dtype=torch.float32, device=dev)
-        row_loss, stats = torch.empty(rows, **f32), torch.empty((rows, 4), **f32)
-        reduce = problem.reduction != PS_REDUCE_NONE
-        loss = torch.empty((), **f32) if reduce else None
-        inv_n = torch.empty(1, **f32) if problem.reduction == PS_REDUCE_MEAN and mask is not None else None
-        grad = used = None
-        if scaler is not None and rows:
-            grad, used = _like_rows(z), torch.empty(1, **f32)
-        with torch.cuda.device(dev):
-            check(lib.ps_distill_forward(
-                C.byref(problem), loss.data_ptr() if reduce else None, row_loss.data_ptr(), stats.data_ptr(),
-                inv_n.data_ptr() if inv_n is not None else None, scaler.state_ptr if grad is not None else None,
-                grad.data_ptr() if grad is not None else None, grad.stride(0) if grad is not None and rows > 1 else
-                z.shape[1], used.data_ptr() if used is not None else None, _stream_ptr(dev)), "ps_distill_forward")
-        ctx.save_for_backward(z, idx, teacher, mask, stats, inv_n, used)
-        ctx.problem, ctx.grad = problem, grad
-        return loss if reduce else row_loss
+        out, buf, ctx.grad = _forward(z, idx, teacher, mask, problem, scaler)
+        ctx.save_for_backward(z, idx, teacher, mask, buf)
+        ctx.problem = problem
+        return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
-        z, idx, teacher, mask, stats, inv_n, used = ctx.saved_tensors
-        rows = z.shape[0]
+        z, idx, teacher, mask, buf = ctx.saved_tensors
+        rows, at = z.shape[0], buf.data_ptr()
         _point(ctx.problem, z, idx, teacher, mask)   # saved tensors may come back elsewhere
         # the forward call's gradient is handed out once: what receives it may add to it in place
         grad, ctx.grad = ctx.grad, None
+        used = at + 4 if grad is not None else None
         if grad is None:
-            grad, used = _like_rows(z), None
-        g = grad_out.to(torch.float32)
+            grad = _like_rows(z)
+        g = grad_out if grad_out.dtype == torch.float32 else grad_out.to(torch.float32)
         if g.dim() and g.stride(0) not in (0, 1):
             g = g.contiguous()
-        with torch.cuda.device(z.device):
+        with _on(z.device):
             check(lib.ps_distill_backward(
-                C.byref(ctx.problem), stats.data_ptr(), inv_n.data_ptr() if inv_n is not None else None, g.data_ptr(),
-                g.stride(0) if g.dim() and rows > 1 else 0, used.data_ptr() if used is not None else None,
+                C.byref(ctx.problem), at + 16, at, g.data_ptr(), g.stride(0) if g.dim() and rows > 1 else 0, used,
                 grad.data_ptr(), grad.stride(0) if rows > 1 else z.shape[1], _stream_ptr(z.device)),
                 "ps_distill_backward")
         return grad, None, None, None, None, None
 
 
 def _rows(t, width):
-    t = t.detach().reshape(math.prod(t.shape[:-1]), width)
+    if t.dim() != 2:
+        t = t.reshape(math.prod(t.shape[:-1]), width)
     return t if t.stride(1) == 1 or width == 1 else t.contiguous()
 
 
@@ -156,19 +156,16 @@ def distillation_loss(logits, indices, teacher, *, temperature=1.0, tail="drop",
             raise ValueError("distillation_loss: a scaler goes with one loss, not with reduction none")
         if scaler.device != logits.device:
             raise ValueError("distillation_loss: logits on %s, the scaler on %s" % (logits.device, scaler.device))
-        if not (torch.is_grad_enabled() and logits.requires_grad):
-            scaler = None
-    z = logits.reshape(math.prod(logits.shape[:-1]), vocab)
-    if z.stride(1) != 1 and vocab > 1:
-        z = z.contiguous()
-    idx, values = _rows(indices, k), _rows(teacher, k)
+    z = _rows(logits, vocab)
+    idx, values = _rows(indices, k), _rows(teacher.detach() if teacher.requires_grad else teacher, k)
     if mask is not None:
-        mask = mask.detach().reshape(-1).contiguous()
-    problem = DistillProblem(
-        rows=z.shape[0], vocab=vocab, k=k, dtype=_DTYPES[z.dtype], index_bytes=idx.element_size(),
-        teacher_dtype=_DTYPES[values.dtype], tail=_TAILS[tail], reduction=_REDUCTIONS[reduction],
-        temperature=temperature, weight=weight)
-    out = _Distill.apply(z, idx, values, mask, problem, scaler)
+        mask = mask.reshape(-1).contiguous()
+    problem = DistillProblem(None, None, None, None, 0, 0, 0, z.shape[0], vocab, k, _DTYPES[z.dtype], idx.element_size(),
+                             _DTYPES[values.dtype], _TAILS[tail], _REDUCTIONS[reduction], temperature, weight)
+    if torch.is_grad_enabled() and z.requires_grad:
+        out = _Distill.apply(z, idx, values, mask, problem, scaler)
+    else:
+        out = _forward(z, idx, values, mask, problem, None)[0]
     return out.view(logits.shape[:-1]) if reduction == "none" else out
 
 
