@@ -615,7 +615,7 @@ int ps_block_matmul_gave_up(uint32_t* count);
 #define PS_REDUCE_SUM 1
 #define PS_REDUCE_MEAN 2 /* over the rows that the mask keeps, or 1 if it keeps none */
 
-#define PS_DISTILL_MAX_VOCAB (1u << 20)
+#define PS_DISTILL_MAX_VOCAB (1u << 20) /* half of it with PS_TAIL_BUCKET */
 #define PS_DISTILL_MAX_K 1024
 
 typedef struct ps_distill_problem {

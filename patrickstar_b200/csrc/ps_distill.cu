@@ -14,11 +14,10 @@
 // One CTA takes a row: one pass with a running maximum and sum of its own in
 // every thread, joined at the end; and for the gradient a second pass that reads
 // the row again, from L2 when it follows the first (148 SMs hold a few rows each,
-// 0.1 to 0.5 MB a row).  Subtracting the maximum before scaling keeps every
-// finite logit in range (a row of the type's lowest value is a uniform one).
+// 0.1 to 0.5 MB a row).
 // The listed entries are few: one warp works on them in 64 bits beside the
 // others' pass.  Their gradient is written over the row's after it, so the pass
-// itself knows nothing of them.  HBM-bound: one read, and one write for the
+// itself knows nothing of them but, for the bucket, one bit per element.  HBM-bound: one read, and one write for the
 // gradient; a power of two per element each pass.
 #include "ps_b200.h"
 
@@ -31,8 +30,9 @@
 
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
+constexpr int kMaxThreads = 512;
+constexpr uint64_t kRowsInL2 = 64ull << 20;  // bytes of rows in work, of 126 MB
+constexpr int kUnroll = 4;  // 16-byte loads in flight a thread
 
 struct DistillArgs {
     const void* z;
@@ -69,6 +69,17 @@ struct Type;
 template <>
 struct Type<__half> {
     static constexpr int kVec = 8;
+    static constexpr uint32_t kNothing = 0xfc00fc00u;  // minus infinities
+    static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b)
+    {
+        const __half2 h = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ float fold(uint32_t a)
+    {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a));
+        return fmaxf(f.x, f.y);
+    }
     static __device__ __forceinline__ float load(const __half* p) { return __half2float(*p); }
     static __device__ __forceinline__ __half round(float f) { return __float2half_rn(f); }
     static __device__ __forceinline__ void unpack(const uint4& q, float (&f)[8])
@@ -94,6 +105,17 @@ struct Type<__half> {
 template <>
 struct Type<__nv_bfloat16> {
     static constexpr int kVec = 8;
+    static constexpr uint32_t kNothing = 0xff80ff80u;
+    static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b)
+    {
+        const __nv_bfloat162 h =
+            __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ float fold(uint32_t a)
+    {
+        return fmaxf(__uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u));
+    }
     static __device__ __forceinline__ float load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
     static __device__ __forceinline__ __nv_bfloat16 round(float f) { return __float2bfloat16_rn(f); }
     static __device__ __forceinline__ void unpack(const uint4& q, float (&f)[8])
@@ -119,6 +141,12 @@ struct Type<__nv_bfloat16> {
 template <>
 struct Type<float> {
     static constexpr int kVec = 4;
+    static constexpr uint32_t kNothing = 0xff800000u;
+    static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b)
+    {
+        return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    }
+    static __device__ __forceinline__ float fold(uint32_t a) { return __uint_as_float(a); }
     static __device__ __forceinline__ float load(const float* p) { return *p; }
     static __device__ __forceinline__ float round(float f) { return f; }
     static __device__ __forceinline__ void unpack(const uint4& q, float (&f)[4])
@@ -185,255 +213,408 @@ __device__ __forceinline__ uint32_t bit_of(const RowShape& s, uint32_t v)
     return u < s.vecs * E ? u : u + s.head;
 }
 
-// Running maximum and sums of one thread.
+// Two 32-bit operations in one instruction.
+struct Pair {
+    uint64_t v;
+    __device__ __forceinline__ Pair() {}
+    __device__ __forceinline__ Pair(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y)); }
+    __device__ __forceinline__ float2 get() const
+    {
+        float2 f;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+        return f;
+    }
+};
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c)
+{
+    Pair d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return d;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b)
+{
+    Pair d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+    return d;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b)
+{
+    Pair d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+    return d;
+}
+
+// What a row's powers of two are relative to: the exponent of element z is z c - r, one rounding, with
+// r = m c rounded and m the largest element.  r itself is the reference, so its rounding does not matter, as
+// long as it moves the largest exponent by less than 2^5: |r| < 2^30.  Beyond that (logits near the end of
+// their type, or tiny temperatures) the exponent is (z - m) c.
+struct Origin {
+    float m = -INFINITY, r = 0.f;
+    bool far = false;
+    __device__ __forceinline__ Origin() {}
+    __device__ __forceinline__ Origin(float top, float c) : m(top)
+    {
+        r = m == -INFINITY ? 0.f : m * c;
+        far = fabsf(r) >= 1073741824.f && fabsf(m) < INFINITY;
+    }
+    __device__ __forceinline__ float exponent(float z, float c) const
+    {
+        return far ? (z - m) * c : fmaf(z, c, -r);
+    }
+    // of sums relative to this one, to make them relative to `to` (no smaller)
+    __device__ __forceinline__ float factor(const Origin& to, float c) const
+    {
+        if (m == -INFINITY) return 1.f;  // sums of 0 (or NaN): they stay themselves
+        return ex2(far || to.far ? (m - to.m) * c : r - to.r);
+    }
+};
+
+// Running origin and sums of one thread: of elements outside of S, and of those in it.
 struct Running {
-    float m = -INFINITY, out = 0.f, in = 0.f;
+    Origin o;
+    Pair out = Pair(0.f, 0.f);
+    float in = 0.f;
     __device__ __forceinline__ void raise(float top, float c)
     {
-        if (top > m) {
-            const float f = ex2((m - top) * c);
-            out *= f, in *= f;
-            m = top;
+        if (top > o.m) {
+            const Origin to(top, c);
+            const float f = o.factor(to, c);
+            out = mul2(out, Pair(f, f)), in *= f;
+            o = to;
         }
     }
-    __device__ __forceinline__ float origin() const { return m == -INFINITY ? 0.f : m; }
 };
 
 constexpr int kLoss = 1, kGrad = 2;
 
+// One row's listed entries and what the pass over it found; two of them, in turn.
+struct RowSlot {
+    double rest, mass;  // p_r, and sum p + p_r: 1 unless the teacher gives nothing, or too much
+    float M, out, in;   // largest logit, sums outside of S and in it
+    float inside, outside;  // factors of e_v in the gradient
+    int keep, bad;      // the mask keeps the row; an index is outside of the vocabulary
+};
+struct Listed {
+    double *p, *log_p;  // probabilities and their logarithms
+    int* idx;           // or -1
+    float* z;           // logits
+    uint32_t* bits;
+};
+__host__ __device__ __forceinline__ uint32_t bitmap_words(uint32_t vocab) { return (vocab + 63) / 64 * 2; }
+
+__device__ __forceinline__ float grad_factor(const DistillArgs& a, float scale)
+{
+    return (float)((double)scale * (double)a.weight * (double)a.temperature *
+                   (double)(a.inv_n != nullptr ? *a.inv_n : a.inv_n_value));
+}
+
+// The listed entries of a row, by one warp, before the pass over it.
 template <typename T, bool kBucket, int kWhat>
-__global__ void __launch_bounds__(kThreads) distill_kernel(const DistillArgs a)
+__device__ void entries_before(const DistillArgs& a, uint32_t row, RowSlot& slot, const Listed& l)
+{
+    const uint32_t lane = threadIdx.x & 31;
+    const bool keep = a.mask == nullptr || a.mask[row] != 0;
+    if (lane == 0) slot.keep = keep, slot.bad = 0;
+    if (!keep) return;
+    const T* const z = reinterpret_cast<const T*>(a.z) + (uint64_t)row * a.ldz;
+    const RowShape shape = row_shape(z, a.vocab);
+    const double inv_t = 1.0 / (double)a.temperature;
+    bool bad = false;
+    double tmax = -INFINITY, tsum = 0.0;
+    for (uint32_t j = lane; j < a.k; j += 32) {
+        const long long v = index_at(a, (uint64_t)row * a.ld_idx + j);
+        const double t = teacher_at(a, (uint64_t)row * a.ld_teacher + j);
+        const bool listed = v >= 0 && v < (long long)a.vocab;
+        if (!listed && v != -1) bad = true;
+        l.idx[j] = listed ? (int)v : -1;
+        l.log_p[j] = t;
+        if (listed) {
+            l.z[j] = Type<T>::load(z + v);
+            if (kBucket && (kWhat & kLoss)) {
+                const uint32_t bit = bit_of<T>(shape, (uint32_t)v);
+                atomicOr(&l.bits[bit >> 5], 1u << (bit & 31));
+            }
+            tmax = (t > tmax || t != t) ? t : tmax;
+        }
+    }
+    if (!kBucket) tmax = warp_max(tmax);
+    const double origin = kBucket || tmax == -INFINITY ? 0.0 : tmax;
+    for (uint32_t j = lane; j < a.k; j += 32) {
+        const double x = kBucket ? l.log_p[j] : (l.log_p[j] - origin) * inv_t;
+        const double p = l.idx[j] >= 0 ? exp(x) : 0.0;
+        l.log_p[j] = x, l.p[j] = p;
+        tsum += p;
+    }
+    tsum = warp_sum(tsum);
+    double rest = 0.0, mass = tsum;
+    if (!kBucket) {
+        mass = tsum == 0.0 ? 0.0 : tsum / tsum;  // a NaN stays
+        const double inv = tsum == 0.0 ? 0.0 : 1.0 / tsum, log_sum = log(tsum);
+        for (uint32_t j = lane; j < a.k; j += 32) l.p[j] *= inv, l.log_p[j] -= log_sum;
+    } else if (kWhat & kLoss) {
+        bool all = false;  // the whole vocabulary is listed
+        if (a.k >= a.vocab) {
+            __syncwarp();
+            uint32_t n = 0;
+            for (uint32_t i = lane; i < (a.vocab + 31) / 32; i += 32) n += __popc(l.bits[i]);
+            all = __reduce_add_sync(0xffffffffu, n) == a.vocab;
+        }
+        rest = tsum != tsum ? tsum : (tsum < 1.0 && !all ? 1.0 - tsum : 0.0);
+        mass = tsum + rest;
+    }
+    bad = __any_sync(0xffffffffu, bad);
+    if (lane == 0) slot.rest = rest, slot.mass = mass, slot.bad = bad;
+}
+
+// ... and after it: the row's loss, and the gradient of the listed elements over what the pass wrote there.
+template <typename T, bool kBucket, int kWhat>
+__device__ void entries_after(const DistillArgs& a, uint32_t row, const RowSlot& slot, const Listed& l, float c, float scale)
+{
+    const uint32_t lane = threadIdx.x & 31;
+    if (!slot.keep) return;
+    const Origin o(slot.M, c);
+    if (kWhat & kLoss) {
+        const double log_z = log((double)(slot.out + slot.in));
+        double t = 0.0;
+        for (uint32_t j = lane; j < a.k; j += 32) {
+            const double x = o.far ? ((double)l.z[j] - (double)slot.M) * (double)c : (double)l.z[j] * (double)c - (double)o.r;
+            const double p = l.p[j];
+            if (l.idx[j] >= 0 && p != 0.0) t += p * (l.log_p[j] - (x * 0.6931471805599453 - log_z));
+        }
+        t = warp_sum(t);
+        if (kBucket && !(slot.rest <= 0.0)) t += slot.rest * (log(slot.rest) - (log((double)slot.out) - log_z));
+        if (slot.bad) t = (double)NAN;
+        if (lane == 0) a.row_loss[row] = (float)(t * (double)a.weight * (double)a.temperature * (double)a.temperature);
+    }
+    if (kWhat & kGrad) {
+        T* const g = reinterpret_cast<T*>(a.grad) + (uint64_t)row * a.ldg;
+        if (!(kWhat & kLoss)) scale = a.grad_out[(uint64_t)row * a.grad_out_stride];
+        const float gf = slot.bad ? NAN : grad_factor(a, scale);
+        for (uint32_t j = lane; j < a.k; j += 32) {
+            const int v = l.idx[j];
+            if (v < 0) continue;
+            float p = 0.f;
+            for (uint32_t i = 0; i < a.k; ++i)
+                if (l.idx[i] == v) p += (float)l.p[i];
+            g[v] = Type<T>::round((ex2(o.exponent(l.z[j], c)) * slot.inside - p) * gf);
+        }
+    }
+    if (kBucket && (kWhat & kLoss)) {  // the bitmap is zeros again
+        __syncwarp();
+        const T* const z = reinterpret_cast<const T*>(a.z) + (uint64_t)row * a.ldz;
+        const RowShape shape = row_shape(z, a.vocab);
+        for (uint32_t j = lane; j < a.k; j += 32)
+            if (l.idx[j] >= 0) l.bits[bit_of<T>(shape, (uint32_t)l.idx[j]) >> 5] = 0;
+        __syncwarp();
+    }
+}
+
+// All warps but the last pass over rows; the last one works on the listed entries of the row before and of the
+// row after meanwhile, so that their chains of 64-bit logarithms and scattered loads hide behind the pass.
+template <typename T, bool kBucket, int kWhat>
+__global__ void __launch_bounds__(kMaxThreads, 2) distill_kernel(const DistillArgs a)
 {
     constexpr int E = Type<T>::kVec;
-    extern __shared__ uint32_t smem[];
-    // listed entries: index (or -1), probability, logit; then the bitmap
-    int* const s_idx = reinterpret_cast<int*>(smem);
-    float* const s_p = reinterpret_cast<float*>(smem + a.k);
-    float* const s_z = reinterpret_cast<float*>(smem + 2 * a.k);
-    uint32_t* const s_bits = smem + 3 * a.k;
-    __shared__ float s_m[kWarps], s_out[kWarps], s_in[kWarps];
-    __shared__ double s_rest, s_mass;  // p_r, and sum p + p_r: 1 unless the teacher gives nothing, or too much
-    __shared__ int s_bad;
-
+    extern __shared__ double smem[];
+    __shared__ RowSlot slots[2];
+    __shared__ float s_m[kMaxThreads / 32], s_out[kMaxThreads / 32], s_in[kMaxThreads / 32];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t threads = blockDim.x - 32, warps = threads >> 5;  // of the pass
     const float c = (float)(1.4426950408889634 / (double)a.temperature);
-    const double inv_t = 1.0 / (double)a.temperature;
+    Listed listed[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        listed[i].p = smem + 2 * i * a.k;
+        listed[i].log_p = smem + (2 * i + 1) * a.k;
+        listed[i].idx = reinterpret_cast<int*>(smem + 4 * a.k) + 2 * i * a.k;
+        listed[i].z = reinterpret_cast<float*>(smem + 4 * a.k) + (2 * i + 1) * a.k;
+        listed[i].bits = reinterpret_cast<uint32_t*>(smem + 6 * a.k) + i * bitmap_words(a.vocab);
+    }
 
     if ((kWhat & kLoss) == 0 && a.used_scale != nullptr && *a.used_scale == *a.grad_out)
         return;  // the forward pass wrote this gradient
     float scale = 1.f;
-    if (kWhat & kGrad) {
-        if (kWhat & kLoss) {
-            scale = a.scaler->dynamic < 0 ? 1.f : (float)a.scaler->cur_scale;
-            if (blockIdx.x == 0 && threadIdx.x == 0) *a.used_scale = scale;
-        }
+    if ((kWhat & kGrad) && (kWhat & kLoss)) {
+        scale = a.scaler->dynamic < 0 ? 1.f : (float)a.scaler->cur_scale;
+        if (blockIdx.x == 0 && threadIdx.x == 0) *a.used_scale = scale;
     }
+    if (kBucket && (kWhat & kLoss)) {
+        for (uint32_t i = threadIdx.x; i < 2 * bitmap_words(a.vocab); i += blockDim.x) listed[0].bits[i] = 0;
+        __syncthreads();
+    }
+    if (warp == warps) entries_before<T, kBucket, kWhat>(a, blockIdx.x, slots[0], listed[0]);
 
-    for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    uint32_t it = 0;
+    for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x, ++it) {
+        __syncthreads();  // this row's entries are there, the row before is written
+        RowSlot& slot = slots[it & 1];
+        if (warp == warps) {
+            const Listed& other = listed[(it + 1) & 1];
+            if (it > 0) entries_after<T, kBucket, kWhat>(a, row - gridDim.x, slots[(it + 1) & 1], other, c, scale);
+            __syncwarp();
+            if (row + gridDim.x < a.rows)
+                entries_before<T, kBucket, kWhat>(a, row + gridDim.x, slots[(it + 1) & 1], other);
+            continue;
+        }
         const T* const z = reinterpret_cast<const T*>(a.z) + (uint64_t)row * a.ldz;
         T* const g = reinterpret_cast<T*>(a.grad) + (uint64_t)row * a.ldg;
-        const RowShape shape = row_shape(z, a.vocab);
-        const bool same_offset = (((uintptr_t)z ^ (uintptr_t)g) & 15u) == 0;
-        if (a.mask != nullptr && a.mask[row] == 0) {
+        if (!slot.keep) {
             if ((kWhat & kLoss) && threadIdx.x == 0) a.row_loss[row] = 0.f, a.stats[row] = make_float4(0.f, 0.f, 0.f, 0.f);
             if (kWhat & kGrad) {
                 const RowShape gs = row_shape(g, a.vocab);
                 uint4* gv = reinterpret_cast<uint4*>(g + gs.head);
-                for (uint32_t i = threadIdx.x; i < gs.vecs; i += kThreads) gv[i] = make_uint4(0, 0, 0, 0);
+                for (uint32_t i = threadIdx.x; i < gs.vecs; i += threads) __stcs(gv + i, make_uint4(0, 0, 0, 0));
                 if (threadIdx.x < gs.head) g[threadIdx.x] = Type<T>::round(0.f);
                 if (threadIdx.x < gs.tail) g[a.vocab - gs.tail + threadIdx.x] = Type<T>::round(0.f);
             }
             continue;
         }
-
-        __syncthreads();  // the row before is done with shared memory
-        if (kBucket && (kWhat & kLoss)) {
-            for (uint32_t i = threadIdx.x; i < (a.vocab + 63) / 32; i += kThreads) s_bits[i] = 0;
-            __syncthreads();
-        }
-        // the listed entries, by the first warp
-        double tmax = -INFINITY, tsum = 0.0;
-        if (warp == 0) {
-            bool bad = false;
-            for (uint32_t j = lane; j < a.k; j += 32) {
-                const long long v = index_at(a, (uint64_t)row * a.ld_idx + j);
-                const double t = teacher_at(a, (uint64_t)row * a.ld_teacher + j);
-                const bool listed = v >= 0 && v < (long long)a.vocab;
-                if (!listed && v != -1) bad = true;
-                s_idx[j] = listed ? (int)v : -1;
-                if (listed) {
-                    s_z[j] = Type<T>::load(z + v);
-                    if (kBucket && (kWhat & kLoss)) {
-                        const uint32_t bit = bit_of<T>(shape, (uint32_t)v);
-                        atomicOr(&s_bits[bit >> 5], 1u << (bit & 31));
-                    }
-                    tmax = (t > tmax || t != t) ? t : tmax;
-                }
-            }
-            tmax = warp_max(tmax);
-            if (!kBucket) {
-                const double origin = tmax == -INFINITY ? 0.0 : tmax;
-                for (uint32_t j = lane; j < a.k; j += 32)
-                    if (s_idx[j] >= 0) tsum += exp((teacher_at(a, (uint64_t)row * a.ld_teacher + j) - origin) * inv_t);
-                tsum = warp_sum(tsum);
-                for (uint32_t j = lane; j < a.k; j += 32)
-                    s_p[j] = s_idx[j] >= 0 && tsum != 0.0
-                                 ? (float)(exp((teacher_at(a, (uint64_t)row * a.ld_teacher + j) - origin) * inv_t) / tsum)
-                                 : 0.f;
-                if (lane == 0) s_mass = tsum == 0.0 ? 0.0 : tsum / tsum;  // a NaN stays
-            } else {
-                for (uint32_t j = lane; j < a.k; j += 32) {
-                    const double p = s_idx[j] >= 0 ? exp(teacher_at(a, (uint64_t)row * a.ld_teacher + j)) : 0.0;
-                    s_p[j] = (float)p;
-                    tsum += p;
-                }
-                tsum = warp_sum(tsum);
-                bool all = false;  // the whole vocabulary is listed
-                if ((kWhat & kLoss) && a.k >= a.vocab) {
-                    __syncwarp();
-                    uint32_t n = 0;
-                    for (uint32_t i = lane; i < (a.vocab + 31) / 32; i += 32) n += __popc(s_bits[i]);
-                    all = __reduce_add_sync(0xffffffffu, n) == a.vocab;
-                }
-                if (lane == 0) {
-                    s_rest = tsum != tsum ? tsum : (tsum < 1.0 && !all ? 1.0 - tsum : 0.0);
-                    s_mass = tsum + s_rest;
-                }
-            }
-            bad = __any_sync(0xffffffffu, bad);
-            if (lane == 0) s_bad = bad;
-        }
-        if (kBucket && (kWhat & kLoss)) __syncthreads();
-
-        float M, inside, outside;
+        const RowShape shape = row_shape(z, a.vocab);
+        const uint4* zv = reinterpret_cast<const uint4*>(z + shape.head);
+        float M, outside;
         if (kWhat & kLoss) {
-            Running r;
-            const uint4* zv = reinterpret_cast<const uint4*>(z + shape.head);
-            const uint8_t* bytes = reinterpret_cast<const uint8_t*>(s_bits);
-            for (uint32_t i = threadIdx.x; i < shape.vecs; i += kThreads) {
-                float f[E];
-                Type<T>::unpack(zv[i], f);
-                float top = f[0];
+            Running run;
+            const uint32_t* const bits = listed[it & 1].bits;
+            const uint8_t* bytes = reinterpret_cast<const uint8_t*>(bits);
+            for (uint32_t i0 = threadIdx.x; i0 < shape.vecs; i0 += kUnroll * threads) {
+                uint4 q[kUnroll];
 #pragma unroll
-                for (int j = 1; j < E; ++j) top = fmaxf(top, f[j]);
-                r.raise(top, c);
-                const float o = r.origin();
-                uint32_t in = 0;
-                if (kBucket) in = E == 8 ? bytes[i] : (bytes[i >> 1] >> (4 * (i & 1))) & 15u;
-                if (in == 0) {
+                for (int u = 0; u < kUnroll; ++u) {
+                    const uint32_t i = i0 + u * threads;
+                    q[u] = make_uint4(Type<T>::kNothing, Type<T>::kNothing, Type<T>::kNothing, Type<T>::kNothing);
+                    if (i < shape.vecs) q[u] = (kWhat & kGrad) ? __ldg(zv + i) : __ldcs(zv + i);
+                }
+                uint32_t top = Type<T>::kNothing;
 #pragma unroll
-                    for (int j = 0; j < E; ++j) r.out += ex2((f[j] - o) * c);
-                } else {
+                for (int u = 0; u < kUnroll; ++u)
+                    top = Type<T>::larger(top, Type<T>::larger(Type<T>::larger(q[u].x, q[u].y), Type<T>::larger(q[u].z, q[u].w)));
+                run.raise(Type<T>::fold(top), c);
+uint32_t in[kUnroll], any = run.o.far ? 1u : 0u;
+                if (kBucket) {
 #pragma unroll
-                    for (int j = 0; j < E; ++j) {
-                        const float e = ex2((f[j] - o) * c);
-                        if ((in >> j) & 1)
-                            r.in += e;
-                        else
-                            r.out += e;
+                    for (int u = 0; u < kUnroll; ++u) {
+                        const uint32_t i = min(i0 + u * threads, shape.vecs - 1);
+                        in[u] = E == 8 ? bytes[i] : (bytes[i >> 1] >> (4 * (i & 1))) & 15u;
+                        any |= in[u];
                     }
                 }
+                if (any == 0) {
+                    const Pair c2(c, c), r2(-run.o.r, -run.o.r);
+#pragma unroll
+                    for (int u = 0; u < kUnroll; ++u) {
+                        float f[E];
+                        Type<T>::unpack(q[u], f);
+#pragma unroll
+                        for (int j = 0; j < E; j += 2) {
+                            const float2 x = fma2(Pair(f[j], f[j + 1]), c2, r2).get();
+                            run.out = add2(run.out, Pair(ex2(x.x), ex2(x.y)));
+                        }
+                    }
+                } else {
+                    float out = 0.f;
+#pragma unroll
+                    for (int u = 0; u < kUnroll; ++u) {
+                        float f[E];
+                        Type<T>::unpack(q[u], f);
+#pragma unroll
+                        for (int j = 0; j < E; ++j) {
+                            const float e = ex2(run.o.exponent(f[j], c));
+                            if (kBucket && ((in[u] >> j) & 1))
+                                run.in += e;
+                            else
+                                out += e;
+                        }
+                    }
+                    run.out = add2(run.out, Pair(out, 0.f));
+                }
             }
-            for (uint32_t i = threadIdx.x; i < shape.head + shape.tail; i += kThreads) {
+            for (uint32_t i = threadIdx.x; i < shape.head + shape.tail; i += threads) {
                 const uint32_t v = i < shape.head ? i : i + shape.vecs * E;
                 const float f = Type<T>::load(z + v);
-                r.raise(f, c);
-                const float e = ex2((f - r.origin()) * c);
+                run.raise(f, c);
+                const float e = ex2(run.o.exponent(f, c));
                 bool in = false;
                 if (kBucket) {
                     const uint32_t bit = bit_of<T>(shape, v);
-                    in = (s_bits[bit >> 5] >> (bit & 31)) & 1;
+                    in = (bits[bit >> 5] >> (bit & 31)) & 1;
                 }
                 if (in)
-                    r.in += e;
+                    run.in += e;
                 else
-                    r.out += e;
+                    run.out = add2(run.out, Pair(e, 0.f));
             }
             // join the threads
-            float m = r.m;
+            float m = run.o.m;
 #pragma unroll
             for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-            float o = m == -INFINITY ? 0.f : m;
-            const float f = r.m == -INFINITY ? 1.f : ex2((r.m - o) * c);  // sums of 0 (or NaN) stay themselves
-            const float w_out = warp_sum(r.out * f), w_in = warp_sum(r.in * f);
+            const float f = run.o.factor(Origin(m, c), c);
+            const float2 two = run.out.get();
+            const float w_out = warp_sum((two.x + two.y) * f), w_in = warp_sum(run.in * f);
             if (lane == 0) s_m[warp] = m, s_out[warp] = w_out, s_in[warp] = w_in;
-            __syncthreads();
-            M = s_m[0];
+            asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory");  // the warps of the pass
+            M = lane < warps ? s_m[lane] : -INFINITY;
+            float out = lane < warps ? s_out[lane] : 0.f, in = lane < warps ? s_in[lane] : 0.f;
+            const Origin mine(M, c);
 #pragma unroll
-            for (int w = 1; w < kWarps; ++w) M = fmaxf(M, s_m[w]);
-            o = M == -INFINITY ? 0.f : M;
-            float out = 0.f, in = 0.f;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float fw = s_m[w] == -INFINITY ? 1.f : ex2((s_m[w] - o) * c);
-                out += s_out[w] * fw, in += s_in[w] * fw;
-            }
-            const float Z = out + in;
-            inside = (float)s_mass / Z;
+            for (int d = 16; d; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+            const float fw = mine.factor(Origin(M, c), c);
+            out = warp_sum(out * fw), in = warp_sum(in * fw);
+            const float inside = (float)slot.mass / (out + in);
             outside = inside;
-            if (kBucket && s_rest > 0.0) outside = inside - (float)(s_rest / (double)out);
-            if (warp == 0) {
-                const double log_z = log((double)Z);
-                double t = 0.0;
-                for (uint32_t j = lane; j < a.k; j += 32) {
-                    if (s_idx[j] < 0) continue;
-                    const double x = teacher_at(a, (uint64_t)row * a.ld_teacher + j);
-                    const double log_p = kBucket ? x : (x - tmax) * inv_t - log(tsum);
-                    const double p = kBucket ? exp(x) : exp((x - (tmax == -INFINITY ? 0.0 : tmax)) * inv_t) / tsum;
-                    const double log_q = ((double)s_z[j] - (double)M) * inv_t - log_z;
-                    if (p != 0.0 && (kBucket || tsum != 0.0)) t += p * (log_p - log_q);
-                }
-                t = warp_sum(t);
-                if (kBucket && !(s_rest <= 0.0)) t += s_rest * (log(s_rest) - (log((double)out) - log_z));
-                if (s_bad) t = (double)NAN;
-                if (lane == 0) {
-                    a.row_loss[row] = (float)(t * (double)a.weight * (double)a.temperature * (double)a.temperature);
-                    a.stats[row] = make_float4(M, inside, outside, 0.f);
-                }
+            if (kBucket && slot.rest > 0.0) outside = inside - (float)(slot.rest / (double)out);
+            if (threadIdx.x == 0) {
+                slot.M = M, slot.out = out, slot.in = in, slot.inside = inside;
+                a.stats[row] = make_float4(M, inside, outside, 0.f);
             }
         } else {
             const float4 st = a.stats[row];
-            M = st.x, inside = st.y, outside = st.z;
+            M = st.x, outside = st.z;
+            if (threadIdx.x == 0) slot.M = M, slot.inside = st.y;
         }
 
         if (kWhat & kGrad) {
-            if (!(kWhat & kLoss)) {
-                scale = a.grad_out[(uint64_t)row * a.grad_out_stride];
-                __syncthreads();  // the listed entries
-            }
-            float gf = (float)((double)scale * (double)a.weight * (double)a.temperature *
-                               (double)(a.inv_n != nullptr ? *a.inv_n : a.inv_n_value));
-            if (s_bad) gf = NAN;
-            const float k_out = outside * gf;
-            const uint4* zv = reinterpret_cast<const uint4*>(z + shape.head);
-            if (same_offset) {
+            if (!(kWhat & kLoss)) scale = a.grad_out[(uint64_t)row * a.grad_out_stride];
+            const float k_out = outside * (slot.bad ? NAN : grad_factor(a, scale));
+            const Origin o(M, c);
+            if ((((uintptr_t)z ^ (uintptr_t)g) & 15u) == 0 && !o.far) {
                 uint4* gv = reinterpret_cast<uint4*>(g + shape.head);
-                for (uint32_t i = threadIdx.x; i < shape.vecs; i += kThreads) {
-                    float f[E];
-                    Type<T>::unpack(zv[i], f);
+                const Pair c2(c, c), r2(-o.r, -o.r), k2(k_out, k_out);
+                for (uint32_t i0 = threadIdx.x; i0 < shape.vecs; i0 += kUnroll * threads) {
+                    uint4 q[kUnroll];
 #pragma unroll
-                    for (int j = 0; j < E; ++j) f[j] = ex2((f[j] - M) * c) * k_out;
-                    gv[i] = Type<T>::pack(f);
+                    for (int u = 0; u < kUnroll; ++u) {
+                        const uint32_t i = i0 + u * threads;
+                        if (i < shape.vecs) q[u] = __ldcs(zv + i);
+                    }
+#pragma unroll
+                    for (int u = 0; u < kUnroll; ++u) {
+                        const uint32_t i = i0 + u * threads;
+                        if (i >= shape.vecs) break;
+                        float f[E];
+                        Type<T>::unpack(q[u], f);
+#pragma unroll
+                        for (int j = 0; j < E; j += 2) {
+                            const float2 x = fma2(Pair(f[j], f[j + 1]), c2, r2).get();
+                            const float2 y = mul2(Pair(ex2(x.x), ex2(x.y)), k2).get();
+                            f[j] = y.x, f[j + 1] = y.y;
+                        }
+                        __stcs(gv + i, Type<T>::pack(f));
+                    }
                 }
-                for (uint32_t i = threadIdx.x; i < shape.head + shape.tail; i += kThreads) {
+                for (uint32_t i = threadIdx.x; i < shape.head + shape.tail; i += threads) {
                     const uint32_t v = i < shape.head ? i : i + shape.vecs * E;
-                    g[v] = Type<T>::round(ex2((Type<T>::load(z + v) - M) * c) * k_out);
+                    g[v] = Type<T>::round(ex2(o.exponent(Type<T>::load(z + v), c)) * k_out);
                 }
             } else {
-                for (uint32_t v = threadIdx.x; v < a.vocab; v += kThreads)
-                    g[v] = Type<T>::round(ex2((Type<T>::load(z + v) - M) * c) * k_out);
-            }
-            __syncthreads();  // the row's gradient is written: now the listed elements over it
-            for (uint32_t j = threadIdx.x; j < a.k; j += kThreads) {
-                const int v = s_idx[j];
-                if (v < 0) continue;
-                float p = 0.f;
-                for (uint32_t i = 0; i < a.k; ++i)
-                    if (s_idx[i] == v) p += s_p[i];
-                g[v] = Type<T>::round((ex2((s_z[j] - M) * c) * inside - p) * gf);
+                for (uint32_t v = threadIdx.x; v < a.vocab; v += threads)
+                    g[v] = Type<T>::round(ex2(o.exponent(Type<T>::load(z + v), c)) * k_out);
             }
         }
     }
+    __syncthreads();
+    if (warp == warps && it > 0)
+        entries_after<T, kBucket, kWhat>(a, blockIdx.x + (it - 1) * gridDim.x, slots[(it - 1) & 1], listed[(it - 1) & 1], c,
+                                         scale);
 }
 
 // 1 / max(1, rows kept)
@@ -471,7 +652,7 @@ int launch(const DistillArgs& a, cudaStream_t st)
 {
     const int sms = ps_internal::sm_count();
     if (sms < 0) return sms;
-    const size_t smem = 12 * (size_t)a.k + (kBucket && (kWhat & kLoss) ? ((size_t)(a.vocab + 63) / 32) * 4 : 0);
+    const size_t smem = 48 * (size_t)a.k + (kBucket && (kWhat & kLoss) ? 8 * (size_t)bitmap_words(a.vocab) : 0);
     if (smem > 40 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(distill_kernel<T, kBucket, kWhat>,
                                                    cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -481,8 +662,17 @@ int launch(const DistillArgs& a, cudaStream_t st)
             return PS_ERR_CUDA;
         }
     }
-    const uint32_t most = (uint32_t)sms * 4;
-    distill_kernel<T, kBucket, kWhat><<<a.rows < most ? a.rows : most, kThreads, smem, st>>>(a);
+    // Enough threads for a row to have two rounds of loads at least, and as many rows in work as SMs hold, but
+    // for the gradient no more than L2 keeps until the second pass.
+    const uint64_t bytes = (uint64_t)a.vocab * sizeof(T);
+    const uint32_t threads = bytes <= 16 * 1024 ? 96 : bytes <= 48 * 1024 ? 224 : 480;
+    uint64_t most = 2048 / (threads + 32);
+    if ((kWhat & kLoss) && (kWhat & kGrad)) {
+        const uint64_t fit = kRowsInL2 / ((uint64_t)sms * bytes);
+        most = fit < 2 ? 2 : fit < most ? fit : most;
+    }
+    most *= (uint64_t)sms;
+    distill_kernel<T, kBucket, kWhat><<<a.rows < most ? a.rows : (uint32_t)most, threads + 32, smem, st>>>(a);
     return ps_internal::after_launch();
 }
 template <typename T>
@@ -512,7 +702,9 @@ int check_problem(const ps_distill_problem* q, const float* inv_n)
         return PS_ERR_INVALID;
     if (q->rows == 0) return PS_OK;
     if (q->vocab == 0 || q->k == 0) return PS_ERR_INVALID;
-    if (q->vocab > PS_DISTILL_MAX_VOCAB || q->k > PS_DISTILL_MAX_K) return PS_ERR_LIMIT;
+    if (q->vocab > (q->tail == PS_TAIL_BUCKET ? PS_DISTILL_MAX_VOCAB / 2 : PS_DISTILL_MAX_VOCAB) ||
+        q->k > PS_DISTILL_MAX_K)
+        return PS_ERR_LIMIT;
     if (q->logits == nullptr || q->indices == nullptr || q->teacher == nullptr) return PS_ERR_INVALID;
     if (q->reduction == PS_REDUCE_MEAN && q->mask != nullptr && inv_n == nullptr) return PS_ERR_INVALID;
     const uint64_t es = q->dtype == PS_DTYPE_F32 ? 4 : 2, ts = q->teacher_dtype == PS_DTYPE_F32 ? 4 : 2;

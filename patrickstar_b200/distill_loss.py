@@ -137,9 +137,10 @@ def distillation_loss(logits, indices, teacher, *, temperature=1.0, tail="drop",
         raise ValueError("distillation_loss: logits [..., vocab], indices [..., k] and teacher [..., k] do not fit: "
                          "%s, %s, %s" % (tuple(logits.shape), tuple(indices.shape), tuple(teacher.shape)))
     vocab, k = logits.shape[-1], indices.shape[-1]
-    if not 1 <= vocab <= PS_DISTILL_MAX_VOCAB or not 1 <= k <= PS_DISTILL_MAX_K:
+    most = PS_DISTILL_MAX_VOCAB // (2 if tail == "bucket" else 1)
+    if not 1 <= vocab <= most or not 1 <= k <= PS_DISTILL_MAX_K:
         raise ValueError("distillation_loss: 1 to %d vocabulary entries and 1 to %d listed ones; got %d and %d"
-                         % (PS_DISTILL_MAX_VOCAB, PS_DISTILL_MAX_K, vocab, k))
+                         % (most, PS_DISTILL_MAX_K, vocab, k))
     if mask is not None:
         if mask.dtype not in (torch.bool, torch.uint8):
             raise TypeError("distillation_loss: mask must be bool or uint8, got %s" % mask.dtype)

@@ -49,6 +49,7 @@ def test_the_c_entries_refuse(ps):
             assert call(**bad) == L.PS_ERR_INVALID, bad
         assert call(vocab=L.PS_DISTILL_MAX_VOCAB + 1) == L.PS_ERR_LIMIT
         assert call(k=L.PS_DISTILL_MAX_K + 1) == L.PS_ERR_LIMIT
+        assert call(vocab=L.PS_DISTILL_MAX_VOCAB // 2 + 1, tail=1) == L.PS_ERR_LIMIT
         for bad in (dict(logits=p + 1), dict(teacher=p + 2), dict(indices=p + 4), dict(stats=p + 8)):
             assert call(**bad) == L.PS_ERR_ALIGN, bad
     assert lib.ps_distill_forward(None, p, p, p, None, None, None, 0, None, None) == L.PS_ERR_INVALID
