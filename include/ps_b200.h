@@ -649,6 +649,10 @@ int ps_distill_backward(const ps_distill_problem* problem, const void* stats_dev
                         const float* grad_out_dev, uint32_t grad_out_stride, const float* used_scale_dev,
                         void* grad_dev, uint64_t ld_grad, void* stream);
 
+/* Like ps_block_matmul_gave_up, for the two calls above: rows of such a thread
+ * block have NaN losses and gradients. */
+int ps_distill_gave_up(uint32_t* count);
+
 /* Tuning knobs for measurements: "unroll" (1, 2, 4: 128-bit groups per thread
  * per tile of the step kernels), "scan_unroll" (1, 2, 4), "blocks_per_sm"
  * (0 = occupancy calculator), "bulk" (0, or 2..4 stages of the bulk-async

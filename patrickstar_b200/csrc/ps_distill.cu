@@ -22,6 +22,7 @@
 #include "ps_b200.h"
 
 #include "ps_internal.h"
+#include "ps_tensor_core.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -30,9 +31,12 @@
 
 namespace {
 
-constexpr int kMaxThreads = 512;
+constexpr int kMaxThreads = 320;
+constexpr uint32_t kMaxSlots = 4;
 constexpr uint64_t kRowsInL2 = 64ull << 20;  // bytes of rows in work, of 126 MB
-constexpr int kUnroll = 4;  // 16-byte loads in flight a thread
+constexpr int kUnroll = 4;  // vectors of a chunk for each thread of the pass
+
+__device__ unsigned int g_gave_up;  // CTAs that ran into the limit of a wait
 
 struct DistillArgs {
     const void* z;
@@ -269,14 +273,16 @@ struct Origin {
     }
 };
 
-// Running origin and sums of one thread: of elements outside of S, and of those in it.
+// Running origin and sums of one thread: of elements outside of S, and of those in it.  The origin is an element,
+// not always the largest one: it is raised when an exponent would pass 2^4 (sums of 2^20 such terms are far from
+// the end of 32 bits), which after a thread's first elements hardly ever happens.
 struct Running {
     Origin o;
     Pair out = Pair(0.f, 0.f);
     float in = 0.f;
     __device__ __forceinline__ void raise(float top, float c)
     {
-        if (top > o.m) {
+        if (o.m == -INFINITY ? top > -INFINITY : o.exponent(top, c) > 16.f) {
             const Origin to(top, c);
             const float f = o.factor(to, c);
             out = mul2(out, Pair(f, f)), in *= f;
@@ -321,21 +327,25 @@ __device__ void entries_before(const DistillArgs& a, uint32_t row, RowSlot& slot
     const double inv_t = 1.0 / (double)a.temperature;
     bool bad = false;
     double tmax = -INFINITY, tsum = 0.0;
+#pragma unroll 4
     for (uint32_t j = lane; j < a.k; j += 32) {
         const long long v = index_at(a, (uint64_t)row * a.ld_idx + j);
-        const double t = teacher_at(a, (uint64_t)row * a.ld_teacher + j);
-        const bool listed = v >= 0 && v < (long long)a.vocab;
-        if (!listed && v != -1) bad = true;
-        l.idx[j] = listed ? (int)v : -1;
-        l.log_p[j] = t;
-        if (listed) {
-            l.z[j] = Type<T>::load(z + v);
-            if (kBucket && (kWhat & kLoss)) {
-                const uint32_t bit = bit_of<T>(shape, (uint32_t)v);
-                atomicOr(&l.bits[bit >> 5], 1u << (bit & 31));
-            }
-            tmax = (t > tmax || t != t) ? t : tmax;
+        const bool is = v >= 0 && v < (long long)a.vocab;
+        if (!is && v != -1) bad = true;
+        l.idx[j] = is ? (int)v : -1;
+        l.log_p[j] = teacher_at(a, (uint64_t)row * a.ld_teacher + j);
+    }
+#pragma unroll 4
+    for (uint32_t j = lane; j < a.k; j += 32) {
+        const int v = l.idx[j];
+        const double t = l.log_p[j];
+        if (v < 0) continue;
+        l.z[j] = Type<T>::load(z + v);
+        if (kBucket && (kWhat & kLoss)) {
+            const uint32_t bit = bit_of<T>(shape, (uint32_t)v);
+            atomicOr(&l.bits[bit >> 5], 1u << (bit & 31));
         }
+        tmax = (t > tmax || t != t) ? t : tmax;
     }
     if (!kBucket) tmax = warp_max(tmax);
     const double origin = kBucket || tmax == -INFINITY ? 0.0 : tmax;
@@ -409,26 +419,42 @@ __device__ void entries_after(const DistillArgs& a, uint32_t row, const RowSlot&
     }
 }
 
-// All warps but the last pass over rows; the last one works on the listed entries of the row before and of the
-// row after meanwhile, so that their chains of 64-bit logarithms and scattered loads hide behind the pass.
+// Where the parts of a CTA's shared memory lie: ring of chunks, barriers, listed entries, bitmaps.
+struct Layout {
+    uint32_t chunk_vecs, slots, threads;  // vectors of a chunk, chunks of the ring, threads of the pass
+};
+__host__ __device__ __forceinline__ size_t smem_bytes(const Layout& l, uint32_t k, uint32_t vocab, bool bits)
+{
+    return (size_t)l.slots * l.chunk_vecs * 16 + 48 * (size_t)k + (bits ? 8 * (size_t)bitmap_words(vocab) : 0);
+}
+
+// One warp fetches a row's vectors in chunks, ahead of their use, with bulk copies into a ring (for the
+// gradient the same ones again behind them).  One warp works on the listed entries of the row before and of
+// the row after meanwhile, so that their chains of 64-bit logarithms and scattered loads hide behind the
+// pass.  The other warps pass over the chunks.
 template <typename T, bool kBucket, int kWhat>
-__global__ void __launch_bounds__(kMaxThreads, 2) distill_kernel(const DistillArgs a)
+__global__ void __launch_bounds__(kMaxThreads, 3) distill_kernel(const DistillArgs a, const Layout lay)
 {
     constexpr int E = Type<T>::kVec;
-    extern __shared__ double smem[];
+    extern __shared__ __align__(128) unsigned char smem[];
     __shared__ RowSlot slots[2];
     __shared__ float s_m[kMaxThreads / 32], s_out[kMaxThreads / 32], s_in[kMaxThreads / 32];
+    __shared__ uint64_t full[kMaxSlots], empty[kMaxSlots];
+    __shared__ volatile int gave_up;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t threads = blockDim.x - 32, warps = threads >> 5;  // of the pass
+    const uint32_t threads = lay.threads, warps = threads >> 5;
     const float c = (float)(1.4426950408889634 / (double)a.temperature);
     Listed listed[2];
+    {
+        double* const d = reinterpret_cast<double*>(smem + (size_t)lay.slots * lay.chunk_vecs * 16);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        listed[i].p = smem + 2 * i * a.k;
-        listed[i].log_p = smem + (2 * i + 1) * a.k;
-        listed[i].idx = reinterpret_cast<int*>(smem + 4 * a.k) + 2 * i * a.k;
-        listed[i].z = reinterpret_cast<float*>(smem + 4 * a.k) + (2 * i + 1) * a.k;
-        listed[i].bits = reinterpret_cast<uint32_t*>(smem + 6 * a.k) + i * bitmap_words(a.vocab);
+        for (int i = 0; i < 2; ++i) {
+            listed[i].p = d + 2 * i * a.k;
+            listed[i].log_p = d + (2 * i + 1) * a.k;
+            listed[i].idx = reinterpret_cast<int*>(d + 4 * a.k) + 2 * i * a.k;
+            listed[i].z = reinterpret_cast<float*>(d + 4 * a.k) + (2 * i + 1) * a.k;
+            listed[i].bits = reinterpret_cast<uint32_t*>(d + 6 * a.k) + i * bitmap_words(a.vocab);
+        }
     }
 
     if ((kWhat & kLoss) == 0 && a.used_scale != nullptr && *a.used_scale == *a.grad_out)
@@ -438,183 +464,251 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_kernel(const DistillAr
         scale = a.scaler->dynamic < 0 ? 1.f : (float)a.scaler->cur_scale;
         if (blockIdx.x == 0 && threadIdx.x == 0) *a.used_scale = scale;
     }
-    if (kBucket && (kWhat & kLoss)) {
+    if (kBucket && (kWhat & kLoss))
         for (uint32_t i = threadIdx.x; i < 2 * bitmap_words(a.vocab); i += blockDim.x) listed[0].bits[i] = 0;
-        __syncthreads();
-    }
-    if (warp == warps) entries_before<T, kBucket, kWhat>(a, blockIdx.x, slots[0], listed[0]);
-
-    uint32_t it = 0;
-    for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x, ++it) {
-        __syncthreads();  // this row's entries are there, the row before is written
-        RowSlot& slot = slots[it & 1];
-        if (warp == warps) {
-            const Listed& other = listed[(it + 1) & 1];
-            if (it > 0) entries_after<T, kBucket, kWhat>(a, row - gridDim.x, slots[(it + 1) & 1], other, c, scale);
-            __syncwarp();
-            if (row + gridDim.x < a.rows)
-                entries_before<T, kBucket, kWhat>(a, row + gridDim.x, slots[(it + 1) & 1], other);
-            continue;
-        }
-        const T* const z = reinterpret_cast<const T*>(a.z) + (uint64_t)row * a.ldz;
-        T* const g = reinterpret_cast<T*>(a.grad) + (uint64_t)row * a.ldg;
-        if (!slot.keep) {
-            if ((kWhat & kLoss) && threadIdx.x == 0) a.row_loss[row] = 0.f, a.stats[row] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (kWhat & kGrad) {
-                const RowShape gs = row_shape(g, a.vocab);
-                uint4* gv = reinterpret_cast<uint4*>(g + gs.head);
-                for (uint32_t i = threadIdx.x; i < gs.vecs; i += threads) __stcs(gv + i, make_uint4(0, 0, 0, 0));
-                if (threadIdx.x < gs.head) g[threadIdx.x] = Type<T>::round(0.f);
-                if (threadIdx.x < gs.tail) g[a.vocab - gs.tail + threadIdx.x] = Type<T>::round(0.f);
-            }
-            continue;
-        }
-        const RowShape shape = row_shape(z, a.vocab);
-        const uint4* zv = reinterpret_cast<const uint4*>(z + shape.head);
-        float M, outside;
-        if (kWhat & kLoss) {
-            Running run;
-            const uint32_t* const bits = listed[it & 1].bits;
-            const uint8_t* bytes = reinterpret_cast<const uint8_t*>(bits);
-            for (uint32_t i0 = threadIdx.x; i0 < shape.vecs; i0 += kUnroll * threads) {
-                uint4 q[kUnroll];
-#pragma unroll
-                for (int u = 0; u < kUnroll; ++u) {
-                    const uint32_t i = i0 + u * threads;
-                    q[u] = make_uint4(Type<T>::kNothing, Type<T>::kNothing, Type<T>::kNothing, Type<T>::kNothing);
-                    if (i < shape.vecs) q[u] = (kWhat & kGrad) ? __ldg(zv + i) : __ldcs(zv + i);
-                }
-                uint32_t top = Type<T>::kNothing;
-#pragma unroll
-                for (int u = 0; u < kUnroll; ++u)
-                    top = Type<T>::larger(top, Type<T>::larger(Type<T>::larger(q[u].x, q[u].y), Type<T>::larger(q[u].z, q[u].w)));
-                run.raise(Type<T>::fold(top), c);
-uint32_t in[kUnroll], any = run.o.far ? 1u : 0u;
-                if (kBucket) {
-#pragma unroll
-                    for (int u = 0; u < kUnroll; ++u) {
-                        const uint32_t i = min(i0 + u * threads, shape.vecs - 1);
-                        in[u] = E == 8 ? bytes[i] : (bytes[i >> 1] >> (4 * (i & 1))) & 15u;
-                        any |= in[u];
-                    }
-                }
-                if (any == 0) {
-                    const Pair c2(c, c), r2(-run.o.r, -run.o.r);
-#pragma unroll
-                    for (int u = 0; u < kUnroll; ++u) {
-                        float f[E];
-                        Type<T>::unpack(q[u], f);
-#pragma unroll
-                        for (int j = 0; j < E; j += 2) {
-                            const float2 x = fma2(Pair(f[j], f[j + 1]), c2, r2).get();
-                            run.out = add2(run.out, Pair(ex2(x.x), ex2(x.y)));
-                        }
-                    }
-                } else {
-                    float out = 0.f;
-#pragma unroll
-                    for (int u = 0; u < kUnroll; ++u) {
-                        float f[E];
-                        Type<T>::unpack(q[u], f);
-#pragma unroll
-                        for (int j = 0; j < E; ++j) {
-                            const float e = ex2(run.o.exponent(f[j], c));
-                            if (kBucket && ((in[u] >> j) & 1))
-                                run.in += e;
-                            else
-                                out += e;
-                        }
-                    }
-                    run.out = add2(run.out, Pair(out, 0.f));
-                }
-            }
-            for (uint32_t i = threadIdx.x; i < shape.head + shape.tail; i += threads) {
-                const uint32_t v = i < shape.head ? i : i + shape.vecs * E;
-                const float f = Type<T>::load(z + v);
-                run.raise(f, c);
-                const float e = ex2(run.o.exponent(f, c));
-                bool in = false;
-                if (kBucket) {
-                    const uint32_t bit = bit_of<T>(shape, v);
-                    in = (bits[bit >> 5] >> (bit & 31)) & 1;
-                }
-                if (in)
-                    run.in += e;
-                else
-                    run.out = add2(run.out, Pair(e, 0.f));
-            }
-            // join the threads
-            float m = run.o.m;
-#pragma unroll
-            for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-            const float f = run.o.factor(Origin(m, c), c);
-            const float2 two = run.out.get();
-            const float w_out = warp_sum((two.x + two.y) * f), w_in = warp_sum(run.in * f);
-            if (lane == 0) s_m[warp] = m, s_out[warp] = w_out, s_in[warp] = w_in;
-            asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory");  // the warps of the pass
-            M = lane < warps ? s_m[lane] : -INFINITY;
-            float out = lane < warps ? s_out[lane] : 0.f, in = lane < warps ? s_in[lane] : 0.f;
-            const Origin mine(M, c);
-#pragma unroll
-            for (int d = 16; d; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-            const float fw = mine.factor(Origin(M, c), c);
-            out = warp_sum(out * fw), in = warp_sum(in * fw);
-            const float inside = (float)slot.mass / (out + in);
-            outside = inside;
-            if (kBucket && slot.rest > 0.0) outside = inside - (float)(slot.rest / (double)out);
-            if (threadIdx.x == 0) {
-                slot.M = M, slot.out = out, slot.in = in, slot.inside = inside;
-                a.stats[row] = make_float4(M, inside, outside, 0.f);
-            }
-        } else {
-            const float4 st = a.stats[row];
-            M = st.x, outside = st.z;
-            if (threadIdx.x == 0) slot.M = M, slot.inside = st.y;
-        }
-
-        if (kWhat & kGrad) {
-            if (!(kWhat & kLoss)) scale = a.grad_out[(uint64_t)row * a.grad_out_stride];
-            const float k_out = outside * (slot.bad ? NAN : grad_factor(a, scale));
-            const Origin o(M, c);
-            if ((((uintptr_t)z ^ (uintptr_t)g) & 15u) == 0 && !o.far) {
-                uint4* gv = reinterpret_cast<uint4*>(g + shape.head);
-                const Pair c2(c, c), r2(-o.r, -o.r), k2(k_out, k_out);
-                for (uint32_t i0 = threadIdx.x; i0 < shape.vecs; i0 += kUnroll * threads) {
-                    uint4 q[kUnroll];
-#pragma unroll
-                    for (int u = 0; u < kUnroll; ++u) {
-                        const uint32_t i = i0 + u * threads;
-                        if (i < shape.vecs) q[u] = __ldcs(zv + i);
-                    }
-#pragma unroll
-                    for (int u = 0; u < kUnroll; ++u) {
-                        const uint32_t i = i0 + u * threads;
-                        if (i >= shape.vecs) break;
-                        float f[E];
-                        Type<T>::unpack(q[u], f);
-#pragma unroll
-                        for (int j = 0; j < E; j += 2) {
-                            const float2 x = fma2(Pair(f[j], f[j + 1]), c2, r2).get();
-                            const float2 y = mul2(Pair(ex2(x.x), ex2(x.y)), k2).get();
-                            f[j] = y.x, f[j + 1] = y.y;
-                        }
-                        __stcs(gv + i, Type<T>::pack(f));
-                    }
-                }
-                for (uint32_t i = threadIdx.x; i < shape.head + shape.tail; i += threads) {
-                    const uint32_t v = i < shape.head ? i : i + shape.vecs * E;
-                    g[v] = Type<T>::round(ex2(o.exponent(Type<T>::load(z + v), c)) * k_out);
-                }
-            } else {
-                for (uint32_t v = threadIdx.x; v < a.vocab; v += threads)
-                    g[v] = Type<T>::round(ex2(o.exponent(Type<T>::load(z + v), c)) * k_out);
-            }
-        }
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < lay.slots; ++s) tc::bar_init(&full[s], 1), tc::bar_init(&empty[s], warps);
+        gave_up = 0;
+        tc::bar_init_fence();
     }
     __syncthreads();
-    if (warp == warps && it > 0)
+
+    constexpr int kPasses = kWhat == (kLoss | kGrad) ? 2 : 1;
+    if (warp == warps + 1) {
+        if (tc::elect_one()) {
+            const uint64_t once = tc::evict_first_policy();
+            uint32_t n = 0, at = 0, phase = 1;  // of the place's barrier `empty`: the first round waits for nothing
+            bool ok = true;
+            for (uint32_t row = blockIdx.x; row < a.rows && ok; row += gridDim.x) {
+                if (a.mask != nullptr && a.mask[row] == 0) continue;
+                const T* const z = reinterpret_cast<const T*>(a.z) + (uint64_t)row * a.ldz;
+                const RowShape shape = row_shape(z, a.vocab);
+                const uint4* const zv = reinterpret_cast<const uint4*>(z + shape.head);
+                for (int pass = 0; pass < kPasses && ok; ++pass)
+                    for (uint32_t v0 = 0; v0 < shape.vecs; v0 += lay.chunk_vecs, ++n) {
+                        if (n >= lay.slots && !tc::bar_wait(&empty[at], phase, &gave_up)) {
+                            ok = false;
+                            break;
+                        }
+                        const uint32_t bytes = min(lay.chunk_vecs, shape.vecs - v0) * 16;
+                        tc::bar_expect(&full[at], bytes);
+                        void* const dst = smem + (size_t)at * lay.chunk_vecs * 16;
+                        if (pass + 1 < kPasses)  // read again soon
+                            tc::load_bulk(dst, zv + v0, bytes, &full[at]);
+                        else
+                            tc::load_bulk(dst, zv + v0, bytes, &full[at], once);
+                        if (++at == lay.slots) at = 0, phase ^= 1;
+                    }
+            }
+            if (gave_up) {
+                // copies may still be landing in this CTA's memory
+                int ignore = 0;
+                for (uint32_t i = n < lay.slots ? 0 : n - lay.slots; i < n; ++i)
+                    tc::bar_wait(&full[i % lay.slots], (i / lay.slots) & 1, &ignore);
+            }
+        }
+    } else if (warp == warps) {
+        entries_before<T, kBucket, kWhat>(a, blockIdx.x, slots[0], listed[0]);
+        uint32_t it = 0;
+        for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x, ++it) {
+            asm volatile("bar.sync 2, %0;" ::"r"(threads + 32) : "memory");  // see below
+            const uint32_t other = (it + 1) & 1;
+            if (it > 0) entries_after<T, kBucket, kWhat>(a, row - gridDim.x, slots[other], listed[other], c, scale);
+            __syncwarp();
+            if (row + gridDim.x < a.rows)
+                entries_before<T, kBucket, kWhat>(a, row + gridDim.x, slots[other], listed[other]);
+        }
+        asm volatile("bar.sync 2, %0;" ::"r"(threads + 32) : "memory");
         entries_after<T, kBucket, kWhat>(a, blockIdx.x + (it - 1) * gridDim.x, slots[(it - 1) & 1], listed[(it - 1) & 1], c,
                                          scale);
+    } else {
+        uint32_t it = 0, at = 0, phase = 0;
+        bool lost = false;  // a chunk did not come
+        for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x, ++it) {
+            // this row's entries are there, the row before is written
+            asm volatile("bar.sync 2, %0;" ::"r"(threads + 32) : "memory");
+            RowSlot& slot = slots[it & 1];
+            const T* const z = reinterpret_cast<const T*>(a.z) + (uint64_t)row * a.ldz;
+            T* const g = reinterpret_cast<T*>(a.grad) + (uint64_t)row * a.ldg;
+            if (!slot.keep) {
+                if ((kWhat & kLoss) && threadIdx.x == 0)
+                    a.row_loss[row] = 0.f, a.stats[row] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (kWhat & kGrad) {
+                    const RowShape gs = row_shape(g, a.vocab);
+                    uint4* gv = reinterpret_cast<uint4*>(g + gs.head);
+                    for (uint32_t i = threadIdx.x; i < gs.vecs; i += threads) __stcs(gv + i, make_uint4(0, 0, 0, 0));
+                    if (threadIdx.x < gs.head) g[threadIdx.x] = Type<T>::round(0.f);
+                    if (threadIdx.x < gs.tail) g[a.vocab - gs.tail + threadIdx.x] = Type<T>::round(0.f);
+                }
+                continue;
+            }
+            const RowShape shape = row_shape(z, a.vocab);
+            const uint32_t edge = shape.head + shape.tail;  // elements outside of the vectors: one for each thread
+            const uint32_t v_edge = threadIdx.x < shape.head ? threadIdx.x : threadIdx.x + shape.vecs * E;
+            float f_edge = -INFINITY;
+            if (threadIdx.x < edge) f_edge = Type<T>::load(z + v_edge);
+
+            // the next chunk's vectors of this thread into q; how many vectors the chunk has
+            auto take = [&](uint32_t v0, uint4(&q)[kUnroll]) -> uint32_t {
+                if (!tc::bar_wait(&full[at], phase, &gave_up)) lost = true;
+                const uint4* const from = reinterpret_cast<const uint4*>(smem) + at * lay.chunk_vecs + threadIdx.x;
+                const uint32_t count = min(lay.chunk_vecs, shape.vecs - v0);
+                if (count == lay.chunk_vecs) {
+#pragma unroll
+                    for (int u = 0; u < kUnroll; ++u) q[u] = from[u * threads];
+                } else {
+#pragma unroll
+                    for (int u = 0; u < kUnroll; ++u) {
+                        q[u] = make_uint4(Type<T>::kNothing, Type<T>::kNothing, Type<T>::kNothing, Type<T>::kNothing);
+                        if (threadIdx.x + u * threads < count) q[u] = from[u * threads];
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) tc::bar_arrive(&empty[at]);  // read: the chunk's place may be filled again
+                if (++at == lay.slots) at = 0, phase ^= 1;
+                return count;
+            };
+
+            float M, outside;
+            if (kWhat & kLoss) {
+                Running run;
+                const uint32_t* const bits = listed[it & 1].bits;
+                const uint8_t* const bytes = reinterpret_cast<const uint8_t*>(bits);
+                for (uint32_t v0 = 0; v0 < shape.vecs; v0 += lay.chunk_vecs) {
+                    uint4 q[kUnroll];
+                    const uint32_t count = take(v0, q);
+                    uint32_t top = Type<T>::kNothing;
+#pragma unroll
+                    for (int u = 0; u < kUnroll; ++u)
+                        top = Type<T>::larger(
+                            top, Type<T>::larger(Type<T>::larger(q[u].x, q[u].y), Type<T>::larger(q[u].z, q[u].w)));
+                    run.raise(Type<T>::fold(top), c);
+                    uint32_t in[kUnroll], any = run.o.far ? 1u : 0u;
+                    if (kBucket) {
+#pragma unroll
+                        for (int u = 0; u < kUnroll; ++u) {
+                            const uint32_t i = v0 + min(threadIdx.x + u * threads, count - 1);
+                            in[u] = E == 8 ? bytes[i] : (bytes[i >> 1] >> (4 * (i & 1))) & 15u;
+                            any |= in[u];
+                        }
+                    }
+                    if (any == 0) {
+                        const Pair c2(c, c), r2(-run.o.r, -run.o.r);
+#pragma unroll
+                        for (int u = 0; u < kUnroll; ++u) {
+                            if (u * threads >= count) break;
+                            float f[E];
+                            Type<T>::unpack(q[u], f);
+#pragma unroll
+                            for (int j = 0; j < E; j += 2) {
+                                const float2 x = fma2(Pair(f[j], f[j + 1]), c2, r2).get();
+                                run.out = add2(run.out, Pair(ex2(x.x), ex2(x.y)));
+                            }
+                        }
+                    } else {
+                        float out = 0.f;
+#pragma unroll
+                        for (int u = 0; u < kUnroll; ++u) {
+                            float f[E];
+                            Type<T>::unpack(q[u], f);
+#pragma unroll
+                            for (int j = 0; j < E; ++j) {
+                                const float e = ex2(run.o.exponent(f[j], c));
+                                if (kBucket && ((in[u] >> j) & 1))
+                                    run.in += e;
+                                else
+                                    out += e;
+                            }
+                        }
+                        run.out = add2(run.out, Pair(out, 0.f));
+                    }
+                }
+                if (threadIdx.x < edge) {
+                    run.raise(f_edge, c);
+                    const float e = ex2(run.o.exponent(f_edge, c));
+                    bool in = false;
+                    if (kBucket) {
+                        const uint32_t bit = bit_of<T>(shape, v_edge);
+                        in = (bits[bit >> 5] >> (bit & 31)) & 1;
+                    }
+                    if (in)
+                        run.in += e;
+                    else
+                        run.out = add2(run.out, Pair(e, 0.f));
+                }
+                // join the threads
+                float m = run.o.m;
+#pragma unroll
+                for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+                const float f = lost ? NAN : run.o.factor(Origin(m, c), c);
+                const float2 two = run.out.get();
+                const float w_out = warp_sum((two.x + two.y) * f), w_in = warp_sum(run.in * f);
+                if (lane == 0) s_m[warp] = m, s_out[warp] = w_out, s_in[warp] = w_in;
+                asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory");  // the warps of the pass
+                M = lane < warps ? s_m[lane] : -INFINITY;
+                float out = lane < warps ? s_out[lane] : 0.f, in = lane < warps ? s_in[lane] : 0.f;
+                const Origin mine(M, c);
+#pragma unroll
+                for (int d = 16; d; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+                const float fw = mine.factor(Origin(M, c), c);
+                out = warp_sum(out * fw), in = warp_sum(in * fw);
+                const float inside = (float)slot.mass / (out + in);
+                outside = inside;
+                if (kBucket && slot.rest > 0.0) outside = inside - (float)(slot.rest / (double)out);
+                if (threadIdx.x == 0) {
+                    slot.M = M, slot.out = out, slot.in = in, slot.inside = inside;
+                    a.stats[row] = make_float4(M, inside, outside, 0.f);
+                }
+            } else {
+                const float4 st = a.stats[row];
+                M = st.x, outside = st.z;
+                if (threadIdx.x == 0) slot.M = M, slot.inside = st.y;
+            }
+
+            if (kWhat & kGrad) {
+                if (!(kWhat & kLoss)) scale = a.grad_out[(uint64_t)row * a.grad_out_stride];
+                const float k_out = outside * (slot.bad ? NAN : grad_factor(a, scale));
+                const Origin o(M, c);
+                const bool same_offset = (((uintptr_t)z ^ (uintptr_t)g) & 15u) == 0;
+                const Pair c2(c, c), r2(-o.r, -o.r), k2(k_out, k_out);
+                for (uint32_t v0 = 0; v0 < shape.vecs; v0 += lay.chunk_vecs) {
+                    uint4 q[kUnroll];
+                    const uint32_t count = take(v0, q);
+                    T* const to = g + shape.head + (uint64_t)v0 * E;
+#pragma unroll
+                    for (int u = 0; u < kUnroll; ++u) {
+                        const uint32_t i = threadIdx.x + u * threads;
+                        if (i >= count) break;
+                        float f[E];
+                        Type<T>::unpack(q[u], f);
+                        if (!o.far) {
+#pragma unroll
+                            for (int j = 0; j < E; j += 2) {
+                                const float2 x = fma2(Pair(f[j], f[j + 1]), c2, r2).get();
+                                const float2 y = mul2(Pair(ex2(x.x), ex2(x.y)), k2).get();
+                                f[j] = y.x, f[j + 1] = y.y;
+                            }
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < E; ++j) f[j] = ex2(o.exponent(f[j], c)) * k_out;
+                        }
+                        if (same_offset) {
+                            __stcs(reinterpret_cast<uint4*>(to) + i, Type<T>::pack(f));
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < E; ++j) to[(uint64_t)i * E + j] = Type<T>::round(f[j]);
+                        }
+                    }
+                    if (lost) to[0] = Type<T>::round(NAN);
+                }
+                if (threadIdx.x < edge) g[v_edge] = Type<T>::round(ex2(o.exponent(f_edge, c)) * k_out);
+            }
+        }
+        asm volatile("bar.sync 2, %0;" ::"r"(threads + 32) : "memory");
+    }
+    __syncwarp();
+    __syncthreads();
+    if (threadIdx.x == 0 && gave_up) atomicAdd(&g_gave_up, 1u);
 }
 
 // 1 / max(1, rows kept)
@@ -652,7 +746,16 @@ int launch(const DistillArgs& a, cudaStream_t st)
 {
     const int sms = ps_internal::sm_count();
     if (sms < 0) return sms;
-    const size_t smem = 48 * (size_t)a.k + (kBucket && (kWhat & kLoss) ? 8 * (size_t)bitmap_words(a.vocab) : 0);
+    // Threads and chunks for a row by its size: four vectors a thread and chunk, four chunks, and from three CTAs
+    // of 64 KB on an SM (rows above 48 KB) to eight small ones, whose rows' own latencies overlap.
+    const uint64_t bytes = (uint64_t)a.vocab * sizeof(T);
+    Layout lay;
+    lay.threads = bytes <= 16 * 1024 ? 64 : bytes <= 48 * 1024 ? 128 : 256;
+    lay.chunk_vecs = kUnroll * lay.threads;
+    lay.slots = kMaxSlots;
+    const bool bits = kBucket && (kWhat & kLoss);
+    while (lay.slots > 2 && smem_bytes(lay, a.k, a.vocab, bits) > 200 * 1024) --lay.slots;
+    const size_t smem = smem_bytes(lay, a.k, a.vocab, bits);
     if (smem > 40 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(distill_kernel<T, kBucket, kWhat>,
                                                    cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -662,17 +765,16 @@ int launch(const DistillArgs& a, cudaStream_t st)
             return PS_ERR_CUDA;
         }
     }
-    // Enough threads for a row to have two rounds of loads at least, and as many rows in work as SMs hold, but
-    // for the gradient no more than L2 keeps until the second pass.
-    const uint64_t bytes = (uint64_t)a.vocab * sizeof(T);
-    const uint32_t threads = bytes <= 16 * 1024 ? 96 : bytes <= 48 * 1024 ? 224 : 480;
-    uint64_t most = 2048 / (threads + 32);
+    // As many rows in work as SMs hold, but for the gradient no more than L2 keeps until the second pass.
+    uint64_t most = 227 * 1024 / (smem + 2048);
+    const uint64_t by_threads = 1024 / (lay.threads + 64);  // 64 registers each
+    most = most < 1 ? 1 : most < by_threads ? most : by_threads;
     if ((kWhat & kLoss) && (kWhat & kGrad)) {
         const uint64_t fit = kRowsInL2 / ((uint64_t)sms * bytes);
-        most = fit < 2 ? 2 : fit < most ? fit : most;
+        most = fit >= most ? most : fit < 2 ? (most < 2 ? most : 2) : fit;
     }
     most *= (uint64_t)sms;
-    distill_kernel<T, kBucket, kWhat><<<a.rows < most ? a.rows : (uint32_t)most, threads + 32, smem, st>>>(a);
+    distill_kernel<T, kBucket, kWhat><<<a.rows < most ? a.rows : (uint32_t)most, lay.threads + 64, smem, st>>>(a, lay);
     return ps_internal::after_launch();
 }
 template <typename T>
@@ -779,6 +881,18 @@ int ps_distill_backward(const ps_distill_problem* q, const void* stats_dev, cons
     a.grad_out_stride = grad_out_stride, a.used_scale = const_cast<float*>(used_scale_dev);
     a.grad = grad_dev, a.ldg = ld_grad;
     return launch(a, q->dtype, q->tail == PS_TAIL_BUCKET, kGrad, (cudaStream_t)stream);
+}
+
+int ps_distill_gave_up(uint32_t* count)
+{
+    if (count == nullptr) return PS_ERR_INVALID;
+    const cudaError_t e = cudaMemcpyFromSymbol(count, g_gave_up, sizeof(*count));
+    if (e != cudaSuccess) {
+        ps_internal::set_cuda_error((int)e);
+        cudaGetLastError();
+        return PS_ERR_CUDA;
+    }
+    return PS_OK;
 }
 
 }  // extern "C"

@@ -397,3 +397,11 @@ def test_saved_tensors_that_come_back_elsewhere():
     with torch.autograd.graph.save_on_cpu():
         got = run()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_no_wait_ran_out():
+    import ctypes as C
+    from patrickstar_b200 import _lib as L
+    n = C.c_uint32(7)
+    L.check(L.lib.ps_distill_gave_up(C.byref(n)), "ps_distill_gave_up")
+    assert n.value == 0
