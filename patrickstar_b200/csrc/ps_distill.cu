@@ -28,11 +28,13 @@
 #include <cuda_fp16.h>
 
 #include <cstring>
+#include <type_traits>
 
 namespace {
 
 constexpr int kMaxThreads = 320;
 constexpr uint32_t kMaxSlots = 4;
+constexpr int kCtas = 3;  // of the largest kind on an SM: 64 registers a thread
 constexpr uint64_t kRowsInL2 = 64ull << 20;  // bytes of rows in work, of 126 MB
 constexpr int kUnroll = 4;  // vectors of a chunk for each thread of the pass
 
@@ -297,16 +299,42 @@ constexpr int kLoss = 1, kGrad = 2;
 struct RowSlot {
     double rest, mass;  // p_r, and sum p + p_r: 1 unless the teacher gives nothing, or too much
     float M, out, in;   // largest logit, sums outside of S and in it
-    float inside, outside;  // factors of e_v in the gradient
-    int keep, bad;      // the mask keeps the row; an index is outside of the vocabulary
+    float inside;           // factor of e_v in the gradient, v in S
+    float grad;             // factor of the gradient: NaN for a bad row
+    int keep, bad, twice;   // the mask keeps the row; an index is outside of the vocabulary; one is listed twice
 };
 struct Listed {
     double *p, *log_p;  // probabilities and their logarithms
     int* idx;           // or -1
     float* z;           // logits
-    uint32_t* bits;
+    uint32_t* bits;     // of every element: is it listed?
+    uint32_t* owners;   // of every thread and chunk: has it a listed element?
+};
+// Threads and shared memory of a CTA: chunks of kUnroll vectors a thread, a ring of them, barriers, listed entries,
+// bitmaps.
+struct Layout {
+    uint32_t chunk_vecs, slots, threads;  // vectors of a chunk, chunks of the ring, threads of the pass
 };
 __host__ __device__ __forceinline__ uint32_t bitmap_words(uint32_t vocab) { return (vocab + 63) / 64 * 2; }
+__host__ __device__ __forceinline__ uint32_t round4(uint32_t k) { return (k + 3) & ~3u; }
+// a vector has four elements at least
+__host__ __device__ __forceinline__ uint32_t owner_words(const Layout& l, uint32_t vocab)
+{
+    return ((vocab / 4 + l.chunk_vecs - 1) / l.chunk_vecs * (l.threads / 32) + 1) / 2 * 2;
+}
+__host__ __device__ __forceinline__ size_t smem_bytes(const Layout& l, uint32_t k, uint32_t vocab, bool bits)
+{
+    return (size_t)l.slots * l.chunk_vecs * 16 + 48 * (size_t)round4(k) +
+           (bits ? 8 * (size_t)(bitmap_words(vocab) + owner_words(l, vocab)) : 0);
+}
+// Word of `owners` for element v of the vectors (bit: thread % 32)
+template <typename T>
+__device__ __forceinline__ uint32_t owner_of(const Layout& lay, const RowShape& s, uint32_t v, uint32_t* bit)
+{
+    const uint32_t i = (v - s.head) / Type<T>::kVec, chunk = i / lay.chunk_vecs, t = i % lay.threads;
+    *bit = t & 31;
+    return chunk * (lay.threads >> 5) + (t >> 5);
+}
 
 __device__ __forceinline__ float grad_factor(const DistillArgs& a, float scale)
 {
@@ -316,7 +344,8 @@ __device__ __forceinline__ float grad_factor(const DistillArgs& a, float scale)
 
 // The listed entries of a row, by one warp, before the pass over it.
 template <typename T, bool kBucket, int kWhat>
-__device__ void entries_before(const DistillArgs& a, uint32_t row, RowSlot& slot, const Listed& l)
+__device__ void entries_before(const DistillArgs& a, const Layout& lay, uint32_t row, RowSlot& slot, const Listed& l,
+                               float scale)
 {
     const uint32_t lane = threadIdx.x & 31;
     const bool keep = a.mask == nullptr || a.mask[row] != 0;
@@ -326,7 +355,9 @@ __device__ void entries_before(const DistillArgs& a, uint32_t row, RowSlot& slot
     const RowShape shape = row_shape(z, a.vocab);
     const double inv_t = 1.0 / (double)a.temperature;
     bool bad = false;
+    bool twice = false;
     double tmax = -INFINITY, tsum = 0.0;
+    if (lane < 3 && a.k + lane < round4(a.k)) l.idx[a.k + lane] = -1;
 #pragma unroll 4
     for (uint32_t j = lane; j < a.k; j += 32) {
         const long long v = index_at(a, (uint64_t)row * a.ld_idx + j);
@@ -344,8 +375,26 @@ __device__ void entries_before(const DistillArgs& a, uint32_t row, RowSlot& slot
         if (kBucket && (kWhat & kLoss)) {
             const uint32_t bit = bit_of<T>(shape, (uint32_t)v);
             atomicOr(&l.bits[bit >> 5], 1u << (bit & 31));
+            if ((uint32_t)v - shape.head < shape.vecs * Type<T>::kVec) {
+                uint32_t of;
+                const uint32_t w = owner_of<T>(lay, shape, (uint32_t)v, &of);
+                atomicOr(&l.owners[w], 1u << of);
+            }
         }
         tmax = (t > tmax || t != t) ? t : tmax;
+    }
+    if (kWhat & kGrad) {  // of the four indices of a group the own one counts as well
+        __syncwarp();
+        for (uint32_t j = lane; j < a.k; j += 32) {
+            const int v = l.idx[j];
+            int n = 0;
+            for (uint32_t i = 0; i < a.k; i += 4) {
+                const int4 w = *reinterpret_cast<const int4*>(l.idx + i);
+                n += (w.x == v) + (w.y == v) + (w.z == v) + (w.w == v);
+            }
+            if (v >= 0 && n > 1) twice = true;
+        }
+        twice = __any_sync(0xffffffffu, twice);
     }
     if (!kBucket) tmax = warp_max(tmax);
     const double origin = kBucket || tmax == -INFINITY ? 0.0 : tmax;
@@ -373,12 +422,17 @@ __device__ void entries_before(const DistillArgs& a, uint32_t row, RowSlot& slot
         mass = tsum + rest;
     }
     bad = __any_sync(0xffffffffu, bad);
-    if (lane == 0) slot.rest = rest, slot.mass = mass, slot.bad = bad;
+    if (kWhat == kGrad) scale = a.grad_out[(uint64_t)row * a.grad_out_stride];
+    if (lane == 0) {
+        slot.rest = rest, slot.mass = mass, slot.bad = bad, slot.twice = twice;
+        if (kWhat & kGrad) slot.grad = bad ? NAN : grad_factor(a, scale);
+    }
 }
 
 // ... and after it: the row's loss, and the gradient of the listed elements over what the pass wrote there.
 template <typename T, bool kBucket, int kWhat>
-__device__ void entries_after(const DistillArgs& a, uint32_t row, const RowSlot& slot, const Listed& l, float c, float scale)
+__device__ void entries_after(const DistillArgs& a, const Layout& lay, uint32_t row, const RowSlot& slot, const Listed& l,
+                              float c)
 {
     const uint32_t lane = threadIdx.x & 31;
     if (!slot.keep) return;
@@ -398,15 +452,16 @@ __device__ void entries_after(const DistillArgs& a, uint32_t row, const RowSlot&
     }
     if (kWhat & kGrad) {
         T* const g = reinterpret_cast<T*>(a.grad) + (uint64_t)row * a.ldg;
-        if (!(kWhat & kLoss)) scale = a.grad_out[(uint64_t)row * a.grad_out_stride];
-        const float gf = slot.bad ? NAN : grad_factor(a, scale);
         for (uint32_t j = lane; j < a.k; j += 32) {
             const int v = l.idx[j];
             if (v < 0) continue;
-            float p = 0.f;
-            for (uint32_t i = 0; i < a.k; ++i)
-                if (l.idx[i] == v) p += (float)l.p[i];
-            g[v] = Type<T>::round((ex2(o.exponent(l.z[j], c)) * slot.inside - p) * gf);
+            float p = (float)l.p[j];
+            if (slot.twice) {
+                p = 0.f;
+                for (uint32_t i = 0; i < a.k; ++i)
+                    if (l.idx[i] == v) p += (float)l.p[i];
+            }
+            g[v] = Type<T>::round((ex2(o.exponent(l.z[j], c)) * slot.inside - p) * slot.grad);
         }
     }
     if (kBucket && (kWhat & kLoss)) {  // the bitmap is zeros again
@@ -414,18 +469,14 @@ __device__ void entries_after(const DistillArgs& a, uint32_t row, const RowSlot&
         const T* const z = reinterpret_cast<const T*>(a.z) + (uint64_t)row * a.ldz;
         const RowShape shape = row_shape(z, a.vocab);
         for (uint32_t j = lane; j < a.k; j += 32)
-            if (l.idx[j] >= 0) l.bits[bit_of<T>(shape, (uint32_t)l.idx[j]) >> 5] = 0;
+            if (l.idx[j] >= 0) {
+                const uint32_t v = (uint32_t)l.idx[j];
+                uint32_t of;
+                l.bits[bit_of<T>(shape, v) >> 5] = 0;
+                if (v - shape.head < shape.vecs * Type<T>::kVec) l.owners[owner_of<T>(lay, shape, v, &of)] = 0;
+            }
         __syncwarp();
     }
-}
-
-// Where the parts of a CTA's shared memory lie: ring of chunks, barriers, listed entries, bitmaps.
-struct Layout {
-    uint32_t chunk_vecs, slots, threads;  // vectors of a chunk, chunks of the ring, threads of the pass
-};
-__host__ __device__ __forceinline__ size_t smem_bytes(const Layout& l, uint32_t k, uint32_t vocab, bool bits)
-{
-    return (size_t)l.slots * l.chunk_vecs * 16 + 48 * (size_t)k + (bits ? 8 * (size_t)bitmap_words(vocab) : 0);
 }
 
 // One warp fetches a row's vectors in chunks, ahead of their use, with bulk copies into a ring (for the
@@ -433,7 +484,7 @@ __host__ __device__ __forceinline__ size_t smem_bytes(const Layout& l, uint32_t 
 // the row after meanwhile, so that their chains of 64-bit logarithms and scattered loads hide behind the
 // pass.  The other warps pass over the chunks.
 template <typename T, bool kBucket, int kWhat>
-__global__ void __launch_bounds__(kMaxThreads, 3) distill_kernel(const DistillArgs a, const Layout lay)
+__global__ void __launch_bounds__(kMaxThreads, kCtas) distill_kernel(const DistillArgs a, const Layout lay)
 {
     constexpr int E = Type<T>::kVec;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -446,14 +497,16 @@ __global__ void __launch_bounds__(kMaxThreads, 3) distill_kernel(const DistillAr
     const float c = (float)(1.4426950408889634 / (double)a.temperature);
     Listed listed[2];
     {
+        const uint32_t k4 = round4(a.k);  // four indices can be read at once
         double* const d = reinterpret_cast<double*>(smem + (size_t)lay.slots * lay.chunk_vecs * 16);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            listed[i].p = d + 2 * i * a.k;
-            listed[i].log_p = d + (2 * i + 1) * a.k;
-            listed[i].idx = reinterpret_cast<int*>(d + 4 * a.k) + 2 * i * a.k;
-            listed[i].z = reinterpret_cast<float*>(d + 4 * a.k) + (2 * i + 1) * a.k;
-            listed[i].bits = reinterpret_cast<uint32_t*>(d + 6 * a.k) + i * bitmap_words(a.vocab);
+            listed[i].p = d + 2 * i * k4;
+            listed[i].log_p = d + (2 * i + 1) * k4;
+            listed[i].idx = reinterpret_cast<int*>(d + 4 * k4) + 2 * i * k4;
+            listed[i].z = reinterpret_cast<float*>(d + 4 * k4) + (2 * i + 1) * k4;
+            listed[i].bits = reinterpret_cast<uint32_t*>(d + 6 * k4) + i * bitmap_words(a.vocab);
+            listed[i].owners = reinterpret_cast<uint32_t*>(d + 6 * k4) + 2 * bitmap_words(a.vocab) + i * owner_words(lay, a.vocab);
         }
     }
 
@@ -465,7 +518,8 @@ __global__ void __launch_bounds__(kMaxThreads, 3) distill_kernel(const DistillAr
         if (blockIdx.x == 0 && threadIdx.x == 0) *a.used_scale = scale;
     }
     if (kBucket && (kWhat & kLoss))
-        for (uint32_t i = threadIdx.x; i < 2 * bitmap_words(a.vocab); i += blockDim.x) listed[0].bits[i] = 0;
+        for (uint32_t i = threadIdx.x; i < 2 * (bitmap_words(a.vocab) + owner_words(lay, a.vocab)); i += blockDim.x)
+            listed[0].bits[i] = 0;
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < lay.slots; ++s) tc::bar_init(&full[s], 1), tc::bar_init(&empty[s], warps);
         gave_up = 0;
@@ -508,19 +562,18 @@ __global__ void __launch_bounds__(kMaxThreads, 3) distill_kernel(const DistillAr
             }
         }
     } else if (warp == warps) {
-        entries_before<T, kBucket, kWhat>(a, blockIdx.x, slots[0], listed[0]);
+        entries_before<T, kBucket, kWhat>(a, lay, blockIdx.x, slots[0], listed[0], scale);
         uint32_t it = 0;
         for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x, ++it) {
             asm volatile("bar.sync 2, %0;" ::"r"(threads + 32) : "memory");  // see below
             const uint32_t other = (it + 1) & 1;
-            if (it > 0) entries_after<T, kBucket, kWhat>(a, row - gridDim.x, slots[other], listed[other], c, scale);
+            if (it > 0) entries_after<T, kBucket, kWhat>(a, lay, row - gridDim.x, slots[other], listed[other], c);
             __syncwarp();
             if (row + gridDim.x < a.rows)
-                entries_before<T, kBucket, kWhat>(a, row + gridDim.x, slots[other], listed[other]);
+                entries_before<T, kBucket, kWhat>(a, lay, row + gridDim.x, slots[other], listed[other], scale);
         }
         asm volatile("bar.sync 2, %0;" ::"r"(threads + 32) : "memory");
-        entries_after<T, kBucket, kWhat>(a, blockIdx.x + (it - 1) * gridDim.x, slots[(it - 1) & 1], listed[(it - 1) & 1], c,
-                                         scale);
+        entries_after<T, kBucket, kWhat>(a, lay, blockIdx.x + (it - 1) * gridDim.x, slots[(it - 1) & 1], listed[(it - 1) & 1], c);
     } else {
         uint32_t it = 0, at = 0, phase = 0;
         bool lost = false;  // a chunk did not come
@@ -548,55 +601,47 @@ __global__ void __launch_bounds__(kMaxThreads, 3) distill_kernel(const DistillAr
             float f_edge = -INFINITY;
             if (threadIdx.x < edge) f_edge = Type<T>::load(z + v_edge);
 
-            // the next chunk's vectors of this thread into q; how many vectors the chunk has
-            auto take = [&](uint32_t v0, uint4(&q)[kUnroll]) -> uint32_t {
+            // the next chunk's vectors of this thread into q; `count` is the vectors the chunk has
+            auto take = [&](uint4(&q)[kUnroll], uint32_t count, auto whole) {
                 if (!tc::bar_wait(&full[at], phase, &gave_up)) lost = true;
                 const uint4* const from = reinterpret_cast<const uint4*>(smem) + at * lay.chunk_vecs + threadIdx.x;
-                const uint32_t count = min(lay.chunk_vecs, shape.vecs - v0);
-                if (count == lay.chunk_vecs) {
 #pragma unroll
-                    for (int u = 0; u < kUnroll; ++u) q[u] = from[u * threads];
-                } else {
-#pragma unroll
-                    for (int u = 0; u < kUnroll; ++u) {
+                for (int u = 0; u < kUnroll; ++u) {
+                    if constexpr (!decltype(whole)::value) {
                         q[u] = make_uint4(Type<T>::kNothing, Type<T>::kNothing, Type<T>::kNothing, Type<T>::kNothing);
-                        if (threadIdx.x + u * threads < count) q[u] = from[u * threads];
+                        if (threadIdx.x + u * threads >= count) continue;
                     }
+                    q[u] = from[u * threads];
                 }
                 __syncwarp();
                 if (lane == 0) tc::bar_arrive(&empty[at]);  // read: the chunk's place may be filled again
                 if (++at == lay.slots) at = 0, phase ^= 1;
-                return count;
             };
+            const uint32_t whole_vecs = shape.vecs / lay.chunk_vecs * lay.chunk_vecs;
 
             float M, outside;
             if (kWhat & kLoss) {
                 Running run;
                 const uint32_t* const bits = listed[it & 1].bits;
                 const uint8_t* const bytes = reinterpret_cast<const uint8_t*>(bits);
-                for (uint32_t v0 = 0; v0 < shape.vecs; v0 += lay.chunk_vecs) {
+                const uint32_t* owners = listed[it & 1].owners + warp;
+                auto add = [&](uint32_t v0, auto whole) {
+                    const uint32_t count = shape.vecs - v0;
                     uint4 q[kUnroll];
-                    const uint32_t count = take(v0, q);
+                    take(q, count, whole);
                     uint32_t top = Type<T>::kNothing;
 #pragma unroll
                     for (int u = 0; u < kUnroll; ++u)
                         top = Type<T>::larger(
                             top, Type<T>::larger(Type<T>::larger(q[u].x, q[u].y), Type<T>::larger(q[u].z, q[u].w)));
                     run.raise(Type<T>::fold(top), c);
-                    uint32_t in[kUnroll], any = run.o.far ? 1u : 0u;
-                    if (kBucket) {
-#pragma unroll
-                        for (int u = 0; u < kUnroll; ++u) {
-                            const uint32_t i = v0 + min(threadIdx.x + u * threads, count - 1);
-                            in[u] = E == 8 ? bytes[i] : (bytes[i >> 1] >> (4 * (i & 1))) & 15u;
-                            any |= in[u];
-                        }
-                    }
-                    if (any == 0) {
+                    bool any = run.o.far;
+                    if (kBucket) any = any || ((*owners >> lane) & 1), owners += warps;
+                    if (!any) {
                         const Pair c2(c, c), r2(-run.o.r, -run.o.r);
 #pragma unroll
                         for (int u = 0; u < kUnroll; ++u) {
-                            if (u * threads >= count) break;
+                            if (!decltype(whole)::value && u * threads >= count) break;
                             float f[E];
                             Type<T>::unpack(q[u], f);
 #pragma unroll
@@ -611,10 +656,15 @@ __global__ void __launch_bounds__(kMaxThreads, 3) distill_kernel(const DistillAr
                         for (int u = 0; u < kUnroll; ++u) {
                             float f[E];
                             Type<T>::unpack(q[u], f);
+                            uint32_t in = 0;
+                            if (kBucket) {
+                                const uint32_t i = min(v0 + threadIdx.x + u * threads, shape.vecs - 1);
+                                in = E == 8 ? bytes[i] : (bytes[i >> 1] >> (4 * (i & 1))) & 15u;
+                            }
 #pragma unroll
                             for (int j = 0; j < E; ++j) {
                                 const float e = ex2(run.o.exponent(f[j], c));
-                                if (kBucket && ((in[u] >> j) & 1))
+                                if (kBucket && ((in >> j) & 1))
                                     run.in += e;
                                 else
                                     out += e;
@@ -622,7 +672,9 @@ __global__ void __launch_bounds__(kMaxThreads, 3) distill_kernel(const DistillAr
                         }
                         run.out = add2(run.out, Pair(out, 0.f));
                     }
-                }
+                };
+                for (uint32_t v0 = 0; v0 < whole_vecs; v0 += lay.chunk_vecs) add(v0, std::true_type());
+                if (whole_vecs < shape.vecs) add(whole_vecs, std::false_type());
                 if (threadIdx.x < edge) {
                     run.raise(f_edge, c);
                     const float e = ex2(run.o.exponent(f_edge, c));
@@ -642,7 +694,7 @@ __global__ void __launch_bounds__(kMaxThreads, 3) distill_kernel(const DistillAr
                 for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
                 const float f = lost ? NAN : run.o.factor(Origin(m, c), c);
                 const float2 two = run.out.get();
-                const float w_out = warp_sum((two.x + two.y) * f), w_in = warp_sum(run.in * f);
+                const float w_out = warp_sum((two.x + two.y) * f), w_in = kBucket ? warp_sum(run.in * f) : 0.f;
                 if (lane == 0) s_m[warp] = m, s_out[warp] = w_out, s_in[warp] = w_in;
                 asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory");  // the warps of the pass
                 M = lane < warps ? s_m[lane] : -INFINITY;
@@ -651,7 +703,8 @@ __global__ void __launch_bounds__(kMaxThreads, 3) distill_kernel(const DistillAr
 #pragma unroll
                 for (int d = 16; d; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
                 const float fw = mine.factor(Origin(M, c), c);
-                out = warp_sum(out * fw), in = warp_sum(in * fw);
+                out = warp_sum(out * fw);
+                if (kBucket) in = warp_sum(in * fw);
                 const float inside = (float)slot.mass / (out + in);
                 outside = inside;
                 if (kBucket && slot.rest > 0.0) outside = inside - (float)(slot.rest / (double)out);
@@ -666,41 +719,42 @@ __global__ void __launch_bounds__(kMaxThreads, 3) distill_kernel(const DistillAr
             }
 
             if (kWhat & kGrad) {
-                if (!(kWhat & kLoss)) scale = a.grad_out[(uint64_t)row * a.grad_out_stride];
-                const float k_out = outside * (slot.bad ? NAN : grad_factor(a, scale));
+                const float k_out = outside * slot.grad;
                 const Origin o(M, c);
                 const bool same_offset = (((uintptr_t)z ^ (uintptr_t)g) & 15u) == 0;
-                const Pair c2(c, c), r2(-o.r, -o.r), k2(k_out, k_out);
-                for (uint32_t v0 = 0; v0 < shape.vecs; v0 += lay.chunk_vecs) {
+                auto write = [&](uint32_t v0, auto whole, auto plain) {
+                    const Pair c2(c, c), r2(-o.r, -o.r), k2(k_out, k_out);
+                    const uint32_t count = shape.vecs - v0;
                     uint4 q[kUnroll];
-                    const uint32_t count = take(v0, q);
-                    T* const to = g + shape.head + (uint64_t)v0 * E;
+                    take(q, count, whole);
+                    T* const to = g + shape.head + ((uint64_t)v0 + threadIdx.x) * E;
 #pragma unroll
                     for (int u = 0; u < kUnroll; ++u) {
-                        const uint32_t i = threadIdx.x + u * threads;
-                        if (i >= count) break;
+                        if (!decltype(whole)::value && threadIdx.x + u * threads >= count) break;
                         float f[E];
                         Type<T>::unpack(q[u], f);
-                        if (!o.far) {
+                        if constexpr (decltype(plain)::value) {
 #pragma unroll
                             for (int j = 0; j < E; j += 2) {
                                 const float2 x = fma2(Pair(f[j], f[j + 1]), c2, r2).get();
                                 const float2 y = mul2(Pair(ex2(x.x), ex2(x.y)), k2).get();
                                 f[j] = y.x, f[j + 1] = y.y;
                             }
+                            __stcs(reinterpret_cast<uint4*>(to) + u * threads, Type<T>::pack(f));
                         } else {
 #pragma unroll
-                            for (int j = 0; j < E; ++j) f[j] = ex2(o.exponent(f[j], c)) * k_out;
-                        }
-                        if (same_offset) {
-                            __stcs(reinterpret_cast<uint4*>(to) + i, Type<T>::pack(f));
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < E; ++j) to[(uint64_t)i * E + j] = Type<T>::round(f[j]);
+                            for (int j = 0; j < E; ++j)
+                                to[(uint64_t)u * threads * E + j] = Type<T>::round(ex2(o.exponent(f[j], c)) * k_out);
                         }
                     }
-                    if (lost) to[0] = Type<T>::round(NAN);
+                };
+                if (same_offset && !o.far) {
+                    for (uint32_t v0 = 0; v0 < whole_vecs; v0 += lay.chunk_vecs) write(v0, std::true_type(), std::true_type());
+                    if (whole_vecs < shape.vecs) write(whole_vecs, std::false_type(), std::true_type());
+                } else {
+                    for (uint32_t v0 = 0; v0 < shape.vecs; v0 += lay.chunk_vecs) write(v0, std::false_type(), std::false_type());
                 }
+                if (lost && shape.vecs > 0) g[shape.head] = Type<T>::round(NAN);
                 if (threadIdx.x < edge) g[v_edge] = Type<T>::round(ex2(o.exponent(f_edge, c)) * k_out);
             }
         }
@@ -767,7 +821,7 @@ int launch(const DistillArgs& a, cudaStream_t st)
     }
     // As many rows in work as SMs hold, but for the gradient no more than L2 keeps until the second pass.
     uint64_t most = 227 * 1024 / (smem + 2048);
-    const uint64_t by_threads = 1024 / (lay.threads + 64);  // 64 registers each
+    const uint64_t by_threads = (uint64_t)kMaxThreads * kCtas / (lay.threads + 64);
     most = most < 1 ? 1 : most < by_threads ? most : by_threads;
     if ((kWhat & kLoss) && (kWhat & kGrad)) {
         const uint64_t fit = kRowsInL2 / ((uint64_t)sms * bytes);
