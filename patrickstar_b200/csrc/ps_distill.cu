@@ -313,7 +313,8 @@ struct Listed {
 // Threads and shared memory of a CTA: chunks of kUnroll vectors a thread, a ring of them, barriers, listed entries,
 // bitmaps.
 struct Layout {
-    uint32_t chunk_vecs, slots, threads;  // vectors of a chunk, chunks of the ring, threads of the pass
+    uint32_t chunk_vecs, slots, threads;  // vectors of a chunk, chunks of the ring, threads of the pass (2^shift)
+    uint32_t shift;
 };
 __host__ __device__ __forceinline__ uint32_t bitmap_words(uint32_t vocab) { return (vocab + 63) / 64 * 2; }
 __host__ __device__ __forceinline__ uint32_t round4(uint32_t k) { return (k + 3) & ~3u; }
@@ -331,9 +332,10 @@ __host__ __device__ __forceinline__ size_t smem_bytes(const Layout& l, uint32_t 
 template <typename T>
 __device__ __forceinline__ uint32_t owner_of(const Layout& lay, const RowShape& s, uint32_t v, uint32_t* bit)
 {
-    const uint32_t i = (v - s.head) / Type<T>::kVec, chunk = i / lay.chunk_vecs, t = i % lay.threads;
+    static_assert(kUnroll == 4, "a chunk is four vectors a thread");
+    const uint32_t i = (v - s.head) / Type<T>::kVec, t = i & (lay.threads - 1);
     *bit = t & 31;
-    return chunk * (lay.threads >> 5) + (t >> 5);
+    return ((i >> (lay.shift + 2)) << (lay.shift - 5)) + (t >> 5);
 }
 
 __device__ __forceinline__ float grad_factor(const DistillArgs& a, float scale)
@@ -601,10 +603,11 @@ __global__ void __launch_bounds__(kMaxThreads, kCtas) distill_kernel(const Disti
             float f_edge = -INFINITY;
             if (threadIdx.x < edge) f_edge = Type<T>::load(z + v_edge);
 
-            // the next chunk's vectors of this thread into q; `count` is the vectors the chunk has
-            auto take = [&](uint4(&q)[kUnroll], uint32_t count, auto whole) {
+            // the next chunk's vectors of this thread into q, of `count` that the row has left, after `look` saw them
+            auto take = [&](uint4(&q)[kUnroll], uint32_t count, auto whole, auto&& look) {
                 if (!tc::bar_wait(&full[at], phase, &gave_up)) lost = true;
-                const uint4* const from = reinterpret_cast<const uint4*>(smem) + at * lay.chunk_vecs + threadIdx.x;
+                uint4* const from = reinterpret_cast<uint4*>(smem) + at * lay.chunk_vecs + threadIdx.x;
+                look(from);
 #pragma unroll
                 for (int u = 0; u < kUnroll; ++u) {
                     if constexpr (!decltype(whole)::value) {
@@ -628,16 +631,36 @@ __global__ void __launch_bounds__(kMaxThreads, kCtas) distill_kernel(const Disti
                 auto add = [&](uint32_t v0, auto whole) {
                     const uint32_t count = shape.vecs - v0;
                     uint4 q[kUnroll];
-                    take(q, count, whole);
+                    take(q, count, whole, [&](uint4* from) {
+                        if (!kBucket) return;
+                        const bool some = (*owners >> lane) & 1;
+                        owners += warps;
+                        if (!some) return;
+                        // the listed elements of this thread are summed apart, and taken out of the chunk
+                        uint32_t in = 0;
+#pragma unroll
+                        for (uint32_t u = 0; u < kUnroll; ++u) {
+                            const uint32_t i = v0 + threadIdx.x + u * threads;
+                            if (i < shape.vecs)
+                                in |= (E == 8 ? (uint32_t)bytes[i] : (bytes[i >> 1] >> (4 * (i & 1))) & 15u) << (8 * u);
+                        }
+                        for (; in != 0; in &= in - 1) {
+                            const uint32_t bit = __ffs(in) - 1;
+                            T* const e = reinterpret_cast<T*>(from + (bit >> 3) * threads) + (bit & 7);
+                            const float f = Type<T>::load(e);
+                            run.raise(f, c);
+                            run.in += ex2(run.o.exponent(f, c));
+                            *e = Type<T>::round(-INFINITY);
+                        }
+                        tc::fence_to_async();  // the next copy into this place comes after these writes
+                    });
                     uint32_t top = Type<T>::kNothing;
 #pragma unroll
                     for (int u = 0; u < kUnroll; ++u)
                         top = Type<T>::larger(
                             top, Type<T>::larger(Type<T>::larger(q[u].x, q[u].y), Type<T>::larger(q[u].z, q[u].w)));
                     run.raise(Type<T>::fold(top), c);
-                    bool any = run.o.far;
-                    if (kBucket) any = any || ((*owners >> lane) & 1), owners += warps;
-                    if (!any) {
+                    if (!run.o.far) {
                         const Pair c2(c, c), r2(-run.o.r, -run.o.r);
 #pragma unroll
                         for (int u = 0; u < kUnroll; ++u) {
@@ -656,19 +679,8 @@ __global__ void __launch_bounds__(kMaxThreads, kCtas) distill_kernel(const Disti
                         for (int u = 0; u < kUnroll; ++u) {
                             float f[E];
                             Type<T>::unpack(q[u], f);
-                            uint32_t in = 0;
-                            if (kBucket) {
-                                const uint32_t i = min(v0 + threadIdx.x + u * threads, shape.vecs - 1);
-                                in = E == 8 ? bytes[i] : (bytes[i >> 1] >> (4 * (i & 1))) & 15u;
-                            }
 #pragma unroll
-                            for (int j = 0; j < E; ++j) {
-                                const float e = ex2(run.o.exponent(f[j], c));
-                                if (kBucket && ((in >> j) & 1))
-                                    run.in += e;
-                                else
-                                    out += e;
-                            }
+                            for (int j = 0; j < E; ++j) out += ex2(run.o.exponent(f[j], c));
                         }
                         run.out = add2(run.out, Pair(out, 0.f));
                     }
@@ -726,7 +738,7 @@ __global__ void __launch_bounds__(kMaxThreads, kCtas) distill_kernel(const Disti
                     const Pair c2(c, c), r2(-o.r, -o.r), k2(k_out, k_out);
                     const uint32_t count = shape.vecs - v0;
                     uint4 q[kUnroll];
-                    take(q, count, whole);
+                    take(q, count, whole, [](uint4*) {});
                     T* const to = g + shape.head + ((uint64_t)v0 + threadIdx.x) * E;
 #pragma unroll
                     for (int u = 0; u < kUnroll; ++u) {
@@ -800,11 +812,13 @@ int launch(const DistillArgs& a, cudaStream_t st)
 {
     const int sms = ps_internal::sm_count();
     if (sms < 0) return sms;
-    // Threads and chunks for a row by its size: four vectors a thread and chunk, four chunks, and from three CTAs
-    // of 64 KB on an SM (rows above 48 KB) to eight small ones, whose rows' own latencies overlap.
+    // Threads and chunks for a row by its size: four vectors a thread and chunk, four chunks.  Small CTAs, since each
+    // brings a warp for listed entries and rows' own latencies overlap (8192 x 50257 fp16, loss: 158 us with 128
+    // threads, 167 us with 256); for the longest rows, of which L2 holds two an SM, more threads.
     const uint64_t bytes = (uint64_t)a.vocab * sizeof(T);
     Layout lay;
-    lay.threads = bytes <= 16 * 1024 ? 64 : bytes <= 48 * 1024 ? 128 : 256;
+    lay.shift = bytes <= 16 * 1024 ? 6 : bytes <= 160 * 1024 ? 7 : 8;
+    lay.threads = 1u << lay.shift;
     lay.chunk_vecs = kUnroll * lay.threads;
     lay.slots = kMaxSlots;
     const bool bits = kBucket && (kWhat & kLoss);
