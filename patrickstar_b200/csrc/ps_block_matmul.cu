@@ -45,6 +45,7 @@ struct ProductArgs {
     int a_k_inner, b_k_inner;  // the contracted dimension is the contiguous one
     int bias_dtype, out_dtype;
     int vec;                   // output rows start on 16-byte boundaries
+    int bias_vec;              // the bias does
 };
 
 __device__ __forceinline__ float bias_at(const ProductArgs& p, uint32_t col)
@@ -52,6 +53,27 @@ __device__ __forceinline__ float bias_at(const ProductArgs& p, uint32_t col)
     if (p.bias_dtype == PS_DTYPE_F16) return __half2float(reinterpret_cast<const __half*>(p.bias)[col]);
     if (p.bias_dtype == PS_DTYPE_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.bias)[col]);
     return reinterpret_cast<const float*>(p.bias)[col];
+}
+// Bias of four columns, 0 behind the last one; the same in all lanes.
+__device__ __forceinline__ float4 bias4_at(const ProductArgs& p, uint32_t col)
+{
+    float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (p.bias_vec && col + 4 <= p.n) {
+        if (p.bias_dtype == PS_DTYPE_F32) return __ldg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.bias) + col));
+        const uint2 w = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p.bias) + col));
+        if (p.bias_dtype == PS_DTYPE_F16) {
+            const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
+            const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+            return make_float4(lo.x, lo.y, hi.x, hi.y);
+        }
+        return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
+                           __uint_as_float(w.y & 0xffff0000u));
+    }
+    if (col < p.n) b.x = bias_at(p, col);
+    if (col + 1 < p.n) b.y = bias_at(p, col + 1);
+    if (col + 2 < p.n) b.z = bias_at(p, col + 2);
+    if (col + 3 < p.n) b.w = bias_at(p, col + 3);
+    return b;
 }
 __device__ __forceinline__ uint32_t pack2(int dtype, float lo, float hi)
 {
@@ -288,27 +310,72 @@ __device__ __forceinline__ void stage_row(unsigned char* buf, uint32_t row, cons
     }
 #pragma unroll
     for (uint32_t q = 0; q < 8; ++q) {  // 16 bytes each, swizzled as the store's map says
-        uint4 w;
-        if constexpr (kOut == PS_DTYPE_F32) {
-            float f[4];
+        constexpr uint32_t kPer = kOut == PS_DTYPE_F32 ? 4 : 8;
+        float f[kPer];
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-                f[i] = __uint_as_float(v[0][4 * q + i]);
-                if (p.bias != nullptr && col + 4 * q + i < p.n) f[i] += bias_at(p, col + 4 * q + i);
-                if (!good) f[i] = __int_as_float(0x7fffffff);
+        for (uint32_t i = 0; i < kPer; ++i) f[i] = __uint_as_float(v[q * kPer / 32][(q * kPer + i) % 32]);
+        if (p.bias != nullptr) {
+#pragma unroll
+            for (uint32_t i = 0; i < kPer; i += 4) {
+                const float4 b = bias4_at(p, col + q * kPer + i);
+                f[i] += b.x, f[i + 1] += b.y, f[i + 2] += b.z, f[i + 3] += b.w;
             }
+        }
+        if (!good) {
+#pragma unroll
+            for (uint32_t i = 0; i < kPer; ++i) f[i] = __int_as_float(0x7fffffff);
+        }
+        uint4 w;
+        if constexpr (kOut == PS_DTYPE_F32)
             w = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+        else
+            w = make_uint4(pack2(kOut, f[0], f[1]), pack2(kOut, f[2], f[3]), pack2(kOut, f[4], f[5]), pack2(kOut, f[6], f[7]));
+        *reinterpret_cast<uint4*>(buf + row * 128 + ((q ^ (row & 7)) << 4)) = w;
+    }
+}
+
+// The staged 32 rows to an output whose rows start anywhere: eight rows at a time, 4 bytes a lane.  In 16 bits
+// the pairs of a row begin with its first or its second element, whichever is on a 4-byte boundary; what is left
+// at the ends of the row is stored by itself.
+template <int kOut>
+__device__ __forceinline__ void store_rows(const ProductArgs& p, const unsigned char* buf, uint32_t row0, uint32_t col)
+{
+    constexpr uint32_t kCols = kOut == PS_DTYPE_F32 ? 32 : 64;
+    const uint32_t lane = threadIdx.x & 31;
+    const uint32_t rows = min(32u, p.m - row0), cols = min(kCols, p.n - col);
+    for (uint32_t r0 = 0; r0 < rows; r0 += 8) {
+        if constexpr (kOut == PS_DTYPE_F32) {
+            float v[8];
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i)
+                v[i] = *reinterpret_cast<const float*>(buf + (r0 + i) * 128 + (((lane >> 2) ^ i) << 4) + (lane & 3) * 4);
+            float* o = reinterpret_cast<float*>(p.out) + (uint64_t)(row0 + r0) * p.ldo + col + lane;
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i)
+                if (r0 + i < rows && lane < cols) o[i * p.ldo] = v[i];
         } else {
-            float f[8];
+            uint16_t* const out = reinterpret_cast<uint16_t*>(p.out) + (uint64_t)(row0 + r0) * p.ldo + col;
+            uint32_t lo[8], hi[8];
 #pragma unroll
             for (uint32_t i = 0; i < 8; ++i) {
-                f[i] = __uint_as_float(v[q / 4][8 * (q & 3) + i]);
-                if (p.bias != nullptr && col + 8 * q + i < p.n) f[i] += bias_at(p, col + 8 * q + i);
-                if (!good) f[i] = __int_as_float(0x7fffffff);
+                const uint32_t odd = (uint32_t)((uintptr_t)(out + i * p.ldo) >> 1) & 1;
+                const uint32_t e = 2 * lane + odd, f = min(e + 1, kCols - 1);
+                const unsigned char* const row = buf + (r0 + i) * 128;
+                lo[i] = *reinterpret_cast<const uint16_t*>(row + (((e >> 3) ^ i) << 4) + (e & 7) * 2);
+                hi[i] = *reinterpret_cast<const uint16_t*>(row + (((f >> 3) ^ i) << 4) + (f & 7) * 2);
             }
-            w = make_uint4(pack2(kOut, f[0], f[1]), pack2(kOut, f[2], f[3]), pack2(kOut, f[4], f[5]), pack2(kOut, f[6], f[7]));
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+                if (r0 + i >= rows) break;
+                uint16_t* const o = out + i * p.ldo;
+                const uint32_t odd = (uint32_t)((uintptr_t)o >> 1) & 1, e = 2 * lane + odd;
+                if (e + 1 < cols)
+                    *reinterpret_cast<uint32_t*>(o + e) = lo[i] | (hi[i] << 16);
+                else if (e < cols)
+                    o[e] = (uint16_t)lo[i];
+                if (odd && lane == 0) o[0] = *reinterpret_cast<const uint16_t*>(buf + (r0 + i) * 128 + (i << 4));
+            }
         }
-        *reinterpret_cast<uint4*>(buf + row * 128 + ((q ^ (row & 7)) << 4)) = w;
     }
 }
 
@@ -456,18 +523,7 @@ block_matmul_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                 if (p.vec) {
                     if (lane == 0) tc::store_box(&map_out, tc::smem_u32(buf), (int)col, (int)row0);
                 } else {
-                    const uint32_t rows = min(32u, p.m - row0), cols = min(kCols, p.n - col);
-                    for (uint32_t r = 0; r < rows; ++r) {
-                        const uint64_t o = (uint64_t)(row0 + r) * p.ldo + col;
-                        for (uint32_t e = lane; e < cols; e += 32) {
-                            constexpr uint32_t kPer = kOut == PS_DTYPE_F32 ? 4 : 8;
-                            const unsigned char* at = buf + r * 128 + (((e / kPer) ^ (r & 7)) << 4);
-                            if constexpr (kOut == PS_DTYPE_F32)
-                                reinterpret_cast<float*>(p.out)[o + e] = reinterpret_cast<const float*>(at)[e % kPer];
-                            else
-                                reinterpret_cast<uint16_t*>(p.out)[o + e] = reinterpret_cast<const uint16_t*>(at)[e % kPer];
-                        }
-                    }
+                    store_rows<kOut>(p, buf, row0, col);
                     __syncwarp();
                 }
             }
@@ -670,6 +726,7 @@ int ps_block_matmul(const ps_block_operand* a, const ps_block_operand* b, uint32
     }
     p.bias = bias_dev, p.bias_dtype = bias_dtype, p.out = out_dev, p.out_dtype = out_dtype, p.ldo = ldo;
     p.m = m, p.n = n, p.n_kb = ceil_div(k, kTile);
+    p.bias_vec = (uintptr_t)bias_dev % 16 == 0;
     p.vec = (uintptr_t)out_dev % 16 == 0 && (ldo * osize) % 16 == 0;
     const int sms = ps_internal::sm_count();
     if (sms < 0) return sms;

@@ -13,17 +13,19 @@
 // the overflow test behind the product.
 //
 // One CTA takes a 128 x 128 tile into registers with all of its loads in
-// flight at once, reduces the magnitudes as integers (an IEEE magnitude orders
-// like its bits, two 16-bit ones to a word), and writes every output the caller
-// wants from that one read: 2 bytes in and 1 or 2 bytes out per 16-bit element.
-// HBM-bound.
+// flight at once, reduces the magnitudes (two 16-bit ones to a word), and writes
+// every output the caller wants from that one read: 2 bytes in and 1 or 2 bytes
+// out per 16-bit element.  HBM-bound, if it gets by with few instructions.
 #include "ps_b200.h"
 
 #include "ps_internal.h"
+#include "ps_pair.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
+
+#include <type_traits>
 
 namespace {
 
@@ -33,86 +35,72 @@ constexpr int kRowsPerThread = 8;  // 16 threads across 128 columns, 16 down, 8 
 constexpr int kWarps = kThreads / 32;
 
 // ---------------------------------------------------------------------------
-// eight consecutive elements of a row, as loaded
+// eight consecutive elements of a row, as loaded, and magnitudes in the same words
 // ---------------------------------------------------------------------------
 template <typename T>
-struct Vec8;
-
-template <>
-struct Vec8<__half> {
-    static constexpr int kWords = 4;  // two magnitudes in each
-    static constexpr uint32_t kInf = 0x7c00u;
-    uint32_t w[4];
-    __device__ __forceinline__ uint32_t key(int i) const { return w[i] & 0x7fff7fffu; }
-    __device__ __forceinline__ float value(int j) const
-    {
-        return __half2float(__ushort_as_half((unsigned short)(w[j >> 1] >> (16 * (j & 1)))));
-    }
-    __device__ __forceinline__ void set(int j, const __half* p)
-    {
-        w[j >> 1] |= (uint32_t)__half_as_ushort(*p) << (16 * (j & 1));
-    }
-};
-template <>
-struct Vec8<__nv_bfloat16> {
+struct Vec8 {  // 16-bit types: two to a word
     static constexpr int kWords = 4;
-    static constexpr uint32_t kInf = 0x7f80u;
+    static constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
     uint32_t w[4];
-    __device__ __forceinline__ uint32_t key(int i) const { return w[i] & 0x7fff7fffu; }
-    __device__ __forceinline__ float value(int j) const
+    __device__ __forceinline__ void set(int j, const T* p)
     {
-        return __uint_as_float((j & 1) ? (w[j >> 1] & 0xffff0000u) : (w[j >> 1] << 16));
+        w[j >> 1] |= (uint32_t)*reinterpret_cast<const unsigned short*>(p) << (16 * (j & 1));
     }
-    __device__ __forceinline__ void set(int j, const __nv_bfloat16* p)
+    __device__ __forceinline__ void get(float (&f)[8]) const
     {
-        w[j >> 1] |= (uint32_t)__bfloat16_as_ushort(*p) << (16 * (j & 1));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (std::is_same<T, __half>::value) {
+                const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+                f[2 * i] = t.x, f[2 * i + 1] = t.y;
+            } else {
+                f[2 * i] = __uint_as_float(w[i] << 16), f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            }
+        }
+    }
+    // the larger of `m` and the magnitude of x; a NaN gives way
+    static __device__ __forceinline__ uint32_t raise(uint32_t m, uint32_t x)
+    {
+        const T2 r = __hmax2(__habs2(*reinterpret_cast<const T2*>(&x)), *reinterpret_cast<const T2*>(&m));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+    static __device__ __forceinline__ bool has_inf(uint32_t m) { return (m & 0xffffu) == kInf || (m >> 16) == kInf; }
+    static __device__ __forceinline__ uint32_t without_inf(uint32_t x)
+    {
+        const uint32_t m = x & 0x7fff7fffu;
+        return x & ~(((m & 0xffffu) == kInf ? 0xffffu : 0u) | ((m >> 16) == kInf ? 0xffff0000u : 0u));
+    }
+    // of the two magnitudes in a word
+    static __device__ __forceinline__ uint32_t fold(uint32_t m) { return max(m & 0xffffu, m >> 16); }
+    static __device__ __forceinline__ float magnitude(uint32_t m)  // in the low half
+    {
+        if constexpr (std::is_same<T, __half>::value)
+            return __half2float(__ushort_as_half((unsigned short)m));
+        else
+            return __uint_as_float(m << 16);
     }
 };
 template <>
-struct Vec8<float> {
-    static constexpr int kWords = 8;  // one magnitude in each
+struct Vec8<float> {  // one to a word
+    static constexpr int kWords = 8;
     static constexpr uint32_t kInf = 0x7f800000u;
     uint32_t w[8];
-    __device__ __forceinline__ uint32_t key(int i) const { return w[i] & 0x7fffffffu; }
-    __device__ __forceinline__ float value(int j) const { return __uint_as_float(w[j]); }
     __device__ __forceinline__ void set(int j, const float* p) { w[j] = __float_as_uint(*p); }
+    __device__ __forceinline__ void get(float (&f)[8]) const
+    {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(w[i]);
+    }
+    static __device__ __forceinline__ uint32_t raise(uint32_t m, uint32_t x)
+    {
+        return __float_as_uint(fmaxf(fabsf(__uint_as_float(x)), __uint_as_float(m)));
+    }
+    static __device__ __forceinline__ bool has_inf(uint32_t m) { return m == kInf; }
+    static __device__ __forceinline__ uint32_t without_inf(uint32_t x) { return (x & 0x7fffffffu) == kInf ? 0u : x; }
+    static __device__ __forceinline__ uint32_t fold(uint32_t m) { return m; }
+    static __device__ __forceinline__ float magnitude(uint32_t m) { return __uint_as_float(m); }
 };
-
-template <typename T>
-__device__ __forceinline__ uint32_t key_max(uint32_t a, uint32_t b)
-{
-    if constexpr (sizeof(T) == 2)
-        return __vmaxu2(a, b);
-    else
-        return a > b ? a : b;
-}
-template <typename T>
-__device__ __forceinline__ uint32_t drop_nonfinite(uint32_t k)
-{
-    if constexpr (sizeof(T) == 2)
-        return k & ~__vcmpgeu2(k, Vec8<T>::kInf * 0x10001u);
-    else
-        return k >= Vec8<T>::kInf ? 0u : k;
-}
-// the larger of the magnitudes a word holds
-template <typename T>
-__device__ __forceinline__ uint32_t key_fold(uint32_t k)
-{
-    if constexpr (sizeof(T) == 2)
-        return max(k & 0xffffu, k >> 16);
-    else
-        return k;
-}
-template <typename T>
-__device__ __forceinline__ float key_float(uint32_t k)
-{
-    if constexpr (std::is_same<T, __half>::value)
-        return __half2float(__ushort_as_half((unsigned short)k));
-    else if constexpr (std::is_same<T, __nv_bfloat16>::value)
-        return __uint_as_float(k << 16);
-    else
-        return __uint_as_float(k);
-}
 
 // scale byte of a finite magnitude
 template <int kFmt>
@@ -171,8 +159,16 @@ struct QuantArgs {
 __host__ __device__ constexpr bool has_row(int mode) { return mode == PS_BLOCKS_ROW || mode == PS_BLOCKS_ROW_COL; }
 __host__ __device__ constexpr bool has_col(int mode) { return mode == PS_BLOCKS_COL || mode == PS_BLOCKS_ROW_COL; }
 
+// CTAs an SM holds: a tile is 32 registers a thread in 16 bits, 64 in 32
+template <typename T>
+__host__ __device__ constexpr int ctas_of()
+{
+    return sizeof(T) == 2 ? 4 : 2;
+}
+
 struct Shared {
     uint32_t key[kWarps][16][8];
+    float inv[kBlock];
     float sum[kWarps][kBlock];
 };
 
@@ -180,6 +176,7 @@ template <typename T, int kMode, int kFmt, bool kSum>
 __device__ __forceinline__ void quantize_tile(const QuantArgs& a, uint32_t tile, Shared& sh)
 {
     using V = Vec8<T>;
+    constexpr bool kRow = has_row(kMode), kCol = has_col(kMode), kTile = kMode == PS_BLOCKS_TILE;
     const uint32_t cb = tile % a.col_blocks, rb = tile / a.col_blocks;
     const uint32_t cg = threadIdx.x & 15, rg = threadIdx.x >> 4;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -211,9 +208,8 @@ __device__ __forceinline__ void quantize_tile(const QuantArgs& a, uint32_t tile,
 
     // magnitudes: rk[i] over the 8 elements of row i, ck[k] over the thread's 8 rows
     uint32_t rk[kRowsPerThread], ck[V::kWords];
-    bool odd = false;  // holds an element that is not finite
-    {
-        uint32_t all = 0;
+    bool odd = false;  // holds an infinity (a NaN gives way to any number, and converts to one)
+    auto maxima = [&](auto&& of) {
 #pragma unroll
         for (int k = 0; k < V::kWords; ++k) ck[k] = 0;
 #pragma unroll
@@ -221,121 +217,88 @@ __device__ __forceinline__ void quantize_tile(const QuantArgs& a, uint32_t tile,
             rk[i] = 0;
 #pragma unroll
             for (int k = 0; k < V::kWords; ++k) {
-                const uint32_t key = v[i].key(k);
-                rk[i] = key_max<T>(rk[i], key);
-                ck[k] = key_max<T>(ck[k], key);
-            }
-            all = key_max<T>(all, rk[i]);
-        }
-        odd = key_fold<T>(all) >= V::kInf;
-        if (odd) {
-#pragma unroll
-            for (int k = 0; k < V::kWords; ++k) ck[k] = 0;
-#pragma unroll
-            for (int i = 0; i < kRowsPerThread; ++i) {
-                rk[i] = 0;
-#pragma unroll
-                for (int k = 0; k < V::kWords; ++k) {
-                    const uint32_t key = drop_nonfinite<T>(v[i].key(k));
-                    rk[i] = key_max<T>(rk[i], key);
-                    ck[k] = key_max<T>(ck[k], key);
-                }
+                if (kRow) rk[i] = V::raise(rk[i], of(v[i].w[k]));
+                if (kCol || kTile) ck[k] = V::raise(ck[k], of(v[i].w[k]));
             }
         }
+        uint32_t all = 0;
+        if constexpr (kCol || kTile) {
+#pragma unroll
+            for (int k = 0; k < V::kWords; ++k) all = V::raise(all, ck[k]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kRowsPerThread; ++i) all = V::raise(all, rk[i]);
+        }
+        return all;
+    };
+    const uint32_t thread_max = maxima([](uint32_t w) { return w; });
+    if (V::has_inf(thread_max)) {
+        odd = true;
+        maxima([](uint32_t w) { return V::without_inf(w); });
     }
 
-    auto put_row = [&](uint8_t* q, int i, const float* inv, bool one) {
-        const uint32_t r = r0 + 16 * i;
-        if (r >= a.rows || c0 >= a.cols) return;
-        uint32_t out[2];
+    float row_inv[kRowsPerThread];
+    if constexpr (kRow) {
+        if constexpr (sizeof(T) == 2) {  // two rows to a word
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int j = 4 * h;
-            const uint32_t lo = to_fp8x2<kFmt>(v[i].value(j) * inv[one ? 0 : j], v[i].value(j + 1) * inv[one ? 0 : j + 1]);
-            const uint32_t hi = to_fp8x2<kFmt>(v[i].value(j + 2) * inv[one ? 0 : j + 2], v[i].value(j + 3) * inv[one ? 0 : j + 3]);
-            out[h] = lo | (hi << 16);
-        }
-        if (odd) {
+            for (int i = 0; i < kRowsPerThread; i += 2) {
+                uint32_t m = V::fold(rk[i]) | (V::fold(rk[i + 1]) << 16);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float f = v[i].value(j);
-                if (!(fabsf(f) < __int_as_float(0x7f800000)))
-                    out[j >> 2] = (out[j >> 2] & ~(0xffu << (8 * (j & 3)))) | (nonfinite_fp8<kFmt>(f) << (8 * (j & 3)));
+                for (int d = 1; d < 16; d <<= 1) m = V::raise(m, __shfl_xor_sync(0xffffffffu, m, d));
+                rk[i] = m & 0xffffu, rk[i + 1] = m >> 16;
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kRowsPerThread; ++i)
+#pragma unroll
+                for (int d = 1; d < 16; d <<= 1) rk[i] = V::raise(rk[i], __shfl_xor_sync(0xffffffffu, rk[i], d));
         }
-        *reinterpret_cast<uint2*>(q + (size_t)r * a.ldq + c0) = make_uint2(out[0], out[1]);
-    };
-
-    if constexpr (has_row(kMode)) {
 #pragma unroll
         for (int i = 0; i < kRowsPerThread; ++i) {
-#pragma unroll
-            for (int d = 1; d < 16; d <<= 1) rk[i] = key_max<T>(rk[i], __shfl_xor_sync(0xffffffffu, rk[i], d));
-            const uint32_t byte = scale_byte<kFmt>(key_float<T>(key_fold<T>(rk[i])));
-            const float inv = scale_inverse(byte);
-            put_row(a.q1, i, &inv, true);
-            if (cg == 0) {
+            const uint32_t byte = scale_byte<kFmt>(V::magnitude(rk[i]));
+            row_inv[i] = scale_inverse(byte);
+            if (cg == i) {
                 const uint32_t r = r0 + 16 * i;
                 put_scale(a.s1, r, cb, a.col_blocks, a.row_blocks, r < a.rows ? byte : 0u);
             }
         }
     }
-
-    if constexpr (kSum) {
-        float cs[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            cs[j] = 0.f;
-#pragma unroll
-            for (int i = 0; i < kRowsPerThread; ++i) cs[j] += v[i].value(j);
-            cs[j] += __shfl_xor_sync(0xffffffffu, cs[j], 16);
-        }
-        if (lane < 16) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sh.sum[warp][cg * 8 + j] = cs[j];
-        }
-    }
-
-    if constexpr (has_col(kMode)) {
+    float col_inv[8];
+    if constexpr (kCol) {
 #pragma unroll
         for (int k = 0; k < V::kWords; ++k) {
-            ck[k] = key_max<T>(ck[k], __shfl_xor_sync(0xffffffffu, ck[k], 16));
+            ck[k] = V::raise(ck[k], __shfl_xor_sync(0xffffffffu, ck[k], 16));
             if (lane < 16) sh.key[warp][cg][k] = ck[k];
         }
         __syncthreads();
+        if (threadIdx.x < kBlock) {
+            const uint32_t c = cb * kBlock + threadIdx.x, j = threadIdx.x & 7;
+            uint32_t m = 0;
 #pragma unroll
-        for (int k = 0; k < V::kWords; ++k) {
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) ck[k] = key_max<T>(ck[k], sh.key[w][cg][k]);
+            for (int w = 0; w < kWarps; ++w)
+                m = V::raise(m, sh.key[w][threadIdx.x >> 3][sizeof(T) == 2 ? j >> 1 : j]);
+            if (sizeof(T) == 2) m = (m >> (16 * (j & 1))) & 0xffffu;
+            const uint32_t byte = scale_byte<kFmt>(V::magnitude(m));
+            sh.inv[threadIdx.x] = scale_inverse(byte);
+            put_scale(a.s0, c, rb, a.row_blocks, a.col_blocks, c < a.cols ? byte : 0u);
         }
-        float inv[8];
-        uint32_t byte[8];
+        __syncthreads();
+        const float4 lo = *reinterpret_cast<const float4*>(&sh.inv[cg * 8]), hi = *reinterpret_cast<const float4*>(&sh.inv[cg * 8 + 4]);
+        col_inv[0] = lo.x, col_inv[1] = lo.y, col_inv[2] = lo.z, col_inv[3] = lo.w;
+        col_inv[4] = hi.x, col_inv[5] = hi.y, col_inv[6] = hi.z, col_inv[7] = hi.w;
+    }
+    if constexpr (kTile) {
+        uint32_t m = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const uint32_t key = sizeof(T) == 2 ? (ck[j >> 1] >> (16 * (j & 1))) & 0xffffu : ck[j % V::kWords];
-            byte[j] = scale_byte<kFmt>(key_float<T>(key));
-            inv[j] = scale_inverse(byte[j]);
-        }
-#pragma unroll
-        for (int i = 0; i < kRowsPerThread; ++i) put_row(a.q0, i, inv, false);
-        if (rg == 0) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                put_scale(a.s0, c0 + j, rb, a.row_blocks, a.col_blocks, c0 + j < a.cols ? byte[j] : 0u);
-        }
-    } else if constexpr (kMode == PS_BLOCKS_TILE) {
-        uint32_t key = 0;
-#pragma unroll
-        for (int k = 0; k < V::kWords; ++k) key = key_max<T>(key, ck[k]);
-        key = __reduce_max_sync(0xffffffffu, key_fold<T>(key));
-        if (lane == 0) sh.key[warp][0][0] = key;
+        for (int k = 0; k < V::kWords; ++k) m = V::raise(m, ck[k]);
+        m = __reduce_max_sync(0xffffffffu, V::fold(m));  // magnitudes order like their bits
+        if (lane == 0) sh.key[warp][0][0] = m;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) key = max(key, sh.key[w][0][0]);
-        const uint32_t byte = scale_byte<kFmt>(key_float<T>(key));
-        const float inv = scale_inverse(byte);
+        for (int w = 0; w < kWarps; ++w) m = max(m, sh.key[w][0][0]);
+        const uint32_t byte = scale_byte<kFmt>(V::magnitude(m));
 #pragma unroll
-        for (int i = 0; i < kRowsPerThread; ++i) put_row(a.q1, i, &inv, true);
+        for (int i = 0; i < kRowsPerThread; ++i) row_inv[i] = scale_inverse(byte);
         if (threadIdx.x < kBlock) {
             const uint32_t r = rb * kBlock + threadIdx.x, c = cb * kBlock + threadIdx.x;
             put_scale(a.s1, r, cb, a.col_blocks, a.row_blocks, r < a.rows ? byte : 0u);
@@ -343,8 +306,59 @@ __device__ __forceinline__ void quantize_tile(const QuantArgs& a, uint32_t tile,
         }
     }
 
+    // every row is unpacked once, for all that is made of it
+    Pair sums[4] = {Pair(0.f, 0.f), Pair(0.f, 0.f), Pair(0.f, 0.f), Pair(0.f, 0.f)};
+    uint8_t* q1 = a.q1 + (size_t)r0 * a.ldq + c0;
+    uint8_t* q0 = a.q0 + (size_t)r0 * a.ldq + c0;
+    auto convert = [&](const float(&f)[8], const Pair(&inv)[4], uint8_t* q) {
+        uint32_t out[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const float2 lo = mul2(Pair(f[4 * h], f[4 * h + 1]), inv[2 * h]).get();
+            const float2 hi = mul2(Pair(f[4 * h + 2], f[4 * h + 3]), inv[2 * h + 1]).get();
+            out[h] = to_fp8x2<kFmt>(lo.x, lo.y) | (to_fp8x2<kFmt>(hi.x, hi.y) << 16);
+        }
+        if (odd) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (!(fabsf(f[j]) < __int_as_float(0x7f800000)))
+                    out[j >> 2] = (out[j >> 2] & ~(0xffu << (8 * (j & 3)))) | (nonfinite_fp8<kFmt>(f[j]) << (8 * (j & 3)));
+        }
+        *reinterpret_cast<uint2*>(q) = make_uint2(out[0], out[1]);
+    };
+    Pair col2[4];
+    if constexpr (kCol) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) col2[j] = Pair(col_inv[2 * j], col_inv[2 * j + 1]);
+    }
+    const bool here = c0 < a.cols;
+#pragma unroll
+    for (int i = 0; i < kRowsPerThread; ++i) {
+        float f[8];
+        v[i].get(f);
+        if constexpr (kSum) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sums[j] = add2(sums[j], Pair(f[2 * j], f[2 * j + 1]));
+        }
+        if (here && r0 + 16 * i < a.rows) {
+            if constexpr (kRow || kTile) {
+                const Pair one(row_inv[i], row_inv[i]);
+                const Pair all[4] = {one, one, one, one};
+                convert(f, all, q1);
+            }
+            if constexpr (kCol) convert(f, col2, q0);
+        }
+        q1 += 16 * a.ldq, q0 += 16 * a.ldq;
+    }
+
     if constexpr (kSum) {
-        if constexpr (!has_col(kMode)) __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float2 t = sums[j].get();
+            t.x += __shfl_xor_sync(0xffffffffu, t.x, 16), t.y += __shfl_xor_sync(0xffffffffu, t.y, 16);
+            if (lane < 16) sh.sum[warp][cg * 8 + 2 * j] = t.x, sh.sum[warp][cg * 8 + 2 * j + 1] = t.y;
+        }
+        __syncthreads();
         if (threadIdx.x < kBlock) {
             const uint32_t c = cb * kBlock + threadIdx.x;
             float t = 0.f;
@@ -356,7 +370,7 @@ __device__ __forceinline__ void quantize_tile(const QuantArgs& a, uint32_t tile,
 }
 
 template <typename T, int kMode, int kFmt, bool kSum>
-__global__ void __launch_bounds__(kThreads) block_quantize_kernel(const QuantArgs a)
+__global__ void __launch_bounds__(kThreads, ctas_of<T>()) block_quantize_kernel(const QuantArgs a)
 {
     __shared__ Shared sh;
     cudaTriggerProgrammaticLaunchCompletion();
@@ -365,7 +379,7 @@ __global__ void __launch_bounds__(kThreads) block_quantize_kernel(const QuantArg
 
 // Two matrices in one launch: the input of a layer (kMode) and, behind its `split` tiles, the weight.
 template <typename T, int kMode>
-__global__ void __launch_bounds__(kThreads) quantize_layer_kernel(const QuantArgs x, const QuantArgs w, uint32_t split)
+__global__ void __launch_bounds__(kThreads, ctas_of<T>()) quantize_layer_kernel(const QuantArgs x, const QuantArgs w, uint32_t split)
 {
     __shared__ Shared sh;
     cudaTriggerProgrammaticLaunchCompletion();

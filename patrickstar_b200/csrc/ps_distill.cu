@@ -22,6 +22,7 @@
 #include "ps_b200.h"
 
 #include "ps_internal.h"
+#include "ps_pair.cuh"
 #include "ps_tensor_core.cuh"
 
 #include <cuda_bf16.h>
@@ -217,37 +218,6 @@ __device__ __forceinline__ uint32_t bit_of(const RowShape& s, uint32_t v)
     if (v < s.head) return s.vecs * E + v;
     const uint32_t u = v - s.head;
     return u < s.vecs * E ? u : u + s.head;
-}
-
-// Two 32-bit operations in one instruction.
-struct Pair {
-    uint64_t v;
-    __device__ __forceinline__ Pair() {}
-    __device__ __forceinline__ Pair(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y)); }
-    __device__ __forceinline__ float2 get() const
-    {
-        float2 f;
-        asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-        return f;
-    }
-};
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c)
-{
-    Pair d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-    return d;
-}
-__device__ __forceinline__ Pair add2(Pair a, Pair b)
-{
-    Pair d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-    return d;
-}
-__device__ __forceinline__ Pair mul2(Pair a, Pair b)
-{
-    Pair d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-    return d;
 }
 
 // What a row's powers of two are relative to: the exponent of element z is z c - r, one rounding, with
