@@ -555,8 +555,8 @@ int ps_block_matmul(const ps_block_operand* a, const ps_block_operand* b, uint32
  * dx = Q_row(dy) Q_tile(weight), dw = Q_col(dy)^T Q_col(x), db = column sums of dy.
  * x and y [tokens, k] and [tokens, n] of x_dtype; weight [n, k] of weight_dtype,
  * or, quantized before, kept_data with both scale arrays of tile blocks (weight
- * is then not read).  Row strides in elements (ld_kept: bytes); y, dx, dw, db
- * are contiguous, dx of x_dtype, dw of weight_dtype, db of bias_dtype.
+ * is then not read).  Row strides in elements (ld_kept: bytes); dw and db are
+ * contiguous, dx is of x_dtype, dw of weight_dtype, db of bias_dtype.
  *
  * keep says what the backward call will want: PS_KEEP_INPUT for dw,
  * PS_KEEP_WEIGHT for dx.  ps_fp8_linear_sizes gives the bytes of the buffers that
@@ -581,10 +581,11 @@ typedef struct ps_fp8_linear {
 } ps_fp8_linear;
 
 int ps_fp8_linear_sizes(const ps_fp8_linear* layer, int keep, uint64_t* sizes);
-int ps_fp8_linear_forward(const ps_fp8_linear* layer, int keep, void* y_dev, void* saved_dev, void* scratch_dev,
-                          void* stream);
+int ps_fp8_linear_forward(const ps_fp8_linear* layer, int keep, void* y_dev, uint64_t ld_y, void* saved_dev,
+                          void* scratch_dev, void* stream);
 int ps_fp8_linear_backward(const ps_fp8_linear* layer, int keep, const void* saved_dev, const void* dy_dev, uint64_t ld_dy,
-                           int grad_fmt, void* dx_dev, void* dw_dev, void* db_dev, void* scratch_dev, void* stream);
+                           int grad_fmt, void* dx_dev, uint64_t ld_dx, void* dw_dev, void* db_dev, void* scratch_dev,
+                           void* stream);
 
 /* Number of thread blocks of ps_block_matmul on the current device that gave up
  * a wait (2 s) since the library was loaded; such a block's part of the output

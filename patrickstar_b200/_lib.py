@@ -170,9 +170,9 @@ SIGNATURES = {
     "ps_distill_forward": (C.c_int, [C.POINTER(DistillProblem), _p, _p, _p, _p, _p, _p, C.c_uint64, _p, _p]),
     "ps_distill_backward": (C.c_int, [C.POINTER(DistillProblem), _p, _p, _p, C.c_uint32, _p, _p, C.c_uint64, _p]),
     "ps_fp8_linear_sizes": (C.c_int, [C.POINTER(Fp8LinearLayer), C.c_int, C.POINTER(C.c_uint64)]),
-    "ps_fp8_linear_forward": (C.c_int, [C.POINTER(Fp8LinearLayer), C.c_int, _p, _p, _p, _p]),
-    "ps_fp8_linear_backward": (C.c_int, [C.POINTER(Fp8LinearLayer), C.c_int, _p, _p, C.c_uint64, C.c_int, _p, _p, _p,
-                                         _p, _p]),
+    "ps_fp8_linear_forward": (C.c_int, [C.POINTER(Fp8LinearLayer), C.c_int, _p, C.c_uint64, _p, _p, _p]),
+    "ps_fp8_linear_backward": (C.c_int, [C.POINTER(Fp8LinearLayer), C.c_int, _p, _p, C.c_uint64, C.c_int, _p,
+                                         C.c_uint64, _p, _p, _p, _p]),
     "ps_distill_gave_up": (C.c_int, [C.POINTER(C.c_uint32)]),
     "ps_block_matmul_gave_up": (C.c_int, [C.POINTER(C.c_uint32)]),
 }

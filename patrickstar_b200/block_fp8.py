@@ -201,14 +201,23 @@ def block_quantize(x, blocks="row", fmt="e4m3"):
     return _quantize(x.detach(), blocks, fmt)
 
 
+def _rows(m, n, dtype, device):
+    """An uninitialised [m, n] tensor whose rows start on 16-byte boundaries: the product then leaves the SM in whole
+    boxes.  Rows of other sizes are a view of longer ones."""
+    per = 16 // dtype.itemsize
+    ld = -(-n // per) * per
+    out = torch.empty((m, ld), dtype=dtype, device=device)
+    return out if ld == n else out[:, :n]
+
+
 def _matmul(a, a_dim, b, b_dim, bias, out_dtype):
     m, n, k = a.shape[1 - a_dim], b.shape[1 - b_dim], a.shape[a_dim]
-    out = torch.empty((m, n), dtype=out_dtype, device=a.device)
+    out = _rows(m, n, out_dtype, a.device)
     with _on(a.device):
         check(lib.ps_block_matmul(
             C.byref(a._operand(a_dim)), C.byref(b._operand(b_dim)), m, n, k,
             bias.data_ptr() if bias is not None else None, _DTYPES[bias.dtype] if bias is not None else 0,
-            out.data_ptr(), _DTYPES[out_dtype], n, _stream_ptr(a.device)), "ps_block_matmul")
+            out.data_ptr(), _DTYPES[out_dtype], max(n, out.stride(0)), _stream_ptr(a.device)), "ps_block_matmul")
     return out
 
 
@@ -231,6 +240,8 @@ def block_matmul(a, b, a_dim=None, b_dim=None, bias=None, out_dtype=torch.float1
 
     Returns ``[outer size of a, outer size of b]`` in ``out_dtype`` (float16, bfloat16 or float32),
     accumulated in 32 bits and rounded once, after ``bias`` (one value for each column) was added.
+    Rows of the result start on 16-byte boundaries: where a row is not a multiple of 16 bytes it is a
+    view of longer rows, not contiguous.
     """
     a_dim, b_dim = _dim(a, a_dim, "a"), _dim(b, b_dim, "b")
     if a.device != b.device:
@@ -289,13 +300,14 @@ def _linear_forward(x, weight, bias, kept, keep):
         bias = bias.contiguous()
     dev = x.device
     saved_bytes, scratch_bytes, _ = _layer_bytes(tokens, k, n, kept is not None, keep)
-    y = torch.empty((tokens, n), dtype=x.dtype, device=dev)
+    y = _rows(tokens, n, x.dtype, dev)
     saved = torch.empty(saved_bytes, dtype=torch.uint8, device=dev) if saved_bytes else None
     scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=dev)
     layer = _layer(x, weight, bias, kept, tokens, k, n)
     with _on(dev):
-        check(lib.ps_fp8_linear_forward(C.byref(layer), keep, y.data_ptr(), None if saved is None else saved.data_ptr(),
-                                        scratch.data_ptr(), _stream_ptr(dev)), "ps_fp8_linear_forward")
+        check(lib.ps_fp8_linear_forward(C.byref(layer), keep, y.data_ptr(), max(n, y.stride(0)),
+                                        None if saved is None else saved.data_ptr(), scratch.data_ptr(),
+                                        _stream_ptr(dev)), "ps_fp8_linear_forward")
     return y, saved, layer
 
 
@@ -335,7 +347,7 @@ class _Fp8Linear(torch.autograd.Function):
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dy = _adjacent(dy)
         tokens, k, n = layer.tokens, layer.k, layer.n
-        dx = torch.empty((tokens, k), dtype=ctx.x_dtype, device=dev) if need_x else None
+        dx = _rows(tokens, k, ctx.x_dtype, dev) if need_x else None
         dw = torch.empty((n, k), dtype=ctx.w_dtype, device=dev) if need_w else None
         db = torch.empty(n, dtype=ctx.b_dtype, device=dev) if need_b else None
         scratch = torch.empty(_layer_bytes(tokens, k, n, bool(layer.kept_data), ctx.keep)[2], dtype=torch.uint8, device=dev)
@@ -343,7 +355,7 @@ class _Fp8Linear(torch.autograd.Function):
             check(lib.ps_fp8_linear_backward(
                 C.byref(layer), ctx.keep, None if saved is None else saved.data_ptr(), dy.data_ptr(),
                 dy.stride(0) if tokens > 1 else n, _FORMATS[ctx.grad_fmt][1], dx.data_ptr() if need_x else None,
-                dw.data_ptr() if need_w else None, db.data_ptr() if need_b else None, scratch.data_ptr(),
+                max(k, dx.stride(0)) if need_x else k, dw.data_ptr() if need_w else None, db.data_ptr() if need_b else None, scratch.data_ptr(),
                 _stream_ptr(dev)), "ps_fp8_linear_backward")
         return dx, dw, db, None, None
 
@@ -354,7 +366,9 @@ def fp8_linear(x, weight, bias=None, grad_fmt="e4m3"):
     ``x`` and ``weight`` are quantized to e4m3 within the call (1 x 128 and 128 x 128 blocks),
     the incoming gradient in the backward pass to ``grad_fmt`` (1 x 128 and 128 x 1 blocks).
     The result and the gradient of ``x`` have the type of ``x``, the gradients of ``weight`` and
-    ``bias`` theirs; the gradient of ``bias`` is summed from the unquantized gradient.  ``weight``
+    ``bias`` theirs; the gradient of ``bias`` is summed from the unquantized gradient.  Rows of the
+    result and of the gradient of ``x`` start on 16-byte boundaries: where N (or K) is not a multiple of
+    16 bytes they are views of longer rows, not contiguous.  ``weight``
     may also be a ``BlockQuantized`` with "tile" blocks, quantized once and kept; it has no
     gradient then.  Between forward and backward the quantized ``x`` and ``weight`` are kept (one
     byte an element), not the originals.

@@ -13,7 +13,8 @@ SOURCES = [os.path.join(HERE, "csrc", name) for name in (
     "ps_kernels.cu", "ps_offload.cu", "ps_block_quantize.cu", "ps_block_matmul.cu", "ps_fp8_linear.cu",
     "ps_distill.cu")]
 HEADERS = [os.path.join(ROOT, "include", "ps_b200.h"), os.path.join(HERE, "csrc", "ps_internal.h"),
-           os.path.join(HERE, "csrc", "ps_tensor_core.cuh"), os.path.join(HERE, "csrc", "ps_pair.cuh")]
+           os.path.join(HERE, "csrc", "ps_tensor_core.cuh"), os.path.join(HERE, "csrc", "ps_pair.cuh"),
+           os.path.join(HERE, "csrc", "ps_launch.cuh")]
 OUT = os.path.join(HERE, "libps_b200.so")
 
 NVCC_FLAGS = [

@@ -18,6 +18,7 @@
 #include "ps_b200.h"
 
 #include "ps_internal.h"
+#include "ps_launch.cuh"
 #include "ps_tensor_core.cuh"
 
 #include <cuda_bf16.h>
@@ -146,6 +147,7 @@ block_matmul_split_kernel(const __grid_constant__ CUtensorMap map_a, const __gri
     __syncthreads();
     tc::fence_after();
     const uint32_t tmem = tmem_base;
+    cudaTriggerProgrammaticLaunchCompletion();
     cudaGridDependencySynchronize();  // up to here nothing that another kernel writes was touched
 
     if (warp == 4 && tc::elect_one()) {
@@ -410,6 +412,7 @@ block_matmul_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     tc::cluster_sync();
     tc::fence_after();
     const uint32_t tmem = tmem_base;
+    cudaTriggerProgrammaticLaunchCompletion();
     cudaGridDependencySynchronize();  // up to here nothing that another kernel writes was touched
 
     if (warp == 4 && tc::elect_one()) {
@@ -595,10 +598,26 @@ int encode_operand(const ps_block_operand* o, uint64_t outer, uint64_t k, uint32
 
 uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 
-// 256 x 256 tiles where they fill the pairs of SMs.
+// CTAs that share a tile of 128 x 128 along k: as many as fill the SMs, with four k blocks each at least.
+uint32_t splits_of(uint64_t tiles, uint32_t n_kb, int sms)
+{
+    uint32_t splits = 1;
+    while (splits < 8 && tiles * splits < (uint64_t)sms && splits * 4 <= n_kb) splits *= 2;
+    return splits;
+}
+
+// 256 x 256 tiles on pairs of SMs, or 128 x 128 tiles on single ones, whichever should be done first: in both a k block
+// takes an SM some 520 cycles, the small tile's for what it reads (32 KB at 64 bytes a cycle), the large one's for its
+// products, so only what the rounds leave idle counts; the large tiles' set-up is that of a few k blocks.
+// (1600 x 1600 x 16385: 49 large tiles 40 us, 169 small ones 72 us; 1 x 6400 x 1600: 25 large 17 us, 100 small 12 us.)
 bool use_pairs(uint32_t m, uint32_t n, uint32_t n_kb, int sms)
 {
-    return n_kb > 0 && (uint64_t)ceil_div(m, kPairTile) * ceil_div(n, kPairTile) >= (uint64_t)sms / 2;
+    if (n_kb == 0) return false;
+    const uint64_t large = (uint64_t)ceil_div(m, kPairTile) * ceil_div(n, kPairTile), pairs = (uint64_t)sms / 2;
+    const uint64_t small = (uint64_t)ceil_div(m, kTile) * ceil_div(n, kTile), splits = splits_of(small, n_kb, sms);
+    const uint64_t as_pairs = (large + pairs - 1) / pairs * n_kb + 4;
+    const uint64_t as_split = (small * splits + sms - 1) / sms * ((n_kb + splits - 1) / splits);
+    return as_pairs <= as_split;
 }
 
 // Lets a kernel have that much shared memory; `seen`: the devices on which that is done.
@@ -619,35 +638,13 @@ int allow_smem(F kernel, uint32_t bytes, std::atomic<uint64_t>& seen)
     return PS_ERR_CUDA;
 }
 
-// The kernel's set-up may run while the kernel before it in the stream finishes (the quantizer lets it).
-template <typename K, typename... Args>
-void launch_in_clusters(K kernel, uint32_t grid, uint32_t threads, uint32_t smem, uint32_t cluster, cudaStream_t st,
-                        const Args&... args)
-{
-    cudaLaunchConfig_t cfg;
-    memset(&cfg, 0, sizeof(cfg));
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute at[2];
-    memset(at, 0, sizeof(at));
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = cluster, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
-    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 2;
-    cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 template <int kOut>
 int launch_pairs_as(const ProductArgs& p, const CUtensorMap* maps, const CUtensorMap& out, uint32_t grid, cudaStream_t st)
 {
     static std::atomic<uint64_t> seen{0};
     const int rc = allow_smem(block_matmul_pair_kernel<kOut>, kPairSmem, seen);
     if (rc != PS_OK) return rc;
-    launch_in_clusters(block_matmul_pair_kernel<kOut>, grid, kPairThreads, kPairSmem, 2, st, maps[0], maps[1], maps[2],
+    launch_behind(block_matmul_pair_kernel<kOut>, grid, kPairThreads, kPairSmem, 2, st, maps[0], maps[1], maps[2],
                        maps[3], out, p);
     return ps_internal::after_launch();
 }
@@ -682,13 +679,12 @@ int launch_split(ProductArgs& p, const CUtensorMap* maps, const ps_block_operand
     p.tiles_m = ceil_div(p.m, kTile), p.tiles_n = ceil_div(p.n, kTile);
     if (p.n_kb > 0) p.idesc = tc::mx_idesc(128, 128, a->fmt, b->fmt, !a->k_dim, !b->k_dim);
     const uint64_t tiles = (uint64_t)p.tiles_m * p.tiles_n;
-    uint32_t splits = 1;
-    while (splits < 8 && tiles * splits < (uint64_t)sms && splits * 4 <= p.n_kb) splits *= 2;
+    const uint32_t splits = splits_of(tiles, p.n_kb, sms);
     if (tiles * splits > 0x7fffffffull) return PS_ERR_LIMIT;
     static std::atomic<uint64_t> seen{0};
     const int rc = allow_smem(block_matmul_split_kernel, kSplitSmem, seen);
     if (rc != PS_OK) return rc;
-    launch_in_clusters(block_matmul_split_kernel, (uint32_t)(tiles * splits), kSplitThreads, kSplitSmem, splits, st, maps[0],
+    launch_behind(block_matmul_split_kernel, (uint32_t)(tiles * splits), kSplitThreads, kSplitSmem, splits, st, maps[0],
                        maps[1], maps[2], maps[3], p, splits);
     return ps_internal::after_launch();
 }

@@ -19,6 +19,7 @@
 #include "ps_b200.h"
 
 #include "ps_internal.h"
+#include "ps_launch.cuh"
 #include "ps_pair.cuh"
 
 #include <cuda_bf16.h>
@@ -374,6 +375,7 @@ __global__ void __launch_bounds__(kThreads, ctas_of<T>()) block_quantize_kernel(
 {
     __shared__ Shared sh;
     cudaTriggerProgrammaticLaunchCompletion();
+    cudaGridDependencySynchronize();
     quantize_tile<T, kMode, kFmt, kSum>(a, blockIdx.x, sh);
 }
 
@@ -383,6 +385,7 @@ __global__ void __launch_bounds__(kThreads, ctas_of<T>()) quantize_layer_kernel(
 {
     __shared__ Shared sh;
     cudaTriggerProgrammaticLaunchCompletion();
+    cudaGridDependencySynchronize();
     if (blockIdx.x < split)
         quantize_tile<T, kMode, PS_FP8_E4M3, false>(x, blockIdx.x, sh);
     else
@@ -394,8 +397,10 @@ template <typename T>
 __global__ void column_sum_kernel(const float* partial, uint32_t blocks, uint32_t cols, T* out)
 {
     const uint32_t c = blockIdx.x * blockDim.x + threadIdx.x;
+    cudaGridDependencySynchronize();
     if (c >= cols) return;
     double t = 0.0;
+#pragma unroll 8
     for (uint32_t b = 0; b < blocks; ++b) t += (double)partial[(size_t)b * cols + c];
     out[c] = (T)(float)t;
 }
@@ -404,15 +409,15 @@ template <typename T, int kFmt>
 void launch(int mode, const QuantArgs& a, uint32_t tiles, cudaStream_t st)
 {
     if (mode == PS_BLOCKS_ROW)
-        block_quantize_kernel<T, PS_BLOCKS_ROW, kFmt, false><<<tiles, kThreads, 0, st>>>(a);
+        launch_behind(block_quantize_kernel<T, PS_BLOCKS_ROW, kFmt, false>, tiles, kThreads, 0, 0, st, a);
     else if (mode == PS_BLOCKS_COL)
-        block_quantize_kernel<T, PS_BLOCKS_COL, kFmt, false><<<tiles, kThreads, 0, st>>>(a);
+        launch_behind(block_quantize_kernel<T, PS_BLOCKS_COL, kFmt, false>, tiles, kThreads, 0, 0, st, a);
     else if (mode == PS_BLOCKS_TILE)
-        block_quantize_kernel<T, PS_BLOCKS_TILE, kFmt, false><<<tiles, kThreads, 0, st>>>(a);
+        launch_behind(block_quantize_kernel<T, PS_BLOCKS_TILE, kFmt, false>, tiles, kThreads, 0, 0, st, a);
     else if (a.colsum == nullptr)
-        block_quantize_kernel<T, PS_BLOCKS_ROW_COL, kFmt, false><<<tiles, kThreads, 0, st>>>(a);
+        launch_behind(block_quantize_kernel<T, PS_BLOCKS_ROW_COL, kFmt, false>, tiles, kThreads, 0, 0, st, a);
     else
-        block_quantize_kernel<T, PS_BLOCKS_ROW_COL, kFmt, true><<<tiles, kThreads, 0, st>>>(a);
+        launch_behind(block_quantize_kernel<T, PS_BLOCKS_ROW_COL, kFmt, true>, tiles, kThreads, 0, 0, st, a);
 }
 
 template <typename T>
@@ -457,9 +462,9 @@ template <typename T>
 void launch_layer(int mode, const QuantArgs& x, uint32_t x_tiles, const QuantArgs& w, uint32_t w_tiles, cudaStream_t st)
 {
     if (mode == PS_BLOCKS_ROW)
-        quantize_layer_kernel<T, PS_BLOCKS_ROW><<<x_tiles + w_tiles, kThreads, 0, st>>>(x, w, x_tiles);
+        launch_behind(quantize_layer_kernel<T, PS_BLOCKS_ROW>, x_tiles + w_tiles, kThreads, 0, 0, st, x, w, x_tiles);
     else
-        quantize_layer_kernel<T, PS_BLOCKS_ROW_COL><<<x_tiles + w_tiles, kThreads, 0, st>>>(x, w, x_tiles);
+        launch_behind(quantize_layer_kernel<T, PS_BLOCKS_ROW_COL>, x_tiles + w_tiles, kThreads, 0, 0, st, x, w, x_tiles);
 }
 
 }  // namespace
@@ -521,11 +526,11 @@ int ps_column_sum(const float* partial_dev, uint32_t blocks, uint32_t cols, void
     const uint32_t grid = (uint32_t)(((uint64_t)cols + 127) / 128);
     cudaStream_t st = (cudaStream_t)stream;
     if (dtype == PS_DTYPE_F16)
-        column_sum_kernel<<<grid, 128, 0, st>>>(partial_dev, blocks, cols, (__half*)out_dev);
+        launch_behind(column_sum_kernel<__half>, grid, 128, 0, 0, st, partial_dev, blocks, cols, (__half*)out_dev);
     else if (dtype == PS_DTYPE_BF16)
-        column_sum_kernel<<<grid, 128, 0, st>>>(partial_dev, blocks, cols, (__nv_bfloat16*)out_dev);
+        launch_behind(column_sum_kernel<__nv_bfloat16>, grid, 128, 0, 0, st, partial_dev, blocks, cols, (__nv_bfloat16*)out_dev);
     else
-        column_sum_kernel<<<grid, 128, 0, st>>>(partial_dev, blocks, cols, (float*)out_dev);
+        launch_behind(column_sum_kernel<float>, grid, 128, 0, 0, st, partial_dev, blocks, cols, (float*)out_dev);
     return ps_internal::after_launch();
 }
 

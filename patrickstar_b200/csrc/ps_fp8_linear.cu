@@ -88,7 +88,8 @@ int ps_fp8_linear_sizes(const ps_fp8_linear* q, int keep, uint64_t* sizes)
     return PS_OK;
 }
 
-int ps_fp8_linear_forward(const ps_fp8_linear* q, int keep, void* y_dev, void* saved_dev, void* scratch_dev, void* stream)
+int ps_fp8_linear_forward(const ps_fp8_linear* q, int keep, void* y_dev, uint64_t ld_y, void* saved_dev,
+                          void* scratch_dev, void* stream)
 {
     int rc = check_layer(q);
     if (rc != PS_OK) return rc;
@@ -116,11 +117,12 @@ int ps_fp8_linear_forward(const ps_fp8_linear* q, int keep, void* y_dev, void* s
         b = {w, tmp.ws1, row_bytes(q->k), PS_FP8_E4M3, 1};
     }
     if (rc != PS_OK) return rc;
-    return ps_block_matmul(&a, &b, q->tokens, q->n, q->k, q->bias, q->bias_dtype, y_dev, q->x_dtype, q->n, stream);
+    return ps_block_matmul(&a, &b, q->tokens, q->n, q->k, q->bias, q->bias_dtype, y_dev, q->x_dtype, ld_y, stream);
 }
 
 int ps_fp8_linear_backward(const ps_fp8_linear* q, int keep, const void* saved_dev, const void* dy_dev, uint64_t ld_dy,
-                           int grad_fmt, void* dx_dev, void* dw_dev, void* db_dev, void* scratch_dev, void* stream)
+                           int grad_fmt, void* dx_dev, uint64_t ld_dx, void* dw_dev, void* db_dev, void* scratch_dev,
+                           void* stream)
 {
     int rc = check_layer(q);
     if (rc != PS_OK) return rc;
@@ -143,7 +145,7 @@ int ps_fp8_linear_backward(const ps_fp8_linear* q, int keep, const void* saved_d
         const ps_block_operand b = q->kept_data != nullptr
                                        ? ps_block_operand{q->kept_data, q->kept_scales0, q->ld_kept, q->kept_fmt, 0}
                                        : ps_block_operand{kept.w, kept.ws0, row_bytes(q->k), PS_FP8_E4M3, 0};
-        rc = ps_block_matmul(&a, &b, q->tokens, q->k, q->n, nullptr, 0, dx_dev, q->x_dtype, q->k, stream);
+        rc = ps_block_matmul(&a, &b, q->tokens, q->k, q->n, nullptr, 0, dx_dev, q->x_dtype, ld_dx, stream);
     }
     if (rc == PS_OK && dw_dev != nullptr) {
         const ps_block_operand a = {tmp.g0, tmp.s0, row_bytes(q->n), grad_fmt, 0};
