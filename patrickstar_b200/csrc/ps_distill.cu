@@ -22,6 +22,7 @@
 #include "ps_b200.h"
 
 #include "ps_internal.h"
+#include "ps_launch.cuh"
 #include "ps_pair.cuh"
 #include "ps_tensor_core.cuh"
 
@@ -33,7 +34,8 @@
 
 namespace {
 
-constexpr int kMaxThreads = 320;
+constexpr int kMaxThreads = 320;   // 256 of the pass
+constexpr int kLongThreads = 576;  // 512 of the pass, for the longest rows
 constexpr uint32_t kMaxSlots = 4;
 constexpr int kCtas = 3;  // of the largest kind on an SM: 64 registers a thread
 constexpr uint64_t kRowsInL2 = 64ull << 20;  // bytes of rows in work, of 126 MB
@@ -53,6 +55,7 @@ struct DistillArgs {
     int idx_bytes, teacher_dtype;
     float temperature, weight;
     float* row_loss;
+    float* loss;         // of a single row (else NULL: the rows are summed by a launch of their own)
     float4* stats;       // per row: M, factors of e_v in the gradient for v in S and for the others, -
     const float* inv_n;  // 1 / rows that the mask keeps, or NULL: then inv_n_value
     float inv_n_value;
@@ -420,7 +423,11 @@ __device__ void entries_after(const DistillArgs& a, const Layout& lay, uint32_t 
         t = warp_sum(t);
         if (kBucket && !(slot.rest <= 0.0)) t += slot.rest * (log(slot.rest) - (log((double)slot.out) - log_z));
         if (slot.bad) t = (double)NAN;
-        if (lane == 0) a.row_loss[row] = (float)(t * (double)a.weight * (double)a.temperature * (double)a.temperature);
+        if (lane == 0) {
+            const float f = (float)(t * (double)a.weight * (double)a.temperature * (double)a.temperature);
+            a.row_loss[row] = f;
+            if (a.loss != nullptr) *a.loss = f;  // a mean over one row, too
+        }
     }
     if (kWhat & kGrad) {
         T* const g = reinterpret_cast<T*>(a.grad) + (uint64_t)row * a.ldg;
@@ -455,13 +462,14 @@ __device__ void entries_after(const DistillArgs& a, const Layout& lay, uint32_t 
 // gradient the same ones again behind them).  One warp works on the listed entries of the row before and of
 // the row after meanwhile, so that their chains of 64-bit logarithms and scattered loads hide behind the
 // pass.  The other warps pass over the chunks.
-template <typename T, bool kBucket, int kWhat>
-__global__ void __launch_bounds__(kMaxThreads, kCtas) distill_kernel(const DistillArgs a, const Layout lay)
+template <typename T, bool kBucket, int kWhat, bool kLong>
+__global__ void __launch_bounds__(kLong ? kLongThreads : kMaxThreads, kLong ? 2 : kCtas)
+distill_kernel(const DistillArgs a, const Layout lay)
 {
     constexpr int E = Type<T>::kVec;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ RowSlot slots[2];
-    __shared__ float s_m[kMaxThreads / 32], s_out[kMaxThreads / 32], s_in[kMaxThreads / 32];
+    __shared__ float s_m[kLongThreads / 32], s_out[kLongThreads / 32], s_in[kLongThreads / 32];
     __shared__ uint64_t full[kMaxSlots], empty[kMaxSlots];
     __shared__ volatile int gave_up;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -482,6 +490,8 @@ __global__ void __launch_bounds__(kMaxThreads, kCtas) distill_kernel(const Disti
         }
     }
 
+    cudaTriggerProgrammaticLaunchCompletion();
+    cudaGridDependencySynchronize();
     if ((kWhat & kLoss) == 0 && a.used_scale != nullptr && *a.used_scale == *a.grad_out)
         return;  // the forward pass wrote this gradient
     float scale = 1.f;
@@ -556,8 +566,10 @@ __global__ void __launch_bounds__(kMaxThreads, kCtas) distill_kernel(const Disti
             const T* const z = reinterpret_cast<const T*>(a.z) + (uint64_t)row * a.ldz;
             T* const g = reinterpret_cast<T*>(a.grad) + (uint64_t)row * a.ldg;
             if (!slot.keep) {
-                if ((kWhat & kLoss) && threadIdx.x == 0)
+                if ((kWhat & kLoss) && threadIdx.x == 0) {
                     a.row_loss[row] = 0.f, a.stats[row] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (a.loss != nullptr) *a.loss = 0.f;
+                }
                 if (kWhat & kGrad) {
                     const RowShape gs = row_shape(g, a.vocab);
                     uint4* gv = reinterpret_cast<uint4*>(g + gs.head);
@@ -751,6 +763,7 @@ __global__ void __launch_bounds__(kMaxThreads, kCtas) distill_kernel(const Disti
 __global__ void distill_count_kernel(const uint8_t* mask, uint32_t rows, float* inv_n)
 {
     __shared__ uint32_t s[32];
+    cudaGridDependencySynchronize();
     uint32_t n = 0;
     for (uint32_t i = threadIdx.x; i < rows; i += blockDim.x) n += mask[i] != 0;
     n = __reduce_add_sync(0xffffffffu, n);
@@ -766,6 +779,7 @@ __global__ void distill_count_kernel(const uint8_t* mask, uint32_t rows, float* 
 __global__ void distill_sum_kernel(const float* row_loss, uint32_t rows, const float* inv_n, float inv_n_value, float* loss)
 {
     __shared__ double s[32];
+    cudaGridDependencySynchronize();
     double t = 0.0;
     for (uint32_t i = threadIdx.x; i < rows; i += blockDim.x) t += (double)row_loss[i];
     t = warp_sum(t);
@@ -777,25 +791,11 @@ __global__ void distill_sum_kernel(const float* row_loss, uint32_t rows, const f
     }
 }
 
-template <typename T, bool kBucket, int kWhat>
-int launch(const DistillArgs& a, cudaStream_t st)
+template <typename T, bool kBucket, int kWhat, bool kLong>
+int launch(const DistillArgs& a, const Layout& lay, size_t smem, uint32_t grid, cudaStream_t st)
 {
-    const int sms = ps_internal::sm_count();
-    if (sms < 0) return sms;
-    // Threads and chunks for a row by its size: four vectors a thread and chunk, four chunks.  Small CTAs, since each
-    // brings a warp for listed entries and rows' own latencies overlap (8192 x 50257 fp16, loss: 158 us with 128
-    // threads, 167 us with 256); for the longest rows, of which L2 holds two an SM, more threads.
-    const uint64_t bytes = (uint64_t)a.vocab * sizeof(T);
-    Layout lay;
-    lay.shift = bytes <= 16 * 1024 ? 6 : bytes <= 160 * 1024 ? 7 : 8;
-    lay.threads = 1u << lay.shift;
-    lay.chunk_vecs = kUnroll * lay.threads;
-    lay.slots = kMaxSlots;
-    const bool bits = kBucket && (kWhat & kLoss);
-    while (lay.slots > 2 && smem_bytes(lay, a.k, a.vocab, bits) > 200 * 1024) --lay.slots;
-    const size_t smem = smem_bytes(lay, a.k, a.vocab, bits);
     if (smem > 40 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(distill_kernel<T, kBucket, kWhat>,
+        const cudaError_t e = cudaFuncSetAttribute(distill_kernel<T, kBucket, kWhat, kLong>,
                                                    cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) {
             ps_internal::set_cuda_error((int)e);
@@ -803,17 +803,44 @@ int launch(const DistillArgs& a, cudaStream_t st)
             return PS_ERR_CUDA;
         }
     }
+    launch_behind(distill_kernel<T, kBucket, kWhat, kLong>, grid, lay.threads + 64, (uint32_t)smem, 0, st, a, lay);
+    return ps_internal::after_launch();
+}
+
+template <typename T, bool kBucket, int kWhat>
+int launch(const DistillArgs& a, cudaStream_t st)
+{
+    const int sms = ps_internal::sm_count();
+    if (sms < 0) return sms;
+    // Threads for a row by its size: four vectors a thread and chunk, four chunks.  Small CTAs, since each brings a
+    // warp for listed entries and rows' own latencies overlap (8192 x 50257 fp16, loss: 158 us with 128 threads,
+    // 167 us with 256).  More threads for the longest rows, of which L2 keeps two an SM for the second pass, and where
+    // there is no more than one row for an SM.
+    const uint64_t bytes = (uint64_t)a.vocab * sizeof(T);
+    const bool few = a.rows <= (uint32_t)sms;
+    Layout lay;
+    lay.shift = bytes <= 16 * 1024 ? 6 : bytes <= 160 * 1024 && !few ? 7 : 8;
+    const bool is_long = lay.shift == 8 && (bytes > 160 * 1024 || few) && bytes > 32 * 1024;
+    if (is_long) lay.shift = 9;
+    lay.threads = 1u << lay.shift;
+    lay.chunk_vecs = kUnroll * lay.threads;
+    lay.slots = kMaxSlots;
+    const bool bits = kBucket && (kWhat & kLoss);
+    const size_t limit = (is_long ? 108 : 200) * 1024;  // two CTAs an SM, or what the longest bitmaps leave
+    while (lay.slots > 2 && smem_bytes(lay, a.k, a.vocab, bits) > limit) --lay.slots;
+    const size_t smem = smem_bytes(lay, a.k, a.vocab, bits);
     // As many rows in work as SMs hold, but for the gradient no more than L2 keeps until the second pass.
     uint64_t most = 227 * 1024 / (smem + 2048);
-    const uint64_t by_threads = (uint64_t)kMaxThreads * kCtas / (lay.threads + 64);
+    const uint64_t by_threads = is_long ? 2 : (uint64_t)kMaxThreads * kCtas / (lay.threads + 64);
     most = most < 1 ? 1 : most < by_threads ? most : by_threads;
     if ((kWhat & kLoss) && (kWhat & kGrad)) {
         const uint64_t fit = kRowsInL2 / ((uint64_t)sms * bytes);
         most = fit >= most ? most : fit < 2 ? (most < 2 ? most : 2) : fit;
     }
     most *= (uint64_t)sms;
-    distill_kernel<T, kBucket, kWhat><<<a.rows < most ? a.rows : (uint32_t)most, lay.threads + 64, smem, st>>>(a, lay);
-    return ps_internal::after_launch();
+    const uint32_t grid = a.rows < most ? a.rows : (uint32_t)most;
+    return is_long ? launch<T, kBucket, kWhat, true>(a, lay, smem, grid, st)
+                   : launch<T, kBucket, kWhat, false>(a, lay, smem, grid, st);
 }
 template <typename T>
 int launch(const DistillArgs& a, bool bucket, int what, cudaStream_t st)
@@ -889,18 +916,20 @@ int ps_distill_forward(const ps_distill_problem* q, float* loss_dev, float* row_
     DistillArgs a = arguments(q, inv_n_dev);
     a.row_loss = row_loss_dev, a.stats = (float4*)stats_dev;
     a.grad = grad_dev, a.ldg = ld_grad, a.scaler = scaler_dev, a.used_scale = used_scale_dev;
+    a.loss = reduce && q->rows == 1 ? loss_dev : nullptr;
     if (q->rows > 0) {
         if (a.inv_n != nullptr) {
-            distill_count_kernel<<<1, 1024, 0, st>>>(a.mask, q->rows, inv_n_dev);
+            launch_behind(distill_count_kernel, 1, 1024, 0, 0, st, a.mask, q->rows, inv_n_dev);
             rc = ps_internal::after_launch();
             if (rc != PS_OK) return rc;
         }
         rc = launch(a, q->dtype, q->tail == PS_TAIL_BUCKET, grad ? kLoss | kGrad : kLoss, st);
         if (rc != PS_OK) return rc;
     }
-    if (!reduce) return PS_OK;
+    if (!reduce || a.loss != nullptr) return PS_OK;
     // no rows: a loss of 0
-    distill_sum_kernel<<<1, 1024, 0, st>>>(row_loss_dev, q->rows, q->rows > 0 ? a.inv_n : nullptr, a.inv_n_value, loss_dev);
+    launch_behind(distill_sum_kernel, 1, 1024, 0, 0, st, (const float*)row_loss_dev, q->rows,
+                  q->rows > 0 ? a.inv_n : (const float*)nullptr, a.inv_n_value, loss_dev);
     return ps_internal::after_launch();
 }
 
