@@ -41,5 +41,6 @@ def __getattr__(name):
         import importlib
         mod, attr = _LAZY[name]
         m = importlib.import_module("." + mod, __name__)
-        return m if attr is None else getattr(m, attr)
+        globals()[name] = m if attr is None else getattr(m, attr)   # looked up once
+        return globals()[name]
     raise AttributeError("module %r has no attribute %r" % (__name__, name))

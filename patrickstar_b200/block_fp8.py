@@ -14,7 +14,6 @@ tensor core applies them.  An element that is not finite stays visible (NaN in
 e4m3, itself in e5m2), so a gradient that overflowed still reaches the overflow
 test of the step.  No counterpart in the reference.
 """
-import contextlib
 import ctypes as C
 import functools
 import math
@@ -24,6 +23,7 @@ import torch
 from ._lib import (PS_BLOCKS_COL, PS_BLOCKS_ROW, PS_BLOCKS_ROW_COL, PS_BLOCKS_TILE, PS_DTYPE_BF16, PS_DTYPE_F16,
                    PS_DTYPE_F32, PS_FP8_E4M3, PS_FP8_E5M2, PS_KEEP_INPUT, PS_KEEP_WEIGHT, BlockOperand, Fp8LinearLayer,
                    check, lib)
+from .streams import current_device, raw_stream
 
 BLOCK = 128
 
@@ -33,20 +33,21 @@ _FORMAT_OF = {dtype: code for dtype, code in _FORMATS.values()}
 _BLOCKS = {"row": PS_BLOCKS_ROW, "col": PS_BLOCKS_COL, "row+col": PS_BLOCKS_ROW_COL, "tile": PS_BLOCKS_TILE}
 
 
-def _stream_ptr(device):
-    return torch._C._cuda_getCurrentRawStream(device.index)   # current_stream(device).cuda_stream, without the object
-
-
-_NO_SWITCH = contextlib.nullcontext()
-
-
-def _on(device):
-    """``torch.cuda.device(device)`` where that is not the current one already."""
-    return _NO_SWITCH if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-
 def _scales_shape(outer, contracted):
     return (-(-contracted // (4 * BLOCK)), -(-outer // BLOCK), 32, 4, 4)
+
+
+def _check_scales(name, scales, blocks, used, outer, contracted, data):
+    if (scales is not None) != used:
+        raise ValueError("%s blocks %s scales in %s" % (blocks, "need" if used else "have no", name))
+    if scales is None:
+        return
+    shape = _scales_shape(outer, contracted)
+    if scales.dtype != torch.uint8 or scales.shape != shape or not scales.is_contiguous():
+        raise ValueError("%s must be contiguous uint8 of shape %s; got %s of shape %s"
+                         % (name, shape, scales.dtype, tuple(scales.shape)))
+    if scales.device != data.device:
+        raise ValueError("values on %s, %s on %s" % (data.device, name, scales.device))
 
 
 class BlockQuantized:
@@ -79,18 +80,8 @@ class BlockQuantized:
                 raise ValueError("the values of a row must be adjacent")
             if data.data_ptr() % 16 or (rows > 1 and (data.stride(0) % 16 or data.stride(0) < cols)):
                 raise ValueError("rows of values must start on 16-byte boundaries")
-        for name, scales, used, shape in (("scales1", scales1, blocks != "col", _scales_shape(rows, cols)),
-                                          ("scales0", scales0, blocks != "row", _scales_shape(cols, rows))):
-            if (scales is not None) != used:
-                raise ValueError("%s %s scales %s %s" % (blocks, "blocks need" if used else "blocks have no",
-                                                         "in", name))
-            if scales is None:
-                continue
-            if scales.dtype != torch.uint8 or tuple(scales.shape) != shape or not scales.is_contiguous():
-                raise ValueError("%s must be contiguous uint8 of shape %s; got %s of shape %s"
-                                 % (name, shape, scales.dtype, tuple(scales.shape)))
-            if scales.device != data.device:
-                raise ValueError("values on %s, %s on %s" % (data.device, name, scales.device))
+        _check_scales("scales1", scales1, blocks, blocks != "col", rows, cols, data)
+        _check_scales("scales0", scales0, blocks, blocks != "row", cols, rows, data)
         self.data, self.blocks, self.scales1, self.scales0 = data, blocks, scales1, scales0
 
     @classmethod
@@ -166,12 +157,12 @@ def _quantize(x, blocks, fmt):
         q0 = torch.empty((rows, ldq), dtype=dtype, device=dev)
     if blocks != "row":
         s0 = torch.empty(_scales_shape(cols, rows), dtype=torch.uint8, device=dev)
-    with _on(dev):
+    with current_device(dev):
         check(lib.ps_block_quantize(
             x.data_ptr(), _DTYPES[x.dtype], x.stride(0) if rows > 1 else cols, rows, cols, _BLOCKS[blocks], code,
             q1.data_ptr() if q1 is not None else None, s1.data_ptr() if s1 is not None else None,
             q0.data_ptr() if q0 is not None else None, s0.data_ptr() if s0 is not None else None, ldq,
-            None, _stream_ptr(dev)), "ps_block_quantize")
+            None, raw_stream(dev)), "ps_block_quantize")
     if cols != ldq:
         q1 = q1 if q1 is None else q1[:, :cols]
         q0 = q0 if q0 is None else q0[:, :cols]
@@ -213,11 +204,11 @@ def _rows(m, n, dtype, device):
 def _matmul(a, a_dim, b, b_dim, bias, out_dtype):
     m, n, k = a.shape[1 - a_dim], b.shape[1 - b_dim], a.shape[a_dim]
     out = _rows(m, n, out_dtype, a.device)
-    with _on(a.device):
+    with current_device(a.device):
         check(lib.ps_block_matmul(
             C.byref(a._operand(a_dim)), C.byref(b._operand(b_dim)), m, n, k,
             bias.data_ptr() if bias is not None else None, _DTYPES[bias.dtype] if bias is not None else 0,
-            out.data_ptr(), _DTYPES[out_dtype], max(n, out.stride(0)), _stream_ptr(a.device)), "ps_block_matmul")
+            out.data_ptr(), _DTYPES[out_dtype], max(n, out.stride(0)), raw_stream(a.device)), "ps_block_matmul")
     return out
 
 
@@ -304,10 +295,10 @@ def _linear_forward(x, weight, bias, kept, keep):
     saved = torch.empty(saved_bytes, dtype=torch.uint8, device=dev) if saved_bytes else None
     scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=dev)
     layer = _layer(x, weight, bias, kept, tokens, k, n)
-    with _on(dev):
+    with current_device(dev):
         check(lib.ps_fp8_linear_forward(C.byref(layer), keep, y.data_ptr(), max(n, y.stride(0)),
                                         None if saved is None else saved.data_ptr(), scratch.data_ptr(),
-                                        _stream_ptr(dev)), "ps_fp8_linear_forward")
+                                        raw_stream(dev)), "ps_fp8_linear_forward")
     return y, saved, layer
 
 
@@ -351,12 +342,12 @@ class _Fp8Linear(torch.autograd.Function):
         dw = torch.empty((n, k), dtype=ctx.w_dtype, device=dev) if need_w else None
         db = torch.empty(n, dtype=ctx.b_dtype, device=dev) if need_b else None
         scratch = torch.empty(_layer_bytes(tokens, k, n, bool(layer.kept_data), ctx.keep)[2], dtype=torch.uint8, device=dev)
-        with _on(dev):
+        with current_device(dev):
             check(lib.ps_fp8_linear_backward(
                 C.byref(layer), ctx.keep, None if saved is None else saved.data_ptr(), dy.data_ptr(),
                 dy.stride(0) if tokens > 1 else n, _FORMATS[ctx.grad_fmt][1], dx.data_ptr() if need_x else None,
-                max(k, dx.stride(0)) if need_x else k, dw.data_ptr() if need_w else None, db.data_ptr() if need_b else None, scratch.data_ptr(),
-                _stream_ptr(dev)), "ps_fp8_linear_backward")
+                max(k, dx.stride(0)) if need_x else k, dw.data_ptr() if need_w else None,
+                db.data_ptr() if need_b else None, scratch.data_ptr(), raw_stream(dev)), "ps_fp8_linear_backward")
         return dx, dw, db, None, None
 
 

@@ -14,7 +14,8 @@ import torch
 
 from ._lib import (PS_DISTILL_MAX_K, PS_DISTILL_MAX_VOCAB, PS_REDUCE_MEAN, PS_REDUCE_NONE, PS_REDUCE_SUM,
                    PS_TAIL_BUCKET, PS_TAIL_DROP, DistillProblem, check, lib)
-from .block_fp8 import _DTYPES, _on, _stream_ptr
+from .block_fp8 import _DTYPES
+from .streams import current_device, raw_stream
 
 _TAILS = {"drop": PS_TAIL_DROP, "bucket": PS_TAIL_BUCKET}
 _REDUCTIONS = {"none": PS_REDUCE_NONE, "sum": PS_REDUCE_SUM, "mean": PS_REDUCE_MEAN}
@@ -49,11 +50,11 @@ def _forward(z, idx, teacher, mask, problem, scaler):
     grad = _like_rows(z) if scaler is not None and rows else None
     at, o = buf.data_ptr(), out.data_ptr()
     _point(problem, z, idx, teacher, mask)
-    with _on(dev):
+    with current_device(dev):
         check(lib.ps_distill_forward(
             C.byref(problem), o if reduce else None, at + 16 + 16 * rows if reduce else o, at + 16, at,
             scaler.state_ptr if grad is not None else None, grad.data_ptr() if grad is not None else None,
-            grad.stride(0) if grad is not None and rows > 1 else z.shape[1], at + 4, _stream_ptr(dev)),
+            grad.stride(0) if grad is not None and rows > 1 else z.shape[1], at + 4, raw_stream(dev)),
             "ps_distill_forward")
     return out, buf, grad
 
@@ -80,10 +81,10 @@ class _Distill(torch.autograd.Function):
         g = grad_out if grad_out.dtype == torch.float32 else grad_out.to(torch.float32)
         if g.dim() and g.stride(0) not in (0, 1):
             g = g.contiguous()
-        with _on(z.device):
+        with current_device(z.device):
             check(lib.ps_distill_backward(
                 C.byref(ctx.problem), at + 16, at, g.data_ptr(), g.stride(0) if g.dim() and rows > 1 else 0, used,
-                grad.data_ptr(), grad.stride(0) if rows > 1 else z.shape[1], _stream_ptr(z.device)),
+                grad.data_ptr(), grad.stride(0) if rows > 1 else z.shape[1], raw_stream(z.device)),
                 "ps_distill_backward")
         return grad, None, None, None, None, None
 

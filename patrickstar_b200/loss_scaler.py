@@ -13,6 +13,7 @@ import ctypes as C
 import torch
 
 from ._lib import ScalerState, check, lib
+from .streams import current_device, raw_stream
 
 
 def _stream_ptr(device):
@@ -93,9 +94,9 @@ class _DeviceScaler:
     def _scale_on_device(self, x):
         x = x.contiguous()
         out = torch.empty_like(x)
-        with torch.cuda.device(self.device):
+        with current_device(x.device):
             check(lib.ps_scale_loss(x.data_ptr(), out.data_ptr(), x.numel(), self._state.data_ptr(),
-                                    _stream_ptr(self.device)), "ps_scale_loss")
+                                    raw_stream(x.device)), "ps_scale_loss")
         return out
 
     def scale_loss(self, loss):
