@@ -67,6 +67,7 @@ struct DistillArgs {
     uint32_t grad_out_stride;
 };
 
+__device__ __forceinline__ void prefetch(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 __device__ __forceinline__ float ex2(float x)
 {
     float y;
@@ -282,7 +283,9 @@ struct Listed {
     float* z;           // logits
     uint32_t* bits;     // of every element: is it listed?
     uint32_t* owners;   // of every thread and chunk: has it a listed element?
+    uint32_t* seen;     // bits of indices seen, without the bitmap: zeros but while entries are looked at
 };
+constexpr uint32_t kSeenWords = 1024;
 // Threads and shared memory of a CTA: chunks of kUnroll vectors a thread, a ring of them, barriers, listed entries,
 // bitmaps.
 struct Layout {
@@ -290,16 +293,15 @@ struct Layout {
     uint32_t shift;
 };
 __host__ __device__ __forceinline__ uint32_t bitmap_words(uint32_t vocab) { return (vocab + 63) / 64 * 2; }
-__host__ __device__ __forceinline__ uint32_t round4(uint32_t k) { return (k + 3) & ~3u; }
 // a vector has four elements at least
 __host__ __device__ __forceinline__ uint32_t owner_words(const Layout& l, uint32_t vocab)
 {
     return ((vocab / 4 + l.chunk_vecs - 1) / l.chunk_vecs * (l.threads / 32) + 1) / 2 * 2;
 }
-__host__ __device__ __forceinline__ size_t smem_bytes(const Layout& l, uint32_t k, uint32_t vocab, bool bits)
+__host__ __device__ __forceinline__ size_t smem_bytes(const Layout& l, uint32_t k, uint32_t vocab, bool bits, bool seen)
 {
-    return (size_t)l.slots * l.chunk_vecs * 16 + 48 * (size_t)round4(k) +
-           (bits ? 8 * (size_t)(bitmap_words(vocab) + owner_words(l, vocab)) : 0);
+    return (size_t)l.slots * l.chunk_vecs * 16 + 48 * (size_t)k +
+           (bits ? 8 * (size_t)(bitmap_words(vocab) + owner_words(l, vocab)) : seen ? 4 * kSeenWords : 0);
 }
 // Word of `owners` for element v of the vectors (bit: thread % 32)
 template <typename T>
@@ -332,7 +334,13 @@ __device__ void entries_before(const DistillArgs& a, const Layout& lay, uint32_t
     bool bad = false;
     bool twice = false;
     double tmax = -INFINITY, tsum = 0.0;
-    if (lane < 3 && a.k + lane < round4(a.k)) l.idx[a.k + lane] = -1;
+    if (row + gridDim.x < a.rows) {  // the entries of the row after are fetched by the time they are wanted
+        const char* const i = reinterpret_cast<const char*>(a.idx) + (uint64_t)(row + gridDim.x) * a.ld_idx * a.idx_bytes;
+        const uint32_t ts = a.teacher_dtype == PS_DTYPE_F32 ? 4 : 2;
+        const char* const t = reinterpret_cast<const char*>(a.teacher) + (uint64_t)(row + gridDim.x) * a.ld_teacher * ts;
+        for (uint32_t at = lane * 128; at < a.k * a.idx_bytes; at += 32 * 128) prefetch(i + at);
+        for (uint32_t at = lane * 128; at < a.k * ts; at += 32 * 128) prefetch(t + at);
+    }
 #pragma unroll 4
     for (uint32_t j = lane; j < a.k; j += 32) {
         const long long v = index_at(a, (uint64_t)row * a.ld_idx + j);
@@ -342,34 +350,32 @@ __device__ void entries_before(const DistillArgs& a, const Layout& lay, uint32_t
         l.log_p[j] = teacher_at(a, (uint64_t)row * a.ld_teacher + j);
     }
 #pragma unroll 4
+    for (uint32_t j = lane; j < a.k; j += 32)
+        if (l.idx[j] >= 0) l.z[j] = Type<T>::load(z + l.idx[j]);
     for (uint32_t j = lane; j < a.k; j += 32) {
         const int v = l.idx[j];
         const double t = l.log_p[j];
         if (v < 0) continue;
-        l.z[j] = Type<T>::load(z + v);
         if (kBucket && (kWhat & kLoss)) {
-            const uint32_t bit = bit_of<T>(shape, (uint32_t)v);
-            atomicOr(&l.bits[bit >> 5], 1u << (bit & 31));
+            const uint32_t bit = bit_of<T>(shape, (uint32_t)v), one = 1u << (bit & 31);
+            if (atomicOr(&l.bits[bit >> 5], one) & one) twice = true;
             if ((uint32_t)v - shape.head < shape.vecs * Type<T>::kVec) {
                 uint32_t of;
                 const uint32_t w = owner_of<T>(lay, shape, (uint32_t)v, &of);
                 atomicOr(&l.owners[w], 1u << of);
             }
+        } else if (kWhat & kGrad) {  // two of an index share a bit (so may others: then it is looked up in vain)
+            const uint32_t bit = (uint32_t)v & (32 * kSeenWords - 1), one = 1u << (bit & 31);
+            if (atomicOr(&l.seen[bit >> 5], one) & one) twice = true;
         }
         tmax = (t > tmax || t != t) ? t : tmax;
     }
-    if (kWhat & kGrad) {  // of the four indices of a group the own one counts as well
-        __syncwarp();
-        for (uint32_t j = lane; j < a.k; j += 32) {
-            const int v = l.idx[j];
-            int n = 0;
-            for (uint32_t i = 0; i < a.k; i += 4) {
-                const int4 w = *reinterpret_cast<const int4*>(l.idx + i);
-                n += (w.x == v) + (w.y == v) + (w.z == v) + (w.w == v);
-            }
-            if (v >= 0 && n > 1) twice = true;
-        }
+    if (kWhat & kGrad) {
         twice = __any_sync(0xffffffffu, twice);
+        __syncwarp();
+        if (!(kBucket && (kWhat & kLoss)))
+            for (uint32_t j = lane; j < a.k; j += 32)
+                if (l.idx[j] >= 0) l.seen[((uint32_t)l.idx[j] & (32 * kSeenWords - 1)) >> 5] = 0;
     }
     if (!kBucket) tmax = warp_max(tmax);
     const double origin = kBucket || tmax == -INFINITY ? 0.0 : tmax;
@@ -383,7 +389,7 @@ __device__ void entries_before(const DistillArgs& a, const Layout& lay, uint32_t
     double rest = 0.0, mass = tsum;
     if (!kBucket) {
         mass = tsum == 0.0 ? 0.0 : tsum / tsum;  // a NaN stays
-        const double inv = tsum == 0.0 ? 0.0 : 1.0 / tsum, log_sum = log(tsum);
+        const double inv = tsum == 0.0 ? 0.0 : 1.0 / tsum, log_sum = (kWhat & kLoss) ? log(tsum) : 0.0;
         for (uint32_t j = lane; j < a.k; j += 32) l.p[j] *= inv, l.log_p[j] -= log_sum;
     } else if (kWhat & kLoss) {
         bool all = false;  // the whole vocabulary is listed
@@ -412,6 +418,7 @@ __device__ void entries_after(const DistillArgs& a, const Layout& lay, uint32_t 
     const uint32_t lane = threadIdx.x & 31;
     if (!slot.keep) return;
     const Origin o(slot.M, c);
+    const T* const zr = reinterpret_cast<const T*>(a.z) + (uint64_t)row * a.ldz;
     if (kWhat & kLoss) {
         const double log_z = log((double)(slot.out + slot.in));
         double t = 0.0;
@@ -445,8 +452,7 @@ __device__ void entries_after(const DistillArgs& a, const Layout& lay, uint32_t 
     }
     if (kBucket && (kWhat & kLoss)) {  // the bitmap is zeros again
         __syncwarp();
-        const T* const z = reinterpret_cast<const T*>(a.z) + (uint64_t)row * a.ldz;
-        const RowShape shape = row_shape(z, a.vocab);
+        const RowShape shape = row_shape(zr, a.vocab);
         for (uint32_t j = lane; j < a.k; j += 32)
             if (l.idx[j] >= 0) {
                 const uint32_t v = (uint32_t)l.idx[j];
@@ -477,16 +483,16 @@ distill_kernel(const DistillArgs a, const Layout lay)
     const float c = (float)(1.4426950408889634 / (double)a.temperature);
     Listed listed[2];
     {
-        const uint32_t k4 = round4(a.k);  // four indices can be read at once
         double* const d = reinterpret_cast<double*>(smem + (size_t)lay.slots * lay.chunk_vecs * 16);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            listed[i].p = d + 2 * i * k4;
-            listed[i].log_p = d + (2 * i + 1) * k4;
-            listed[i].idx = reinterpret_cast<int*>(d + 4 * k4) + 2 * i * k4;
-            listed[i].z = reinterpret_cast<float*>(d + 4 * k4) + (2 * i + 1) * k4;
-            listed[i].bits = reinterpret_cast<uint32_t*>(d + 6 * k4) + i * bitmap_words(a.vocab);
-            listed[i].owners = reinterpret_cast<uint32_t*>(d + 6 * k4) + 2 * bitmap_words(a.vocab) + i * owner_words(lay, a.vocab);
+            listed[i].p = d + 2 * i * a.k;
+            listed[i].log_p = d + (2 * i + 1) * a.k;
+            listed[i].idx = reinterpret_cast<int*>(d + 4 * a.k) + 2 * i * a.k;
+            listed[i].z = reinterpret_cast<float*>(d + 4 * a.k) + (2 * i + 1) * a.k;
+            listed[i].bits = reinterpret_cast<uint32_t*>(d + 6 * a.k) + i * bitmap_words(a.vocab);
+            listed[i].seen = reinterpret_cast<uint32_t*>(d + 6 * a.k);
+            listed[i].owners = reinterpret_cast<uint32_t*>(d + 6 * a.k) + 2 * bitmap_words(a.vocab) + i * owner_words(lay, a.vocab);
         }
     }
 
@@ -502,6 +508,8 @@ distill_kernel(const DistillArgs a, const Layout lay)
     if (kBucket && (kWhat & kLoss))
         for (uint32_t i = threadIdx.x; i < 2 * (bitmap_words(a.vocab) + owner_words(lay, a.vocab)); i += blockDim.x)
             listed[0].bits[i] = 0;
+    else if (kWhat & kGrad)
+        for (uint32_t i = threadIdx.x; i < kSeenWords; i += blockDim.x) listed[0].seen[i] = 0;
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < lay.slots; ++s) tc::bar_init(&full[s], 1), tc::bar_init(&empty[s], warps);
         gave_up = 0;
@@ -825,10 +833,10 @@ int launch(const DistillArgs& a, cudaStream_t st)
     lay.threads = 1u << lay.shift;
     lay.chunk_vecs = kUnroll * lay.threads;
     lay.slots = kMaxSlots;
-    const bool bits = kBucket && (kWhat & kLoss);
+    const bool bits = kBucket && (kWhat & kLoss), seen = kWhat & kGrad;
     const size_t limit = (is_long ? 108 : 200) * 1024;  // two CTAs an SM, or what the longest bitmaps leave
-    while (lay.slots > 2 && smem_bytes(lay, a.k, a.vocab, bits) > limit) --lay.slots;
-    const size_t smem = smem_bytes(lay, a.k, a.vocab, bits);
+    while (lay.slots > 2 && smem_bytes(lay, a.k, a.vocab, bits, seen) > limit) --lay.slots;
+    const size_t smem = smem_bytes(lay, a.k, a.vocab, bits, seen);
     // As many rows in work as SMs hold, but for the gradient no more than L2 keeps until the second pass.
     uint64_t most = 227 * 1024 / (smem + 2048);
     const uint64_t by_threads = is_long ? 2 : (uint64_t)kMaxThreads * kCtas / (lay.threads + 64);
@@ -870,7 +878,7 @@ int check_problem(const ps_distill_problem* q, const float* inv_n)
     if (q->rows == 0) return PS_OK;
     if (q->vocab == 0 || q->k == 0) return PS_ERR_INVALID;
     if (q->vocab > (q->tail == PS_TAIL_BUCKET ? PS_DISTILL_MAX_VOCAB / 2 : PS_DISTILL_MAX_VOCAB) ||
-        q->k > PS_DISTILL_MAX_K)
+        q->k > PS_DISTILL_MAX_K || q->rows > 0x7fffffffu)
         return PS_ERR_LIMIT;
     if (q->logits == nullptr || q->indices == nullptr || q->teacher == nullptr) return PS_ERR_INVALID;
     if (q->reduction == PS_REDUCE_MEAN && q->mask != nullptr && inv_n == nullptr) return PS_ERR_INVALID;

@@ -113,6 +113,42 @@ def test_the_c_entries_refuse(L):
     assert lib.ps_block_matmul_gave_up(None) == L.PS_ERR_INVALID
 
 
+def test_the_layer_entries_refuse(L):
+    lib, p = L.lib, 4096
+
+    def layer(**kw):
+        d = dict(x=p, weight=p, ld_x=64, ld_weight=64, tokens=4, k=64, n=32)
+        d.update(kw)
+        return C.byref(L.Fp8LinearLayer(**d))
+
+    def forward(keep=0, y=p, ld=32, saved=p, scratch=p, **kw):
+        return lib.ps_fp8_linear_forward(layer(**kw), keep, y, ld, saved, scratch, None)
+
+    def backward(keep=3, saved=p, dy=p, ld=32, fmt=0, dx=p, dw=p, db=p, scratch=p, **kw):
+        return lib.ps_fp8_linear_backward(layer(**kw), keep, saved, dy, ld, fmt, dx, 64, dw, db, scratch, None)
+
+    for call in (forward, backward):
+        for bad in (dict(x_dtype=3), dict(x_dtype=-1), dict(kept_data=p, kept_fmt=2), dict(scratch=None)):
+            assert call(**bad) == L.PS_ERR_INVALID, bad
+        assert call(tokens=2 ** 31) == L.PS_ERR_LIMIT and call(k=2 ** 32 - 1) == L.PS_ERR_LIMIT
+        for bad in (dict(saved=p + 16), dict(scratch=p + 128)):
+            assert call(**bad) == L.PS_ERR_ALIGN, bad
+    assert forward(tokens=0, scratch=None) == 0 and forward(n=0) == 0
+    for bad in (dict(x=None), dict(weight=None), dict(weight_dtype=7), dict(keep=3, saved=None)):
+        assert forward(**bad) == L.PS_ERR_INVALID, bad
+    for bad in (dict(fmt=2), dict(keep=0), dict(keep=1), dict(keep=2), dict(saved=None), dict(dy=None)):
+        assert backward(**bad) == L.PS_ERR_INVALID, bad
+    assert backward(dx=None, dw=None, db=None) == 0
+    sizes = (C.c_uint64 * 3)()
+    assert lib.ps_fp8_linear_sizes(layer(), 3, None) == L.PS_ERR_INVALID
+    assert lib.ps_fp8_linear_sizes(None, 3, sizes) == L.PS_ERR_INVALID
+    assert lib.ps_fp8_linear_sizes(layer(tokens=130, k=70, n=40), 0, sizes) == 0 and sizes[0] == 0
+    # x and weight in rows of 80 bytes, scales of 128 for each of 512 contracted, pieces rounded up to 256
+    assert sizes[1] == (130 * 80 + 96) + 1024 + 512 + 3328 + 512
+    assert lib.ps_fp8_linear_sizes(layer(tokens=130, k=70, n=40), 3, sizes) == 0
+    assert sizes[0] == 3328 + 512 + (130 * 80 + 96) + 512
+
+
 def test_layers_are_changed_in_place(ps):
     net = torch.nn.Sequential(torch.nn.Linear(4, 5), torch.nn.Tanh(), torch.nn.Bilinear(2, 2, 2),
                               torch.nn.Sequential(torch.nn.Linear(5, 6, bias=False)))

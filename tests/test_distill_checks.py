@@ -50,6 +50,7 @@ def test_the_c_entries_refuse(ps):
         assert call(vocab=L.PS_DISTILL_MAX_VOCAB + 1) == L.PS_ERR_LIMIT
         assert call(k=L.PS_DISTILL_MAX_K + 1) == L.PS_ERR_LIMIT
         assert call(vocab=L.PS_DISTILL_MAX_VOCAB // 2 + 1, tail=1) == L.PS_ERR_LIMIT
+        assert call(rows=2 ** 31) == L.PS_ERR_LIMIT
         for bad in (dict(logits=p + 1), dict(teacher=p + 2), dict(indices=p + 4), dict(stats=p + 8)):
             assert call(**bad) == L.PS_ERR_ALIGN, bad
     assert lib.ps_distill_forward(None, p, p, p, None, None, None, 0, None, None) == L.PS_ERR_INVALID
@@ -60,4 +61,5 @@ def test_the_c_entries_refuse(ps):
     for bad in (dict(g=None), dict(grad=None), dict(ld=9), dict(used=p, reduction=0)):
         assert backward(**bad) == L.PS_ERR_INVALID, bad
     assert backward(grad=p + 1) == L.PS_ERR_ALIGN
+    assert lib.ps_distill_gave_up(None) == L.PS_ERR_INVALID
     assert backward(rows=0, logits=None) == 0 and forward(rows=0, logits=None, reduction=0, row=None, stats=None) == 0

@@ -336,6 +336,61 @@ def test_gradients_of_broadcast_and_strided_inputs():
     assert torch.equal(a.t(), c)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("shape", [(130, 129, 41), (700, 260, 2305)])
+def test_rows_of_results_start_on_16_byte_boundaries(shape, dtype):
+    """Widths that are no multiple of 16 bytes: results are views of longer rows, and what reads them (a next layer,
+    its backward pass) takes them as they are."""
+    ps = _ps()
+    tokens, k, n = shape
+    x, w, _, _ = (t.to(DEV) for t in linear_case(tokens, k, n, dtype, 7))
+    x = x.view(2, tokens // 2, k).requires_grad_(True)
+    y = ps.fp8_linear(x, w)
+    assert y.shape == (2, tokens // 2, n) and (y.stride(1) * y.element_size()) % 16 == 0 and y.stride(2) == 1
+    assert torch.equal(y.view(-1, n), y.reshape(-1, n))
+    w2 = (torch.randn(24, n, device=DEV) * 0.1).to(dtype)
+    out = ps.fp8_linear(y, w2)
+    assert torch.equal(out, ps.fp8_linear(y.contiguous(), w2))
+    g = torch.randn_like(out)
+    got = torch.autograd.grad(out, x, g)[0]
+    leaf = y.detach().contiguous().requires_grad_(True)
+    dy = torch.autograd.grad(ps.fp8_linear(leaf, w2), leaf, g)[0]
+    assert torch.equal(got, torch.autograd.grad(ps.fp8_linear(x, w), x, dy.contiguous())[0])
+
+
+def test_a_second_derivative_is_refused():
+    ps = _ps()
+    x = torch.randn(8, 32, device=DEV).half().requires_grad_(True)
+    w = torch.randn(16, 32, device=DEV).half()
+    g = torch.autograd.grad(ps.fp8_linear(x, w).float().square().sum(), x, create_graph=True)[0]
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), x)
+
+
+def test_two_threads_at_once():
+    import threading
+    ps = _ps()
+    cases = [[t.to(DEV) for t in linear_case(300 + 100 * i, 640, 200, torch.float16, i)] for i in range(4)]
+    want = [ps.fp8_linear(x, w, b) for x, w, b, _ in cases]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                x, w, b, _ = cases[i]
+                if not torch.equal(ps.fp8_linear(x, w, b), want[i]):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
 def test_same_bits_every_time_and_on_another_stream():
     ps = _ps()
     x, w, b, dy = (t.to(DEV) for t in linear_case(700, 1600, 300, torch.bfloat16, 3))

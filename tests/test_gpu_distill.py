@@ -301,7 +301,7 @@ def test_no_rows():
     for kw in (dict(), dict(scaler=ps.LossScaler(4.0)), dict(mask=torch.zeros(0, dtype=torch.bool, device=DEV)),
                dict(reduction="sum"), dict(reduction="none")):
         loss = ps.distillation_loss(z, idx, teacher, **kw)
-        assert loss.shape == ((0,) if kw.get("reduction") == "none" else ()) and float(loss.sum()) == 0.0
+        assert loss.shape == ((0,) if kw.get("reduction") == "none" else ()) and float(loss.detach().sum()) == 0.0
         assert torch.autograd.grad(loss.sum(), z)[0].shape == (0, 50)
 
 
@@ -361,6 +361,31 @@ def test_same_bits_every_time_other_stream_and_replay():
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(captured, step()))
+
+
+@pytest.mark.parametrize("tail", ["drop", "bucket"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tau", [1e-4, 1e4])
+def test_extreme_logits_and_temperatures(dtype, tail, tau):
+    """Exponents beyond 2^30 (a small temperature, logits near the end of the type) and nearly none."""
+    ps = _ps()
+    z, idx, teacher = make(3, 300, 5, torch.float32, 20, "bucket")
+    z[1] = z[1] * (torch.finfo(dtype).max / 16)
+    z = z.to(dtype)
+    z.requires_grad_(True)
+    loss = ps.distillation_loss(z, idx, teacher, temperature=tau, tail=tail, reduction="none")
+    g = torch.autograd.grad(loss.sum(), z)[0]
+    want, wgrad = definition(z.detach(), idx, teacher, tau, tail)
+    # an exponent |z - M| / tau has a relative error of three roundings (and of 2^-24 in 1 / tau): of the exponents
+    # themselves where entries are far below the maximum, and those are summed with probabilities of at most 1 in all
+    size = (z.detach().double().cpu().amax(1) - z.detach().double().cpu().amin(1)) / tau
+    bound = (4 * 2.0 ** -24 * size + 4 * exponential_error(z.detach(), tau)) * tau * tau * 2 + 2.0 ** -22 * want.abs()
+    fine = torch.isfinite(want.float())
+    assert ((loss.detach().double().cpu() - want).abs() <= bound)[fine].all() and torch.isfinite(loss[fine.to(DEV)]).all()
+    # the gradient of a softmax whose exponents are off by e is off by at most 2 e of q (1 - q), and by q itself
+    # where e is large: then only its sign and size are held
+    q = (wgrad / tau).abs().max()
+    assert torch.isfinite(g).all() and float((g.double().cpu() / tau).abs().max()) <= 1.01 * float(q) + 1e-3
 
 
 def test_offsets_beyond_32_bits():
