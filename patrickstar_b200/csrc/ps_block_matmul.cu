@@ -46,7 +46,6 @@ struct ProductArgs {
     int a_k_inner, b_k_inner;  // the contracted dimension is the contiguous one
     int bias_dtype, out_dtype;
     int vec;                   // output rows start on 16-byte boundaries
-    int bias_vec;              // the bias does
 };
 
 __device__ __forceinline__ float bias_at(const ProductArgs& p, uint32_t col)
@@ -54,27 +53,6 @@ __device__ __forceinline__ float bias_at(const ProductArgs& p, uint32_t col)
     if (p.bias_dtype == PS_DTYPE_F16) return __half2float(reinterpret_cast<const __half*>(p.bias)[col]);
     if (p.bias_dtype == PS_DTYPE_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.bias)[col]);
     return reinterpret_cast<const float*>(p.bias)[col];
-}
-// Bias of four columns, 0 behind the last one; the same in all lanes.
-__device__ __forceinline__ float4 bias4_at(const ProductArgs& p, uint32_t col)
-{
-    float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (p.bias_vec && col + 4 <= p.n) {
-        if (p.bias_dtype == PS_DTYPE_F32) return __ldg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.bias) + col));
-        const uint2 w = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p.bias) + col));
-        if (p.bias_dtype == PS_DTYPE_F16) {
-            const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
-            const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
-            return make_float4(lo.x, lo.y, hi.x, hi.y);
-        }
-        return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
-                           __uint_as_float(w.y & 0xffff0000u));
-    }
-    if (col < p.n) b.x = bias_at(p, col);
-    if (col + 1 < p.n) b.y = bias_at(p, col + 1);
-    if (col + 2 < p.n) b.z = bias_at(p, col + 2);
-    if (col + 3 < p.n) b.w = bias_at(p, col + 3);
-    return b;
 }
 __device__ __forceinline__ uint32_t pack2(int dtype, float lo, float hi)
 {
@@ -277,9 +255,10 @@ block_matmul_split_kernel(const __grid_constant__ CUtensorMap map_a, const __gri
 constexpr uint32_t kPairTile = 256;
 constexpr int kPairStages = 5;
 constexpr uint32_t kPairStageBytes = 2 * kBoxBytes + 4 * kScaleBytes;  // scales: 1 of A, 2 of B, 1 unused
-constexpr uint32_t kPairThreads = 192;                                 // warps 0-3 epilogue, 4 loads, 5 tensor core
+constexpr uint32_t kPairWarps = 8;                                     // of the epilogue; behind them loads, tensor core
+constexpr uint32_t kPairThreads = 32 * (kPairWarps + 2);
 constexpr uint32_t kStoreBytes = 32 * 128;                             // 32 rows of 128 bytes a warp
-constexpr uint32_t kPairSmem = 1024 + kPairStages * kPairStageBytes + 4 * 2 * kStoreBytes;
+constexpr uint32_t kPairSmem = 1024 + kPairStages * kPairStageBytes + kPairWarps * kStoreBytes;
 constexpr uint32_t kAccStride = 224;
 constexpr uint32_t kScaleColumn = kAccStride + kPairTile;  // 480: twice 4 columns of A and 8 of B
 static_assert(kScaleColumn + 2 * 12 <= 512, "tensor memory");
@@ -296,19 +275,23 @@ __device__ __forceinline__ void tile_at(const ProductArgs& p, uint32_t t, uint32
 
 // 128 bytes of an output row from the accumulator's values; kOut is its type.
 template <int kOut>
-__device__ __forceinline__ void stage_row(unsigned char* buf, uint32_t row, const ProductArgs& p, uint32_t col,
-                                          uint32_t tmem, bool good, bool* loaded, uint64_t* drained)
+__device__ __forceinline__ void stage_row(unsigned char* buf, const ProductArgs& p, const float* bias, uint32_t tmem,
+                                          bool good, bool first, uint64_t* drained)
 {
+    const uint32_t row = threadIdx.x & 31;
     constexpr uint32_t kCols = kOut == PS_DTYPE_F32 ? 32 : 64;
     uint32_t v[kCols / 32][32];
 #pragma unroll
     for (uint32_t h = 0; h < kCols / 32; ++h) tc::tmem_ld32(tmem + 32 * h, v[h]);
     tc::tmem_ld_wait();
-    if (!*loaded) {
-        *loaded = true;
+    if (first) {
         tc::fence_before();
         __syncwarp();
-        if ((threadIdx.x & 31) == 0) tc::bar_arrive_at(drained, 0);
+        if (row == 0) tc::bar_arrive_at(drained, 0);
+    }
+    if (p.vec) {  // the store before has read the buffer
+        if (row == 0) tc::store_wait_read<0>();
+        __syncwarp();
     }
 #pragma unroll
     for (uint32_t q = 0; q < 8; ++q) {  // 16 bytes each, swizzled as the store's map says
@@ -319,7 +302,7 @@ __device__ __forceinline__ void stage_row(unsigned char* buf, uint32_t row, cons
         if (p.bias != nullptr) {
 #pragma unroll
             for (uint32_t i = 0; i < kPer; i += 4) {
-                const float4 b = bias4_at(p, col + q * kPer + i);
+                const float4 b = *reinterpret_cast<const float4*>(bias + q * kPer + i);
                 f[i] += b.x, f[i + 1] += b.y, f[i + 2] += b.z, f[i + 3] += b.w;
             }
         }
@@ -390,6 +373,7 @@ block_matmul_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     extern __shared__ unsigned char smem_raw[];
     __shared__ uint64_t full[kPairStages], empty[kPairStages], done, drained, ended;
     __shared__ uint32_t tmem_base;
+    __shared__ __align__(16) float s_bias[kPairWarps][kPairTile / 2];
     __shared__ volatile int gave_up;
 
     const uint32_t base = (tc::smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -401,12 +385,12 @@ block_matmul_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     if (threadIdx.x == 0) {
         for (int s = 0; s < kPairStages; ++s) tc::bar_init(&full[s], 1), tc::bar_init(&empty[s], 1);
         tc::bar_init(&done, 1);
-        tc::bar_init(&drained, 8);  // the four epilogue warps of both CTAs
+        tc::bar_init(&drained, 2 * kPairWarps);  // the epilogue's warps of both CTAs
         tc::bar_init(&ended, 1);
         gave_up = 0;
         tc::bar_init_fence();
     }
-    if (warp == 5) tc::tmem_alloc<2>(&tmem_base, 512);
+    if (warp == kPairWarps + 1) tc::tmem_alloc<2>(&tmem_base, 512);
     tc::fence_before();
     __syncthreads();
     tc::cluster_sync();
@@ -415,7 +399,7 @@ block_matmul_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     cudaTriggerProgrammaticLaunchCompletion();
     cudaGridDependencySynchronize();  // up to here nothing that another kernel writes was touched
 
-    if (warp == 4 && tc::elect_one()) {
+    if (warp == kPairWarps && tc::elect_one()) {
         uint32_t issued = 0;
         bool ok = true;
         for (uint32_t t = first; t < tiles && ok; t += step) {
@@ -452,7 +436,7 @@ block_matmul_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
             for (uint32_t i = issued < kPairStages ? 0 : issued - kPairStages; i < issued; ++i)
                 tc::bar_wait(&full[i % kPairStages], (i / kPairStages) & 1, &ignore);
         }
-    } else if (warp == 5 && rank == 0 && tc::elect_one()) {
+    } else if (warp == kPairWarps + 1 && rank == 0 && tc::elect_one()) {
         const uint32_t a_step = p.a_k_inner ? 32 : 32 * kTile, b_step = p.b_k_inner ? 32 : 32 * kTile;
         uint32_t used = 0, groups = 0, it = 0;
         bool ok = true;
@@ -493,42 +477,43 @@ block_matmul_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
             int ignore = 0;
             tc::bar_wait(&ended, 0, &ignore);
         }
-    } else if (warp < 4) {
-        constexpr uint32_t kCols = kOut == PS_DTYPE_F32 ? 32 : 64, kChunks = kPairTile / kCols;
-        unsigned char* const bufs = base_ptr + kPairStages * kPairStageBytes + warp * 2 * kStoreBytes;
-        uint32_t it = 0, n = 0;
+    } else if (warp < kPairWarps) {
+        // eight warps: four groups of 32 lanes, two halves of the columns
+        constexpr uint32_t kCols = kOut == PS_DTYPE_F32 ? 32 : 64, kChunks = kPairTile / 2 / kCols;
+        const uint32_t quarter = warp & 3, half = warp >> 2;
+        unsigned char* const buf = base_ptr + kPairStages * kPairStageBytes + warp * kStoreBytes;
+        uint32_t it = 0;
         bool good = true;
         for (uint32_t t = first; t < tiles; t += step, ++it) {
             uint32_t tm, tn;
             tile_at(p, t, &tm, &tn);
+            const uint32_t row0 = tm * kPairTile + rank * kTile + quarter * 32;
+            if (p.bias != nullptr) {
+                for (uint32_t i = lane; i < kPairTile / 2; i += 32) {
+                    const uint32_t col = tn * kPairTile + half * (kPairTile / 2) + i;
+                    s_bias[warp][i] = col < p.n ? bias_at(p, col) : 0.f;
+                }
+                __syncwarp();
+            }
             good = good && tc::bar_wait(&done, it & 1, &gave_up);
             good = __all_sync(0xffffffffu, good);
             tc::fence_after();
-            const uint32_t acc = tmem + (it & 1) * kAccStride + (warp << 21);
-            const uint32_t row0 = tm * kPairTile + rank * kTile + warp * 32;
-            bool loaded = false;
-            for (uint32_t c = 0; c < kChunks; ++c, ++n) {
+            const uint32_t acc = tmem + (it & 1) * kAccStride + (quarter << 21);
+            for (uint32_t c = 0; c < kChunks; ++c) {
                 // the overlapping columns first: the last ones of the lower accumulator, the first of the upper
-                const uint32_t chunk = (it & 1) ? c : (c == 0 ? kChunks - 1 : c - 1);
-                const uint32_t col = tn * kPairTile + chunk * kCols;
-                unsigned char* const buf = bufs + (n & 1) * kStoreBytes;
-                if (p.vec) {
-                    if (lane == 0) tc::store_wait_read<1>();
-                    __syncwarp();
-                }
-                stage_row<kOut>(buf, lane, p, col, acc + chunk * kCols, good, &loaded, &drained);
+                const uint32_t in_half = (it & 1) ? c : kChunks - 1 - c, at = half * (kPairTile / 2) + in_half * kCols;
+                const uint32_t col = tn * kPairTile + at;
+                stage_row<kOut>(buf, p, &s_bias[warp][in_half * kCols], acc + at, good, c == 0, &drained);
                 if (p.vec) tc::fence_to_async();
                 __syncwarp();
-                if (row0 >= p.m || col >= p.n) {
-                    if (p.vec && lane == 0) tc::store_none();
-                    continue;
+                if (row0 < p.m && col < p.n) {
+                    if (p.vec) {
+                        if (lane == 0) tc::store_box(&map_out, tc::smem_u32(buf), (int)col, (int)row0);
+                    } else {
+                        store_rows<kOut>(p, buf, row0, col);
+                    }
                 }
-                if (p.vec) {
-                    if (lane == 0) tc::store_box(&map_out, tc::smem_u32(buf), (int)col, (int)row0);
-                } else {
-                    store_rows<kOut>(p, buf, row0, col);
-                    __syncwarp();
-                }
+                __syncwarp();
             }
         }
         if (lane == 0) tc::store_wait_read<0>();
@@ -537,7 +522,7 @@ block_matmul_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     __syncwarp();
     __syncthreads();
     tc::cluster_sync();
-    if (warp == 5) tc::tmem_free<2>(tmem, 512);
+    if (warp == kPairWarps + 1) tc::tmem_free<2>(tmem, 512);
     if (threadIdx.x == 0 && gave_up) atomicAdd(&g_gave_up, 1u);
 }
 
@@ -722,7 +707,6 @@ int ps_block_matmul(const ps_block_operand* a, const ps_block_operand* b, uint32
     }
     p.bias = bias_dev, p.bias_dtype = bias_dtype, p.out = out_dev, p.out_dtype = out_dtype, p.ldo = ldo;
     p.m = m, p.n = n, p.n_kb = ceil_div(k, kTile);
-    p.bias_vec = (uintptr_t)bias_dev % 16 == 0;
     p.vec = (uintptr_t)out_dev % 16 == 0 && (ldo * osize) % 16 == 0;
     const int sms = ps_internal::sm_count();
     if (sms < 0) return sms;

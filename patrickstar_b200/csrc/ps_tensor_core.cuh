@@ -182,8 +182,6 @@ __device__ __forceinline__ void store_box(const CUtensorMap* m, uint32_t src, in
                  : "memory");
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
-// Stands for a store that was left out.
-__device__ __forceinline__ void store_none() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 // Until at most `kLeft` of this thread's stores still read shared memory.
 template <int kLeft>
 __device__ __forceinline__ void store_wait_read()
