@@ -151,12 +151,12 @@ def _quantize(x, blocks, fmt):
     dev = x.device
     q1 = s1 = q0 = s0 = None
     if blocks != "col":
-        q1 = torch.empty((rows, ldq), dtype=dtype, device=dev)
-        s1 = torch.empty(_scales_shape(rows, cols), dtype=torch.uint8, device=dev)
+        q1 = x.new_empty((rows, ldq), dtype=dtype)
+        s1 = x.new_empty(_scales_shape(rows, cols), dtype=torch.uint8)
     if blocks in ("col", "row+col"):
-        q0 = torch.empty((rows, ldq), dtype=dtype, device=dev)
+        q0 = x.new_empty((rows, ldq), dtype=dtype)
     if blocks != "row":
-        s0 = torch.empty(_scales_shape(cols, rows), dtype=torch.uint8, device=dev)
+        s0 = x.new_empty(_scales_shape(cols, rows), dtype=torch.uint8)
     with current_device(dev):
         check(lib.ps_block_quantize(
             x.data_ptr(), _DTYPES[x.dtype], x.stride(0) if rows > 1 else cols, rows, cols, _BLOCKS[blocks], code,
@@ -192,18 +192,18 @@ def block_quantize(x, blocks="row", fmt="e4m3"):
     return _quantize(x.detach(), blocks, fmt)
 
 
-def _rows(m, n, dtype, device):
-    """An uninitialised [m, n] tensor whose rows start on 16-byte boundaries: the product then leaves the SM in whole
+def _rows(like, m, n, dtype):
+    """An uninitialised [m, n] tensor on the device of ``like`` whose rows start on 16-byte boundaries: the product then leaves the SM in whole
     boxes.  Rows of other sizes are a view of longer ones."""
     per = 16 // dtype.itemsize
     ld = -(-n // per) * per
-    out = torch.empty((m, ld), dtype=dtype, device=device)
+    out = like.new_empty((m, ld), dtype=dtype)
     return out if ld == n else out[:, :n]
 
 
 def _matmul(a, a_dim, b, b_dim, bias, out_dtype):
     m, n, k = a.shape[1 - a_dim], b.shape[1 - b_dim], a.shape[a_dim]
-    out = _rows(m, n, out_dtype, a.device)
+    out = _rows(a.data, m, n, out_dtype)
     with current_device(a.device):
         check(lib.ps_block_matmul(
             C.byref(a._operand(a_dim)), C.byref(b._operand(b_dim)), m, n, k,
@@ -291,9 +291,9 @@ def _linear_forward(x, weight, bias, kept, keep):
         bias = bias.contiguous()
     dev = x.device
     saved_bytes, scratch_bytes, _ = _layer_bytes(tokens, k, n, kept is not None, keep)
-    y = _rows(tokens, n, x.dtype, dev)
-    saved = torch.empty(saved_bytes, dtype=torch.uint8, device=dev) if saved_bytes else None
-    scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=dev)
+    y = _rows(x, tokens, n, x.dtype)
+    saved = x.new_empty(saved_bytes, dtype=torch.uint8) if saved_bytes else None
+    scratch = x.new_empty(scratch_bytes, dtype=torch.uint8)
     layer = _layer(x, weight, bias, kept, tokens, k, n)
     with current_device(dev):
         check(lib.ps_fp8_linear_forward(C.byref(layer), keep, y.data_ptr(), max(n, y.stride(0)),
@@ -338,10 +338,10 @@ class _Fp8Linear(torch.autograd.Function):
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dy = _adjacent(dy)
         tokens, k, n = layer.tokens, layer.k, layer.n
-        dx = _rows(tokens, k, ctx.x_dtype, dev) if need_x else None
-        dw = torch.empty((n, k), dtype=ctx.w_dtype, device=dev) if need_w else None
-        db = torch.empty(n, dtype=ctx.b_dtype, device=dev) if need_b else None
-        scratch = torch.empty(_layer_bytes(tokens, k, n, bool(layer.kept_data), ctx.keep)[2], dtype=torch.uint8, device=dev)
+        dx = _rows(dy, tokens, k, ctx.x_dtype) if need_x else None
+        dw = dy.new_empty((n, k), dtype=ctx.w_dtype) if need_w else None
+        db = dy.new_empty(n, dtype=ctx.b_dtype) if need_b else None
+        scratch = dy.new_empty(_layer_bytes(tokens, k, n, bool(layer.kept_data), ctx.keep)[2], dtype=torch.uint8)
         with current_device(dev):
             check(lib.ps_fp8_linear_backward(
                 C.byref(layer), ctx.keep, None if saved is None else saved.data_ptr(), dy.data_ptr(),

@@ -114,6 +114,8 @@ block_matmul_split_kernel(const __grid_constant__ CUtensorMap map_a, const __gri
     const uint32_t kb0 = (uint32_t)((uint64_t)p.n_kb * rank / splits);
     const uint32_t kb1 = (uint32_t)((uint64_t)p.n_kb * (rank + 1) / splits);
 
+    if (warp == 4 && p.n_kb > 0 && tc::elect_one())
+        tc::prefetch_map(&map_a), tc::prefetch_map(&map_b), tc::prefetch_map(&map_sa), tc::prefetch_map(&map_sb);
     if (threadIdx.x == 0) {
         for (int s = 0; s < kSplitStages; ++s) tc::bar_init(&full[s], 1), tc::bar_init(&empty[s], 1);
         tc::bar_init(&done, 1);
@@ -185,7 +187,7 @@ block_matmul_split_kernel(const __grid_constant__ CUtensorMap map_a, const __gri
         tc::fence_after();
         float* row = reinterpret_cast<float*>(base_ptr) + (size_t)(warp * 32 + lane) * kPartialPitch;
         const bool good = ok && !gave_up;
-        for (uint32_t c = 0; c < kTile; c += 32) {
+        for (uint32_t c = 0; c < kTile && tm * kTile + warp * 32 < p.m; c += 32) {  // rows that there are
             uint32_t v[32];
             if (kb0 < kb1) {
                 tc::tmem_ld32(tmem + (warp << 21) + c, v);
@@ -382,6 +384,8 @@ block_matmul_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     const uint32_t rank = tc::cluster_rank();
     const uint32_t tiles = p.tiles_m * p.tiles_n, first = blockIdx.x / 2, step = gridDim.x / 2;
 
+    if (warp == kPairWarps && tc::elect_one())
+        tc::prefetch_map(&map_a), tc::prefetch_map(&map_b), tc::prefetch_map(&map_sa), tc::prefetch_map(&map_sb);
     if (threadIdx.x == 0) {
         for (int s = 0; s < kPairStages; ++s) tc::bar_init(&full[s], 1), tc::bar_init(&empty[s], 1);
         tc::bar_init(&done, 1);

@@ -29,8 +29,8 @@ def _like_rows(z):
     ld = vocab + (z.stride(0) - vocab) % per if rows > 1 else vocab
     off = z.data_ptr() % 16 // z.element_size()
     if ld == vocab and off == 0:
-        return torch.empty((rows, vocab), dtype=z.dtype, device=z.device)
-    return torch.empty(rows * ld + off, dtype=z.dtype, device=z.device).as_strided((rows, vocab), (ld, 1), off)
+        return z.new_empty((rows, vocab))
+    return z.new_empty(rows * ld + off).as_strided((rows, vocab), (ld, 1), off)
 
 
 def _point(problem, z, idx, teacher, mask):
@@ -45,8 +45,8 @@ def _forward(z, idx, teacher, mask, problem, scaler):
     the scale of the gradient, two unused ones, four for each row."""
     dev, rows = z.device, z.shape[0]
     reduce = problem.reduction != PS_REDUCE_NONE
-    out = torch.empty(() if reduce else rows, dtype=torch.float32, device=dev)
-    buf = torch.empty(4 + (5 if reduce else 4) * rows, dtype=torch.float32, device=dev)
+    out = z.new_empty(() if reduce else rows, dtype=torch.float32)
+    buf = z.new_empty(4 + (5 if reduce else 4) * rows, dtype=torch.float32)
     grad = _like_rows(z) if scaler is not None and rows else None
     at, o = buf.data_ptr(), out.data_ptr()
     _point(problem, z, idx, teacher, mask)
