@@ -254,14 +254,16 @@ __device__ __forceinline__ void quantize_tile(const QuantArgs& a, uint32_t tile,
 #pragma unroll
                 for (int d = 1; d < 16; d <<= 1) rk[i] = V::raise(rk[i], __shfl_xor_sync(0xffffffffu, rk[i], d));
         }
+        uint32_t mine = 0;  // eight of the sixteen lanes of a row group write one row's byte each
 #pragma unroll
         for (int i = 0; i < kRowsPerThread; ++i) {
             const uint32_t byte = scale_byte<kFmt>(V::magnitude(rk[i]));
             row_inv[i] = scale_inverse(byte);
-            if (cg == i) {
-                const uint32_t r = r0 + 16 * i;
-                put_scale(a.s1, r, cb, a.col_blocks, a.row_blocks, r < a.rows ? byte : 0u);
-            }
+            if (cg == i) mine = byte;
+        }
+        if (cg < kRowsPerThread) {
+            const uint32_t r = r0 + 16 * cg;
+            put_scale(a.s1, r, cb, a.col_blocks, a.row_blocks, r < a.rows ? mine : 0u);
         }
     }
     float col_inv[8];
