@@ -45,7 +45,7 @@ struct ProductArgs {
     uint32_t idesc;
     int a_k_inner, b_k_inner;  // the contracted dimension is the contiguous one
     int bias_dtype, out_dtype;
-    int vec;                   // output rows start on 16-byte boundaries
+    int vec, n_vec;            // output rows start, and end, on 16-byte boundaries
 };
 
 __device__ __forceinline__ float bias_at(const ProductArgs& p, uint32_t col)
@@ -249,6 +249,10 @@ block_matmul_split_kernel(const __grid_constant__ CUtensorMap map_a, const __gri
 // 256 x 256 tiles, one after another on each pair of SMs: the pair's tensor
 // cores work as one (cta_group::2), each CTA holding 128 rows of A, 128 rows of
 // B and 128 rows of the accumulator.
+//
+// A k block keeps an SM's tensor core busy for 512 cycles and brings it 32 KB, 64 bytes a cycle, all that an SM can
+// read; tiles of 128 x 128 would need twice that.  8192^3: 363 us in a burst (3.03 PF), 444 us at the power cap; a
+// sixth stage of 34 KB instead of the second store buffer gains nothing there.
 //
 // Two accumulators of 256 columns and the scales do not fit into 512 columns of
 // tensor memory, so the accumulators overlap in 32 columns: the epilogue reads
@@ -511,7 +515,8 @@ block_matmul_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                 if (p.vec) tc::fence_to_async();
                 __syncwarp();
                 if (row0 < p.m && col < p.n) {
-                    if (p.vec) {
+                    // a box reaches over the last column in steps of 16 bytes: what is behind it would be written
+                    if (p.vec && (p.n_vec || col + kCols <= p.n)) {
                         if (lane == 0) tc::store_box(&map_out, tc::smem_u32(buf), (int)col, (int)row0);
                     } else {
                         store_rows<kOut>(p, buf, row0, col);
@@ -595,17 +600,18 @@ uint32_t splits_of(uint64_t tiles, uint32_t n_kb, int sms)
     return splits;
 }
 
-// 256 x 256 tiles on pairs of SMs, or 128 x 128 tiles on single ones, whichever should be done first: in both a k block
-// takes an SM some 520 cycles, the small tile's for what it reads (32 KB at 64 bytes a cycle), the large one's for its
-// products, so only what the rounds leave idle counts; the large tiles' set-up is that of a few k blocks.
-// (1600 x 1600 x 16385: 49 large tiles 40 us, 169 small ones 72 us; 1 x 6400 x 1600: 25 large 17 us, 100 small 12 us.)
+// 256 x 256 tiles on pairs of SMs, or 128 x 128 tiles, two to an SM and split along k, whichever should be done first.
+// In hundredths of a microsecond, from a fit to measured products: 400 and 32 for each round and k block, or 650 and 60 (the
+// small tile reads twice as much for a product, and its cluster meets twice).  Measured, large / small: 300 x 300 x 16000
+// 73 / 18 us; 1 x 6400 x 1600 8.1 / 7.8; 64 x 1600 x 800 6.1 / 8.6; 1024 x 1600 x 4800 16.1 / 17.1; 1 x 20480 x 5120
+// 35 / 42; 1600 x 1600 x 16385 45 / 73; 4096 x 4800 x 1600 28 / 59.
 bool use_pairs(uint32_t m, uint32_t n, uint32_t n_kb, int sms)
 {
     if (n_kb == 0) return false;
     const uint64_t large = (uint64_t)ceil_div(m, kPairTile) * ceil_div(n, kPairTile), pairs = (uint64_t)sms / 2;
     const uint64_t small = (uint64_t)ceil_div(m, kTile) * ceil_div(n, kTile), splits = splits_of(small, n_kb, sms);
-    const uint64_t as_pairs = (large + pairs - 1) / pairs * n_kb + 4;
-    const uint64_t as_split = (small * splits + sms - 1) / sms * ((n_kb + splits - 1) / splits);
+    const uint64_t as_pairs = 400 + 32 * ((large + pairs - 1) / pairs) * n_kb;
+    const uint64_t as_split = 650 + 60 * ((small * splits + 2 * sms - 1) / (2 * sms)) * ((n_kb + splits - 1) / splits);
     return as_pairs <= as_split;
 }
 
@@ -711,6 +717,7 @@ int ps_block_matmul(const ps_block_operand* a, const ps_block_operand* b, uint32
     }
     p.bias = bias_dev, p.bias_dtype = bias_dtype, p.out = out_dev, p.out_dtype = out_dtype, p.ldo = ldo;
     p.m = m, p.n = n, p.n_kb = ceil_div(k, kTile);
+    p.n_vec = (n * osize) % 16 == 0;
     p.vec = (uintptr_t)out_dev % 16 == 0 && (ldo * osize) % 16 == 0;
     const int sms = ps_internal::sm_count();
     if (sms < 0) return sms;

@@ -15,7 +15,9 @@
 // One CTA takes a 128 x 128 tile into registers with all of its loads in
 // flight at once, reduces the magnitudes (two 16-bit ones to a word), and writes
 // every output the caller wants from that one read: 2 bytes in and 1 or 2 bytes
-// out per 16-bit element.  HBM-bound, if it gets by with few instructions.
+// out per 16-bit element.  HBM-bound where it gets by with few instructions: rows
+// alone 5.9 TB/s, columns alone 6.6 TB/s, both 5.2 to 5.8 TB/s (8192 x 5120 and
+// 8192 x 20480 fp16), tiles 6.2 TB/s.
 #include "ps_b200.h"
 
 #include "ps_internal.h"
@@ -160,7 +162,8 @@ struct QuantArgs {
 __host__ __device__ constexpr bool has_row(int mode) { return mode == PS_BLOCKS_ROW || mode == PS_BLOCKS_ROW_COL; }
 __host__ __device__ constexpr bool has_col(int mode) { return mode == PS_BLOCKS_COL || mode == PS_BLOCKS_ROW_COL; }
 
-// CTAs an SM holds: a tile is 32 registers a thread in 16 bits, 64 in 32
+// CTAs an SM holds: a tile is 32 registers a thread in 16 bits, 64 in 32.  (Both directions of 8192 x 5120 fp16: 35 us
+// with four CTAs of 64 registers, some of them spilled, 38 us with three.)
 template <typename T>
 __host__ __device__ constexpr int ctas_of()
 {

@@ -17,7 +17,9 @@
 // 0.1 to 0.5 MB a row).
 // The listed entries are few: one warp works on them in 64 bits beside the
 // others' pass.  Their gradient is written over the row's after it, so the pass
-// itself knows nothing of them but, for the bucket, one bit per element.  HBM-bound: one read, and one write for the
+// itself knows nothing of them but, for the bucket, one bit per element.
+// 4096 x 131073 bf16: loss alone 6.1 TB/s; 8192 x 50257 fp16, k = 64: loss 154 us
+// (5.4 TB/s), with the gradient 373 us (4.4 TB/s of one read and one write).  HBM-bound: one read, and one write for the
 // gradient; a power of two per element each pass.
 #include "ps_b200.h"
 
@@ -38,7 +40,9 @@ constexpr int kMaxThreads = 320;   // 256 of the pass
 constexpr int kLongThreads = 576;  // 512 of the pass, for the longest rows
 constexpr uint32_t kMaxSlots = 4;
 constexpr int kCtas = 3;  // of the largest kind on an SM: 64 registers a thread
-constexpr uint64_t kRowsInL2 = 64ull << 20;  // bytes of rows in work, of 126 MB
+// Bytes of rows in work, of 126 MB of L2.  8192 x 50257 fp16 with gradient: 373 us with 64 MB, 460 us with 32 MB (two
+// CTAs an SM), 377 us with 128 MB; 4096 x 50257 fp32 318, 434 and 371 us.
+constexpr uint64_t kRowsInL2 = 64ull << 20;
 constexpr int kUnroll = 4;  // vectors of a chunk for each thread of the pass
 
 __device__ unsigned int g_gave_up;  // CTAs that ran into the limit of a wait

@@ -209,21 +209,28 @@ def test_empty_and_one():
     assert ps.fp8_linear(torch.zeros(2, 3, 40, device=DEV).half(), w.detach()).shape == (2, 3, 24)
 
 
-def test_output_behind_the_last_column_and_row_stays():
-    """Through the C entry with a row stride larger than the columns."""
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,n,ldo", [(5, 19, 32), (130, 131, 140), (1000, 900, 913), (1000, 900, 912), (300, 257, 264),
+                                     (2100, 2303, 2304), (2100, 2305, 2320), (600, 2001, 2001), (129, 512, 520)])
+def test_output_behind_the_last_column_and_row_stays(m, n, ldo, dtype):
+    """Through the C entry with a row stride larger than the columns.  Sums of 100 products of at most 4 4 in
+    size and scales of at most 2^2 each are whole numbers below 25600; those above 2048 (fp16) or 256 (bf16) are
+    rounded once."""
     import ctypes as C
     from patrickstar_b200 import _lib as L
-    ps = _ps()
-    for m, n, ldo in ((5, 19, 32), (130, 131, 140), (1000, 900, 913)):
-        gen = torch.Generator().manual_seed(n)
-        a, av = integer_operand(m, 200, "row", "e4m3", gen)
-        b, bv = integer_operand(n, 200, "row", "e4m3", gen)
-        out = torch.full((m + 2, ldo), 123.0, device=DEV)
-        L.check(L.lib.ps_block_matmul(C.byref(a._operand(1)), C.byref(b._operand(1)), m, n, 200, None, 0,
-                                      out.data_ptr(), L.PS_DTYPE_F32, ldo,
+    code = {torch.float16: L.PS_DTYPE_F16, torch.bfloat16: L.PS_DTYPE_BF16, torch.float32: L.PS_DTYPE_F32}[dtype]
+    gen = torch.Generator().manual_seed(n)
+    a, av = integer_operand(m, 100, "row", "e4m3", gen)
+    b, bv = integer_operand(n, 100, "row", "e4m3", gen)
+    bias = torch.randint(-100, 100, (n,), generator=gen).to(dtype)
+    for shift in (0, 1):    # the second time from an address that is not on a 16-byte boundary
+        flat = torch.full(((m + 2) * ldo + shift,), 123.0, dtype=dtype, device=DEV)
+        out = flat[shift:].view(m + 2, ldo)
+        L.check(L.lib.ps_block_matmul(C.byref(a._operand(1)), C.byref(b._operand(1)), m, n, 100, bias.to(DEV).data_ptr(),
+                                      code, out.data_ptr(), code, ldo,
                                       C.c_void_p(torch.cuda.current_stream().cuda_stream)), "ps_block_matmul")
         got = out.cpu()
-        assert torch.equal(got[:m, :n].double(), av @ bv.t())
+        assert torch.equal(got[:m, :n], (av @ bv.t() + bias.double()).to(dtype))
         assert (got[m:] == 123.0).all() and (got[:, n:] == 123.0).all()
 
 
