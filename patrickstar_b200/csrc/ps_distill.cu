@@ -2,7 +2,7 @@
 // and its gradient with respect to the student's logits.
 //
 // For a row of logits z over the vocabulary, temperature T and c = log2(e) / T:
-//     M = max z,  e_v = 2^((z_v - M) c),  Z = sum e_v,  q_v = e_v / Z
+//     M an element near the largest,  e_v = 2^((z_v - M) c),  Z = sum e_v,  q_v = e_v / Z
 // and for the k listed entries (idx_j, t_j), S the set of listed indices:
 //     drop    p = softmax(t / T) over the listed;   p_r = 0
 //     bucket  p_j = exp(t_j);   p_r = max(0, 1 - sum p_j),   q_r = sum of q_v, v not in S
@@ -276,7 +276,7 @@ constexpr int kLoss = 1, kGrad = 2;
 // One row's listed entries and what the pass over it found; two of them, in turn.
 struct RowSlot {
     double rest, mass;  // p_r, and sum p + p_r: 1 unless the teacher gives nothing, or too much
-    float M, out, in;   // largest logit, sums outside of S and in it
+    float M, out, in;   // element that exponents are relative to, sums outside of S and in it
     float inside;           // factor of e_v in the gradient, v in S
     float grad;             // factor of the gradient: NaN for a bad row
     int keep, bad, twice;   // the mask keeps the row; an index is outside of the vocabulary; one is listed twice
@@ -830,17 +830,19 @@ int launch(const DistillArgs& a, cudaStream_t st)
     // there is no more than one row for an SM.
     const uint64_t bytes = (uint64_t)a.vocab * sizeof(T);
     const bool few = a.rows <= (uint32_t)sms;
-    Layout lay;
-    lay.shift = bytes <= 16 * 1024 ? 6 : bytes <= 160 * 1024 && !few ? 7 : 8;
-    const bool is_long = lay.shift == 8 && (bytes > 160 * 1024 || few) && bytes > 32 * 1024;
-    if (is_long) lay.shift = 9;
-    lay.threads = 1u << lay.shift;
-    lay.chunk_vecs = kUnroll * lay.threads;
-    lay.slots = kMaxSlots;
     const bool bits = kBucket && (kWhat & kLoss), seen = kWhat & kGrad;
-    const size_t limit = (is_long ? 108 : 200) * 1024;  // two CTAs an SM, or what the longest bitmaps leave
-    while (lay.slots > 2 && smem_bytes(lay, a.k, a.vocab, bits, seen) > limit) --lay.slots;
-    const size_t smem = smem_bytes(lay, a.k, a.vocab, bits, seen);
+    Layout lay;
+    lay.shift = bytes <= 16 * 1024 ? 6 : bytes <= 160 * 1024 && !few ? 7 : bytes <= 32 * 1024 ? 8 : 9;
+    size_t smem;
+    for (;; --lay.shift) {
+        lay.threads = 1u << lay.shift;
+        lay.chunk_vecs = kUnroll * lay.threads;
+        const size_t limit = (lay.shift == 9 ? 108 : 200) * 1024;  // two CTAs an SM
+        for (lay.slots = kMaxSlots; lay.slots > 2 && smem_bytes(lay, a.k, a.vocab, bits, seen) > limit; --lay.slots) {}
+        smem = smem_bytes(lay, a.k, a.vocab, bits, seen);
+        if (smem <= 224 * 1024 || lay.shift == 6) break;  // the longest bitmaps leave room for small chunks only
+    }
+    const bool is_long = lay.shift == 9;
     // As many rows in work as SMs hold, but for the gradient no more than L2 keeps until the second pass.
     uint64_t most = 227 * 1024 / (smem + 2048);
     const uint64_t by_threads = is_long ? 2 : (uint64_t)kMaxThreads * kCtas / (lay.threads + 64);

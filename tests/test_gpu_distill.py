@@ -388,6 +388,28 @@ def test_extreme_logits_and_temperatures(dtype, tail, tau):
     assert torch.isfinite(g).all() and float((g.double().cpu() / tau).abs().max()) <= 1.01 * float(q) + 1e-3
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab,k,tail", [(2 ** 19, 1024, "bucket"), (2 ** 19, 1, "bucket"), (2 ** 20, 1024, "drop"),
+                                          (300001, 700, "bucket")])
+def test_the_largest_sizes(vocab, k, tail, dtype):
+    """Bitmaps and listed entries that leave little shared memory for anything else."""
+    ps = _ps()
+    for rows in (1, 150):
+        z, idx, teacher = make(1, vocab, k, dtype, k, tail)
+        z, idx, teacher = z.repeat(rows, 1).requires_grad_(True), idx.repeat(rows, 1), teacher.repeat(rows, 1)
+        loss = ps.distillation_loss(z, idx, teacher, tail=tail, reduction="none")
+        g = torch.autograd.grad(loss, z, torch.full_like(loss, 256.0))[0]
+        check(z[-1:].detach(), idx[-1:], teacher[-1:], 1.0, tail, loss[-1:].detach(), g[-1:], 256.0)
+        scaler = ps.LossScaler(256.0 * rows)
+        total = ps.distillation_loss(z, idx, teacher, tail=tail, scaler=scaler)
+        fused = torch.autograd.grad(scaler.scale_loss(total), z)[0]
+        # every eighth row starts at the same offset from a 16-byte boundary (8 vocab elements are a multiple of it),
+        # so its terms are added in the same order; the others' in another one, as above
+        for t in (fused, g):
+            assert torch.equal(t[:1].expand(len(t[::8]), -1), t[::8])
+        check(z[:1].detach(), idx[:1], teacher[:1], 1.0, tail, total.detach().view(1), fused[:1], 256.0)
+
+
 def test_offsets_beyond_32_bits():
     """More than 2^32 bytes and 2^31 elements of logits; the last rows are right."""
     ps = _ps()
