@@ -97,6 +97,9 @@ def parse_config(config):
                          "got %r" % (mode,))
     out["fused_collectives"] = mode
     fp8 = config.get("fp8") or {}
+    for key in fp8:
+        if key not in ("enabled", "grad_format"):
+            raise ValueError("fp8 takes enabled and grad_format; got %r" % (key,))
     if fp8.get("enabled", False):
         out["fp8"] = fp8.get("grad_format", "e4m3")
         if out["fp8"] not in ("e4m3", "e5m2"):

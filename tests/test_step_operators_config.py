@@ -16,7 +16,7 @@ def test_values_and_refusals():
     p = parse_config({"distillation": {"temperature": 2.0, "tail": "bucket"}})
     assert p["distillation"] == {"temperature": 2.0, "tail": "bucket", "weight": 1.0}
     assert parse_config(None)["distillation"]["temperature"] == 1.0    # the defaults are not what was set above
-    for bad in ({"fp8": {"enabled": True, "grad_format": "e3m4"}}, {"distillation": {"tail": "rest"}},
+    for bad in ({"fp8": {"enabled": True, "grad_format": "e3m4"}}, {"fp8": {"enabled": True, "format": "e5m2"}}, {"distillation": {"tail": "rest"}},
                 {"distillation": {"alpha": 0.5}}):
         with pytest.raises(ValueError):
             parse_config(bad)
