@@ -72,6 +72,11 @@ struct DistillArgs {
 };
 
 __device__ __forceinline__ void prefetch(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+// Four bytes into shared memory, there after a cp.async.wait_all of the same thread.
+__device__ __forceinline__ void fetch4(void* dst, const void* src)
+{
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(tc::smem_u32(dst)), "l"(src) : "memory");
+}
 __device__ __forceinline__ float ex2(float x)
 {
     float y;
@@ -96,6 +101,10 @@ struct Type<__half> {
         return fmaxf(f.x, f.y);
     }
     static __device__ __forceinline__ float load(const __half* p) { return __half2float(*p); }
+    static __device__ __forceinline__ float half_of(uint32_t w, bool upper)
+    {
+        return __half2float(__ushort_as_half((unsigned short)(upper ? w >> 16 : w)));
+    }
     static __device__ __forceinline__ __half round(float f) { return __float2half_rn(f); }
     static __device__ __forceinline__ void unpack(const uint4& q, float (&f)[8])
     {
@@ -132,6 +141,10 @@ struct Type<__nv_bfloat16> {
         return fmaxf(__uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u));
     }
     static __device__ __forceinline__ float load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+    static __device__ __forceinline__ float half_of(uint32_t w, bool upper)
+    {
+        return __uint_as_float(upper ? w & 0xffff0000u : w << 16);
+    }
     static __device__ __forceinline__ __nv_bfloat16 round(float f) { return __float2bfloat16_rn(f); }
     static __device__ __forceinline__ void unpack(const uint4& q, float (&f)[8])
     {
@@ -284,7 +297,7 @@ struct RowSlot {
 struct Listed {
     double *p, *log_p;  // probabilities and their logarithms
     int* idx;           // or -1
-    float* z;           // logits
+    uint32_t* z;        // logits, or the words that hold them
     uint32_t* bits;     // of every element: is it listed?
     uint32_t* owners;   // of every thread and chunk: has it a listed element?
     uint32_t* seen;     // bits of indices seen, without the bitmap: zeros but while entries are looked at
@@ -353,9 +366,10 @@ __device__ void entries_before(const DistillArgs& a, const Layout& lay, uint32_t
         l.idx[j] = is ? (int)v : -1;
         l.log_p[j] = teacher_at(a, (uint64_t)row * a.ld_teacher + j);
     }
-#pragma unroll 4
+    // the logits of the listed entries are on their way until the pass over the row is done; of 16-bit types the
+    // aligned word that holds them
     for (uint32_t j = lane; j < a.k; j += 32)
-        if (l.idx[j] >= 0) l.z[j] = Type<T>::load(z + l.idx[j]);
+        if (l.idx[j] >= 0) fetch4(&l.z[j], reinterpret_cast<const void*>((uintptr_t)(z + l.idx[j]) & ~(uintptr_t)3));
     for (uint32_t j = lane; j < a.k; j += 32) {
         const int v = l.idx[j];
         const double t = l.log_p[j];
@@ -423,13 +437,24 @@ __device__ void entries_after(const DistillArgs& a, const Layout& lay, uint32_t 
     if (!slot.keep) return;
     const Origin o(slot.M, c);
     const T* const zr = reinterpret_cast<const T*>(a.z) + (uint64_t)row * a.ldz;
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    auto logit = [&](uint32_t j, int v) {  // every lane looks at what it has fetched itself
+        const uint32_t w = l.z[j];
+        if constexpr (sizeof(T) == 4)
+            return __uint_as_float(w);
+        else
+            return Type<T>::half_of(w, ((uintptr_t)(zr + v) >> 1) & 1);
+    };
     if (kWhat & kLoss) {
         const double log_z = log((double)(slot.out + slot.in));
         double t = 0.0;
         for (uint32_t j = lane; j < a.k; j += 32) {
-            const double x = o.far ? ((double)l.z[j] - (double)slot.M) * (double)c : (double)l.z[j] * (double)c - (double)o.r;
+            const int v = l.idx[j];
             const double p = l.p[j];
-            if (l.idx[j] >= 0 && p != 0.0) t += p * (l.log_p[j] - (x * 0.6931471805599453 - log_z));
+            if (v < 0 || p == 0.0) continue;
+            const double z = (double)logit(j, v);
+            const double x = o.far ? (z - (double)slot.M) * (double)c : z * (double)c - (double)o.r;
+            t += p * (l.log_p[j] - (x * 0.6931471805599453 - log_z));
         }
         t = warp_sum(t);
         if (kBucket && !(slot.rest <= 0.0)) t += slot.rest * (log(slot.rest) - (log((double)slot.out) - log_z));
@@ -451,7 +476,7 @@ __device__ void entries_after(const DistillArgs& a, const Layout& lay, uint32_t 
                 for (uint32_t i = 0; i < a.k; ++i)
                     if (l.idx[i] == v) p += (float)l.p[i];
             }
-            g[v] = Type<T>::round((ex2(o.exponent(l.z[j], c)) * slot.inside - p) * slot.grad);
+            g[v] = Type<T>::round((ex2(o.exponent(logit(j, v), c)) * slot.inside - p) * slot.grad);
         }
     }
     if (kBucket && (kWhat & kLoss)) {  // the bitmap is zeros again
@@ -493,7 +518,7 @@ distill_kernel(const DistillArgs a, const Layout lay)
             listed[i].p = d + 2 * i * a.k;
             listed[i].log_p = d + (2 * i + 1) * a.k;
             listed[i].idx = reinterpret_cast<int*>(d + 4 * a.k) + 2 * i * a.k;
-            listed[i].z = reinterpret_cast<float*>(d + 4 * a.k) + (2 * i + 1) * a.k;
+            listed[i].z = reinterpret_cast<uint32_t*>(d + 4 * a.k) + (2 * i + 1) * a.k;
             listed[i].bits = reinterpret_cast<uint32_t*>(d + 6 * a.k) + i * bitmap_words(a.vocab);
             listed[i].seen = reinterpret_cast<uint32_t*>(d + 6 * a.k);
             listed[i].owners = reinterpret_cast<uint32_t*>(d + 6 * a.k) + 2 * bitmap_words(a.vocab) + i * owner_words(lay, a.vocab);
