@@ -620,7 +620,8 @@ int ps_block_matmul_gave_up(uint32_t* count);
 #define PS_DISTILL_MAX_K 1024
 
 typedef struct ps_distill_problem {
-    const void* logits;  /* [rows, vocab], dtype; row stride in elements, any alignment of the type */
+    const void* logits;  /* [rows, vocab], dtype; row stride in elements, any alignment of the type (16-bit
+                            logits that are listed are read as the aligned 4-byte words that hold them) */
     const void* indices; /* [rows, k], int32 or int64 */
     const void* teacher; /* [rows, k], teacher_dtype */
     const void* mask;    /* uint8 [rows], or NULL: all rows */

@@ -18,8 +18,8 @@
 // The listed entries are few: one warp works on them in 64 bits beside the
 // others' pass.  Their gradient is written over the row's after it, so the pass
 // itself knows nothing of them but, for the bucket, one bit per element.
-// 4096 x 131073 bf16: loss alone 6.1 TB/s; 8192 x 50257 fp16, k = 64: loss 154 us
-// (5.4 TB/s), with the gradient 373 us (4.4 TB/s of one read and one write).  HBM-bound: one read, and one write for the
+// 4096 x 131073 bf16: loss alone 6.1 TB/s; 8192 x 50257 fp16, k = 64: loss 155 us
+// (5.3 TB/s), with the gradient 357 us (4.6 TB/s of one read and one write).  HBM-bound: one read, and one write for the
 // gradient; a power of two per element each pass.
 #include "ps_b200.h"
 
@@ -851,13 +851,21 @@ int launch(const DistillArgs& a, cudaStream_t st)
     if (sms < 0) return sms;
     // Threads for a row by its size: four vectors a thread and chunk, four chunks.  Small CTAs, since each brings a
     // warp for listed entries and rows' own latencies overlap (8192 x 50257 fp16, loss: 158 us with 128 threads,
-    // 167 us with 256).  More threads for the longest rows, of which L2 keeps two an SM for the second pass, and where
-    // there is no more than one row for an SM.
+    // 167 us with 256).  With the gradient, where L2 limits the rows in work, 256 threads do better (385 -> 357 us with
+    // 64 entries; 4096 x 70000 bf16 302 -> 240 us) if a row is long for its entries (128 of them: 455 -> 570 us).  512
+    // threads for the longest rows, of which L2 keeps two an SM for the second pass, and where there is no more than one
+    // row for an SM.
     const uint64_t bytes = (uint64_t)a.vocab * sizeof(T);
     const bool few = a.rows <= (uint32_t)sms;
     const bool bits = kBucket && (kWhat & kLoss), seen = kWhat & kGrad;
     Layout lay;
-    lay.shift = bytes <= 16 * 1024 ? 6 : bytes <= 160 * 1024 && !few ? 7 : bytes <= 32 * 1024 ? 8 : 9;
+    const bool wide = kWhat == (kLoss | kGrad) && !kBucket && bytes >= 1280 * (uint64_t)a.k;
+    if (bytes <= 16 * 1024)
+        lay.shift = 6;
+    else if (!few && bytes <= (wide ? 48 : 160) * 1024)
+        lay.shift = 7;
+    else
+        lay.shift = bytes <= 32 * 1024 || (!few && bytes <= 160 * 1024) ? 8 : 9;
     size_t smem;
     for (;; --lay.shift) {
         lay.threads = 1u << lay.shift;
