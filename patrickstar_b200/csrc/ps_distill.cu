@@ -10,6 +10,11 @@
 //     loss = T^2 ( sum_j p_j (log p_j - log q_idx_j) + p_r (log p_r - log q_r) )
 //     d loss / d z_v = T ( (sum p + p_r) q_v - sum_{j: idx_j = v} p_j - [v not in S] p_r q_v / q_r )
 // where sum p + p_r is 1, but for a row that lists nothing (0) or a teacher that gives more than 1.
+// The listed elements may lie so far above the others that relative to M nothing of these is left in 32 bits.  So
+// with the bucket the sum over the others is relative to an element M_out near the largest of them,
+//     e'_v = 2^((z_v - M_out) c),  Z' = sum of e'_v, v not in S,  q_r = Z' / (Z' + sum of the listed, brought to M_out)
+//     d loss / d z_v = T e'_v ((sum p + p_r) q_r - p_r) / Z',  v not in S
+// whose every factor is bounded.
 //
 // One CTA takes a row: one pass with a running maximum and sum of its own in
 // every thread, joined at the end; and for the gradient a second pass that reads
@@ -60,7 +65,7 @@ struct DistillArgs {
     float temperature, weight;
     float* row_loss;
     float* loss;         // of a single row (else NULL: the rows are summed by a launch of their own)
-    float4* stats;       // per row: M, factors of e_v in the gradient for v in S and for the others, -
+    float4* stats;       // per row: M, factors of e_v in the gradient for v in S and of e'_v for the others, M_out
     const float* inv_n;  // 1 / rows that the mask keeps, or NULL: then inv_n_value
     float inv_n_value;
     void* grad;
@@ -258,6 +263,8 @@ struct Origin {
     {
         return far ? (z - m) * c : fmaf(z, c, -r);
     }
+    // what the exponents are relative to
+    __device__ __forceinline__ double reference(float c) const { return far ? (double)m * (double)c : (double)r; }
     // of sums relative to this one, to make them relative to `to` (no smaller)
     __device__ __forceinline__ float factor(const Origin& to, float c) const
     {
@@ -268,19 +275,27 @@ struct Origin {
 
 // Running origin and sums of one thread: of elements outside of S, and of those in it.  The origin is an element,
 // not always the largest one: it is raised when an exponent would pass 2^4 (sums of 2^20 such terms are far from
-// the end of 32 bits), which after a thread's first elements hardly ever happens.
+// the end of 32 bits), which after a thread's first elements hardly ever happens.  The listed ones are few; their
+// sum is relative to the largest of them itself.
 struct Running {
     Origin o;
     Pair out = Pair(0.f, 0.f);
-    float in = 0.f;
+    float m_in = -INFINITY, in = 0.f;
     __device__ __forceinline__ void raise(float top, float c)
     {
         if (o.m == -INFINITY ? top > -INFINITY : o.exponent(top, c) > 16.f) {
             const Origin to(top, c);
             const float f = o.factor(to, c);
-            out = mul2(out, Pair(f, f)), in *= f;
+            out = mul2(out, Pair(f, f));
             o = to;
         }
+    }
+    __device__ __forceinline__ void add_listed(float z, float c)
+    {
+        if (z > m_in)
+            in = fmaf(in, ex2((m_in - z) * c), 1.f), m_in = z;
+        else if (z != -INFINITY)
+            in += ex2((z - m_in) * c);
     }
 };
 
@@ -289,7 +304,8 @@ constexpr int kLoss = 1, kGrad = 2;
 // One row's listed entries and what the pass over it found; two of them, in turn.
 struct RowSlot {
     double rest, mass;  // p_r, and sum p + p_r: 1 unless the teacher gives nothing, or too much
-    float M, out, in;   // element that exponents are relative to, sums outside of S and in it
+    float M, Z;             // element that exponents are relative to, and the sum of their powers
+    float M_out, out;       // the same of the elements outside of S (with the bucket)
     float inside;           // factor of e_v in the gradient, v in S
     float grad;             // factor of the gradient: NaN for a bad row
     int keep, bad, twice;   // the mask keeps the row; an index is outside of the vocabulary; one is listed twice
@@ -446,7 +462,7 @@ __device__ void entries_after(const DistillArgs& a, const Layout& lay, uint32_t 
             return Type<T>::half_of(w, ((uintptr_t)(zr + v) >> 1) & 1);
     };
     if (kWhat & kLoss) {
-        const double log_z = log((double)(slot.out + slot.in));
+        const double log_z = log((double)slot.Z);
         double t = 0.0;
         for (uint32_t j = lane; j < a.k; j += 32) {
             const int v = l.idx[j];
@@ -457,7 +473,10 @@ __device__ void entries_after(const DistillArgs& a, const Layout& lay, uint32_t 
             t += p * (l.log_p[j] - (x * 0.6931471805599453 - log_z));
         }
         t = warp_sum(t);
-        if (kBucket && !(slot.rest <= 0.0)) t += slot.rest * (log(slot.rest) - (log((double)slot.out) - log_z));
+        if (kBucket && !(slot.rest <= 0.0)) {
+            const double apart = Origin(slot.M_out, c).reference(c) - o.reference(c);
+            t += slot.rest * (log(slot.rest) - (apart * 0.6931471805599453 + log((double)slot.out) - log_z));
+        }
         if (slot.bad) t = (double)NAN;
         if (lane == 0) {
             const float f = (float)(t * (double)a.weight * (double)a.temperature * (double)a.temperature);
@@ -504,7 +523,7 @@ distill_kernel(const DistillArgs a, const Layout lay)
     constexpr int E = Type<T>::kVec;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ RowSlot slots[2];
-    __shared__ float s_m[kLongThreads / 32], s_out[kLongThreads / 32], s_in[kLongThreads / 32];
+    __shared__ float s_m[kLongThreads / 32], s_out[kLongThreads / 32], s_m_in[kLongThreads / 32], s_in[kLongThreads / 32];
     __shared__ uint64_t full[kMaxSlots], empty[kMaxSlots];
     __shared__ volatile int gave_up;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -641,7 +660,7 @@ distill_kernel(const DistillArgs a, const Layout lay)
             };
             const uint32_t whole_vecs = shape.vecs / lay.chunk_vecs * lay.chunk_vecs;
 
-            float M, outside;
+            float M_out, outside;  // what the pass writes in the gradient is relative to
             if (kWhat & kLoss) {
                 Running run;
                 const uint32_t* const bits = listed[it & 1].bits;
@@ -666,9 +685,7 @@ distill_kernel(const DistillArgs a, const Layout lay)
                         for (; in != 0; in &= in - 1) {
                             const uint32_t bit = __ffs(in) - 1;
                             T* const e = reinterpret_cast<T*>(from + (bit >> 3) * threads) + (bit & 7);
-                            const float f = Type<T>::load(e);
-                            run.raise(f, c);
-                            run.in += ex2(run.o.exponent(f, c));
+                            run.add_listed(Type<T>::load(e), c);
                             *e = Type<T>::round(-INFINITY);
                         }
                         tc::fence_to_async();  // the next copy into this place comes after these writes
@@ -707,17 +724,17 @@ distill_kernel(const DistillArgs a, const Layout lay)
                 for (uint32_t v0 = 0; v0 < whole_vecs; v0 += lay.chunk_vecs) add(v0, std::true_type());
                 if (whole_vecs < shape.vecs) add(whole_vecs, std::false_type());
                 if (threadIdx.x < edge) {
-                    run.raise(f_edge, c);
-                    const float e = ex2(run.o.exponent(f_edge, c));
                     bool in = false;
                     if (kBucket) {
                         const uint32_t bit = bit_of<T>(shape, v_edge);
                         in = (bits[bit >> 5] >> (bit & 31)) & 1;
                     }
-                    if (in)
-                        run.in += e;
-                    else
-                        run.out = add2(run.out, Pair(e, 0.f));
+                    if (in) {
+                        run.add_listed(f_edge, c);
+                    } else {
+                        run.raise(f_edge, c);
+                        run.out = add2(run.out, Pair(ex2(run.o.exponent(f_edge, c)), 0.f));
+                    }
                 }
                 // join the threads
                 float m = run.o.m;
@@ -725,33 +742,55 @@ distill_kernel(const DistillArgs a, const Layout lay)
                 for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
                 const float f = lost ? NAN : run.o.factor(Origin(m, c), c);
                 const float2 two = run.out.get();
-                const float w_out = warp_sum((two.x + two.y) * f), w_in = kBucket ? warp_sum(run.in * f) : 0.f;
-                if (lane == 0) s_m[warp] = m, s_out[warp] = w_out, s_in[warp] = w_in;
-                asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory");  // the warps of the pass
-                M = lane < warps ? s_m[lane] : -INFINITY;
-                float out = lane < warps ? s_out[lane] : 0.f, in = lane < warps ? s_in[lane] : 0.f;
-                const Origin mine(M, c);
+                const float w_out = warp_sum((two.x + two.y) * f);
+                if (lane == 0) s_m[warp] = m, s_out[warp] = w_out;
+                // the listed ones' sum, from `from` to the largest of them
+                auto bring = [c](float from, float to) { return from == -INFINITY ? 1.f : ex2((from - to) * c); };
+                if (kBucket) {
+                    float m_in = run.m_in;
 #pragma unroll
-                for (int d = 16; d; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-                const float fw = mine.factor(Origin(M, c), c);
-                out = warp_sum(out * fw);
-                if (kBucket) in = warp_sum(in * fw);
-                const float inside = (float)slot.mass / (out + in);
-                outside = inside;
-                if (kBucket && slot.rest > 0.0) outside = inside - (float)(slot.rest / (double)out);
+                    for (int d = 16; d; d >>= 1) m_in = fmaxf(m_in, __shfl_xor_sync(0xffffffffu, m_in, d));
+                    const float w_in = warp_sum(run.in * bring(run.m_in, m_in));
+                    if (lane == 0) s_m_in[warp] = m_in, s_in[warp] = w_in;
+                }
+                asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory");  // the warps of the pass
+                M_out = lane < warps ? s_m[lane] : -INFINITY;
+                float out = lane < warps ? s_out[lane] : 0.f;
+                const Origin mine(M_out, c);
+#pragma unroll
+                for (int d = 16; d; d >>= 1) M_out = fmaxf(M_out, __shfl_xor_sync(0xffffffffu, M_out, d));
+                out = warp_sum(out * mine.factor(Origin(M_out, c), c));
+                float M = M_out, Z = out, inside;
+                if (kBucket) {
+                    float m_in = lane < warps ? s_m_in[lane] : -INFINITY, in = lane < warps ? s_in[lane] : 0.f;
+                    const float from = m_in;
+#pragma unroll
+                    for (int d = 16; d; d >>= 1) m_in = fmaxf(m_in, __shfl_xor_sync(0xffffffffu, m_in, d));
+                    in = warp_sum(in * bring(from, m_in));
+                    M = fmaxf(M_out, m_in);
+                    const Origin o(M, c);
+                    const float rest = out * Origin(M_out, c).factor(o, c);
+                    if (m_in != -INFINITY) in *= ex2(o.exponent(m_in, c));
+                    Z = rest + in;
+                    inside = (float)slot.mass / Z;
+                    outside = (float)((slot.mass * (double)(rest / Z) - slot.rest) / (double)out);
+                    if (out == 0.f && Z > 0.f && slot.rest <= 0.0) outside = 0.f;  // nothing there, and nothing wanted
+                } else {
+                    inside = outside = (float)slot.mass / Z;
+                }
                 if (threadIdx.x == 0) {
-                    slot.M = M, slot.out = out, slot.in = in, slot.inside = inside;
-                    a.stats[row] = make_float4(M, inside, outside, 0.f);
+                    slot.M = M, slot.Z = Z, slot.M_out = M_out, slot.out = out, slot.inside = inside;
+                    a.stats[row] = make_float4(M, inside, outside, M_out);
                 }
             } else {
                 const float4 st = a.stats[row];
-                M = st.x, outside = st.z;
-                if (threadIdx.x == 0) slot.M = M, slot.inside = st.y;
+                M_out = st.w, outside = st.z;
+                if (threadIdx.x == 0) slot.M = st.x, slot.inside = st.y;
             }
 
             if (kWhat & kGrad) {
                 const float k_out = outside * slot.grad;
-                const Origin o(M, c);
+                const Origin o(M_out, c);
                 const bool same_offset = (((uintptr_t)z ^ (uintptr_t)g) & 15u) == 0;
                 auto write = [&](uint32_t v0, auto whole, auto plain) {
                     const Pair c2(c, c), r2(-o.r, -o.r), k2(k_out, k_out);
