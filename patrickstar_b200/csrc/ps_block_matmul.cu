@@ -615,24 +615,6 @@ bool use_pairs(uint32_t m, uint32_t n, uint32_t n_kb, int sms)
     return as_pairs <= as_split;
 }
 
-// Lets a kernel have that much shared memory; `seen`: the devices on which that is done.
-template <typename F>
-int allow_smem(F kernel, uint32_t bytes, std::atomic<uint64_t>& seen)
-{
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    const uint64_t bit = 1ull << (dev & 63);
-    if (e == cudaSuccess && dev < 64 && (seen.load(std::memory_order_relaxed) & bit)) return PS_OK;
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    if (e == cudaSuccess) {
-        seen.fetch_or(bit, std::memory_order_relaxed);
-        return PS_OK;
-    }
-    ps_internal::set_cuda_error((int)e);
-    cudaGetLastError();
-    return PS_ERR_CUDA;
-}
-
 template <int kOut>
 int launch_pairs_as(const ProductArgs& p, const CUtensorMap* maps, const CUtensorMap& out, uint32_t grid, cudaStream_t st)
 {

@@ -48,6 +48,7 @@ constexpr int kCtas = 3;  // of the largest kind on an SM: 64 registers a thread
 // Bytes of rows in work, of 126 MB of L2.  8192 x 50257 fp16 with gradient: 373 us with 64 MB, 460 us with 32 MB (two
 // CTAs an SM), 377 us with 128 MB; 4096 x 50257 fp32 318, 434 and 371 us.
 constexpr uint64_t kRowsInL2 = 64ull << 20;
+constexpr uint32_t kMostSmem = 224 * 1024;  // of a CTA: what the layout below may take, beside 3 KB that are static
 constexpr int kUnroll = 4;  // vectors of a chunk for each thread of the pass
 
 __device__ unsigned int g_gave_up;  // CTAs that ran into the limit of a wait
@@ -870,15 +871,10 @@ __global__ void distill_sum_kernel(const float* row_loss, uint32_t rows, const f
 template <typename T, bool kBucket, int kWhat, bool kLong>
 int launch(const DistillArgs& a, const Layout& lay, size_t smem, uint32_t grid, cudaStream_t st)
 {
-    if (smem > 40 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(distill_kernel<T, kBucket, kWhat, kLong>,
-                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) {
-            ps_internal::set_cuda_error((int)e);
-            cudaGetLastError();
-            return PS_ERR_CUDA;
-        }
-    }
+    if (smem > kMostSmem) return PS_ERR_LIMIT;
+    static std::atomic<uint64_t> seen{0};
+    const int rc = allow_smem(distill_kernel<T, kBucket, kWhat, kLong>, kMostSmem, seen);
+    if (rc != PS_OK) return rc;
     launch_behind(distill_kernel<T, kBucket, kWhat, kLong>, grid, lay.threads + 64, (uint32_t)smem, 0, st, a, lay);
     return ps_internal::after_launch();
 }
@@ -912,7 +908,7 @@ int launch(const DistillArgs& a, cudaStream_t st)
         const size_t limit = (lay.shift == 9 ? 108 : 200) * 1024;  // two CTAs an SM
         for (lay.slots = kMaxSlots; lay.slots > 2 && smem_bytes(lay, a.k, a.vocab, bits, seen) > limit; --lay.slots) {}
         smem = smem_bytes(lay, a.k, a.vocab, bits, seen);
-        if (smem <= 224 * 1024 || lay.shift == 6) break;  // the longest bitmaps leave room for small chunks only
+        if (smem <= kMostSmem || lay.shift == 6) break;  // the longest bitmaps leave room for small chunks only
     }
     const bool is_long = lay.shift == 9;
     // As many rows in work as SMs hold, but for the gradient no more than L2 keeps until the second pass.

@@ -7,8 +7,12 @@
 #ifndef PS_B200_LAUNCH_CUH
 #define PS_B200_LAUNCH_CUH
 
+#include "ps_b200.h"
+#include "ps_internal.h"
+
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <cstring>
 
@@ -31,6 +35,26 @@ void launch_behind(K kernel, uint32_t grid, uint32_t threads, uint32_t smem, uin
     cfg.attrs = at;
     cfg.numAttrs = cluster > 0 ? 2 : 1;
     cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// Lets a kernel have that much shared memory; `seen`: the devices on which that is done.  The limit belongs to the
+// kernel, not to a launch: `bytes` is the most that any launch of it asks for, since another thread may be between
+// this and its own launch.
+template <typename F>
+int allow_smem(F kernel, uint32_t bytes, std::atomic<uint64_t>& seen)
+{
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    const uint64_t bit = 1ull << (dev & 63);
+    if (e == cudaSuccess && dev < 64 && (seen.load(std::memory_order_relaxed) & bit)) return PS_OK;
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess) {
+        seen.fetch_or(bit, std::memory_order_relaxed);
+        return PS_OK;
+    }
+    ps_internal::set_cuda_error((int)e);
+    cudaGetLastError();
+    return PS_ERR_CUDA;
 }
 
 #endif

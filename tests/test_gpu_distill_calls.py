@@ -1,0 +1,41 @@
+"""Calls of the distillation loss from several threads."""
+import threading
+
+import pytest
+import torch
+
+from test_gpu_distill import DEV, _ps, make
+
+pytestmark = pytest.mark.gpu
+
+
+def test_threads_with_different_sizes():
+    """Vocabularies that take very different amounts of shared memory in the same kernel, from eight threads with as
+    little as possible between the calls: none of them may find the kernel set up for another's size."""
+    import ctypes as C
+    from patrickstar_b200 import _lib as L
+    vocabs = [2 ** 19, 20000, 100000, 2 ** 19, 40000, 30000, 2 ** 19, 20000]
+    wrong, ready = [], threading.Barrier(len(vocabs), timeout=120)
+
+    def work(i):
+        z, idx, teacher = make(1, vocabs[i], 1, torch.float16, i, "bucket")
+        problem = L.DistillProblem(z.data_ptr(), idx.data_ptr(), teacher.data_ptr(), None, vocabs[i], 1, 1, 1, vocabs[i], 1,
+                                   L.PS_DTYPE_F16, 8, L.PS_DTYPE_F32, L.PS_TAIL_BUCKET, L.PS_REDUCE_NONE, 1.0, 1.0)
+        out = torch.zeros(8, device=DEV)
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        args = (C.byref(problem), None, out.data_ptr(), out.data_ptr() + 16, None, None, None, 0, None, stream.cuda_stream)
+        ready.wait()
+        codes = [L.lib.ps_distill_forward(*args) for _ in range(2000)]
+        stream.synchronize()
+        want = _ps().distillation_loss(z, idx, teacher, tail="bucket", reduction="none")
+        if any(codes) or not torch.equal(out[:1], want):
+            wrong.append((vocabs[i], sum(c != 0 for c in codes)))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(vocabs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not wrong
