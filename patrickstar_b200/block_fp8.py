@@ -19,6 +19,7 @@ import functools
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import (PS_BLOCKS_COL, PS_BLOCKS_ROW, PS_BLOCKS_ROW_COL, PS_BLOCKS_TILE, PS_DTYPE_BF16, PS_DTYPE_F16,
                    PS_DTYPE_F32, PS_FP8_E4M3, PS_FP8_E5M2, PS_KEEP_INPUT, PS_KEEP_WEIGHT, BlockOperand, Fp8LinearLayer,
@@ -312,6 +313,14 @@ def _aligned(data):
     return out
 
 
+def _autograd_sees(*tensors):
+    """Whether a call has to go through its autograd function: for a gradient, or inside of a forward-mode level, where
+    the function refuses tensors that carry a tangent (``requires_grad`` does not tell) instead of losing it."""
+    if forward_ad._current_level >= 0:
+        return True
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 class _Fp8Linear(torch.autograd.Function):
     """y = Q_row(x) Q_tile(w)^T + b;  dx = Q_row(dy) Q_tile(w);  dw = Q_col(dy)^T Q_col(x);  db = sum of dy."""
 
@@ -362,7 +371,7 @@ def fp8_linear(x, weight, bias=None, grad_fmt="e4m3"):
     16 bytes they are views of longer rows, not contiguous.  ``weight``
     may also be a ``BlockQuantized`` with "tile" blocks, quantized once and kept; it has no
     gradient then.  Between forward and backward the quantized ``x`` and ``weight`` are kept (one
-    byte an element), not the originals.
+    byte an element), not the originals.  A second derivative and forward-mode derivatives are refused.
     """
     _check_float(x, "fp8_linear: x")
     if x.dim() < 1:
@@ -387,8 +396,7 @@ def fp8_linear(x, weight, bias=None, grad_fmt="e4m3"):
     if bias is not None:
         _check_bias(bias, n, dev, "fp8_linear")
     x2 = x if len(shape) == 2 else x.reshape(math.prod(shape[:-1]), k)
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
-                                    (bias is not None and bias.requires_grad)):
+    if _autograd_sees(x, weight, bias):
         y = _Fp8Linear.apply(x2, weight, bias, kept, grad_fmt)
     else:
         y = _linear_forward(x2, weight, bias, kept, 0)[0]

@@ -14,7 +14,7 @@ import torch
 
 from ._lib import (PS_DISTILL_MAX_K, PS_DISTILL_MAX_VOCAB, PS_REDUCE_MEAN, PS_REDUCE_NONE, PS_REDUCE_SUM,
                    PS_TAIL_BUCKET, PS_TAIL_DROP, DistillProblem, check, lib)
-from .block_fp8 import _DTYPES
+from .block_fp8 import _DTYPES, _autograd_sees
 from .streams import current_device, raw_stream
 
 _TAILS = {"drop": PS_TAIL_DROP, "bucket": PS_TAIL_BUCKET}
@@ -116,7 +116,7 @@ def distillation_loss(logits, indices, teacher, *, temperature=1.0, tail="drop",
                  that arrives with another factor computes it anew.  Not with reduction "none"
 
     The loss is float32, computed from 32-bit exponentials and 64-bit logarithms; the gradient has the type
-    of ``logits`` and is rounded once.
+    of ``logits`` and is rounded once.  A second derivative and forward-mode derivatives are refused.
     """
     for t, name in ((logits, "logits"), (teacher, "teacher")):
         if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in _DTYPES:
@@ -164,7 +164,7 @@ def distillation_loss(logits, indices, teacher, *, temperature=1.0, tail="drop",
         mask = mask.reshape(-1).contiguous()
     problem = DistillProblem(None, None, None, None, 0, 0, 0, z.shape[0], vocab, k, _DTYPES[z.dtype], idx.element_size(),
                              _DTYPES[values.dtype], _TAILS[tail], _REDUCTIONS[reduction], temperature, weight)
-    if torch.is_grad_enabled() and z.requires_grad:
+    if _autograd_sees(z):
         out = _Distill.apply(z, idx, values, mask, problem, scaler)
     else:
         out = _forward(z, idx, values, mask, problem, None)[0]

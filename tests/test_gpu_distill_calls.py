@@ -1,8 +1,9 @@
-"""Calls of the distillation loss from several threads."""
+"""Calls of the distillation loss from several threads and under forward-mode differentiation."""
 import threading
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 from test_gpu_distill import DEV, _ps, make
 
@@ -39,3 +40,24 @@ def test_threads_with_different_sizes():
         t.join()
     torch.cuda.synchronize()
     assert not wrong
+
+
+@pytest.mark.parametrize("which", [0, 2])
+def test_a_forward_mode_derivative_is_refused(which):
+    ps = _ps()
+    args = list(make(4, 333, 5, torch.float32, 1, "drop"))
+    ps_loss = ps.distillation_loss(*args)
+    with fwd.dual_level():
+        assert torch.equal(ps.distillation_loss(*args), ps_loss)     # no tangent: as ever
+        args[which] = fwd.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(RuntimeError):
+            ps.distillation_loss(*args)
+        with torch.no_grad(), pytest.raises(RuntimeError):
+            ps.distillation_loss(*args)
+
+
+def test_jvp_is_refused():
+    ps = _ps()
+    z, idx, teacher = make(4, 333, 5, torch.float32, 1, "drop")
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda t: ps.distillation_loss(t, idx, teacher), (z,), (torch.ones_like(z),))
