@@ -194,12 +194,10 @@ def block_quantize(x, blocks="row", fmt="e4m3"):
 
 
 def _rows(like, m, n, dtype):
-    """An uninitialised [m, n] tensor on the device of ``like`` whose rows start on 16-byte boundaries: the product then leaves the SM in whole
-    boxes.  Rows of other sizes are a view of longer ones."""
+    """An uninitialised [m, n] tensor on the device of ``like`` whose rows start on 16-byte boundaries: the product then
+    leaves the SM in whole boxes.  It is no view: autograd refuses in-place operations on views that a function made."""
     per = 16 // dtype.itemsize
-    ld = -(-n // per) * per
-    out = like.new_empty((m, ld), dtype=dtype)
-    return out if ld == n else out[:, :n]
+    return like.new_empty_strided((m, n), (-(-n // per) * per, 1), dtype=dtype)
 
 
 def _matmul(a, a_dim, b, b_dim, bias, out_dtype):
@@ -232,8 +230,8 @@ def block_matmul(a, b, a_dim=None, b_dim=None, bias=None, out_dtype=torch.float1
 
     Returns ``[outer size of a, outer size of b]`` in ``out_dtype`` (float16, bfloat16 or float32),
     accumulated in 32 bits and rounded once, after ``bias`` (one value for each column) was added.
-    Rows of the result start on 16-byte boundaries: where a row is not a multiple of 16 bytes it is a
-    view of longer rows, not contiguous.
+    Rows of the result start on 16-byte boundaries: where a row is not a multiple of 16 bytes the result
+    is not contiguous.
     """
     a_dim, b_dim = _dim(a, a_dim, "a"), _dim(b, b_dim, "b")
     if a.device != b.device:
@@ -368,10 +366,10 @@ def fp8_linear(x, weight, bias=None, grad_fmt="e4m3"):
     The result and the gradient of ``x`` have the type of ``x``, the gradients of ``weight`` and
     ``bias`` theirs; the gradient of ``bias`` is summed from the unquantized gradient.  Rows of the
     result and of the gradient of ``x`` start on 16-byte boundaries: where N (or K) is not a multiple of
-    16 bytes they are views of longer rows, not contiguous.  ``weight``
-    may also be a ``BlockQuantized`` with "tile" blocks, quantized once and kept; it has no
-    gradient then.  Between forward and backward the quantized ``x`` and ``weight`` are kept (one
-    byte an element), not the originals.  A second derivative and forward-mode derivatives are refused.
+    16 bytes they are not contiguous.  ``weight`` may also be a ``BlockQuantized`` with "tile" blocks,
+    quantized once and kept; it has no gradient then.  Between forward and backward the quantized ``x``
+    and ``weight`` are kept (one byte an element), not the originals.  A second derivative and
+    forward-mode derivatives are refused.
     """
     _check_float(x, "fp8_linear: x")
     if x.dim() < 1:

@@ -1,4 +1,5 @@
-"""The 8-bit layer where a model has it in the place of `torch.nn.Linear`: forward-mode differentiation."""
+"""The 8-bit layer where a model has it in the place of `torch.nn.Linear`: results changed in place,
+forward-mode differentiation."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
@@ -6,6 +7,35 @@ import torch.autograd.forward_ad as fwd
 from test_gpu_block_fp8 import DEV, _ps, linear_case
 
 pytestmark = pytest.mark.gpu
+WIDTHS = [1, 2, 13, 130, 2305]
+
+
+def layer(n, k=96, dtype=torch.float16, bias=True):
+    torch.manual_seed(n)
+    m = torch.nn.Linear(k, n, bias=bias).to(DEV, dtype)
+    assert _ps().use_fp8_linears(m) == 1
+    return m
+
+
+@pytest.mark.parametrize("n", WIDTHS)
+@pytest.mark.parametrize("op,args", [("relu", ()), ("add", (1.5,)), ("div", (2.0,))])
+@pytest.mark.parametrize("how", ["layer", "function", "matrix"])
+def test_results_are_changed_in_place(how, op, args, n):
+    """... by what reads them next, at any width, with the gradients of the same operation out of place."""
+    ps = _ps()
+    m = layer(n)
+    x = torch.randn(4, 33, 96, device=DEV).half()
+    got = []
+    for name in (op + "_", op):
+        leaves = [t.detach().clone().requires_grad_(True) for t in (x, m.weight, m.bias)]
+        if how == "layer":
+            y = torch.func.functional_call(m, {"weight": leaves[1], "bias": leaves[2]}, (leaves[0],))
+        else:
+            y = ps.fp8_linear(leaves[0] if how == "function" else leaves[0].view(-1, 96), leaves[1], leaves[2])
+        z = getattr(y, name)(*args)
+        assert (z is y) == name.endswith("_")
+        got.append([z.detach()] + list(torch.autograd.grad(z.float().sum(), leaves)))
+    assert all(torch.equal(p, q) for p, q in zip(*got))
 
 
 @pytest.mark.parametrize("which", [0, 1, 2])
