@@ -1,5 +1,5 @@
-"""The 8-bit layer where a model has it in the place of `torch.nn.Linear`: results changed in place,
-forward-mode differentiation."""
+"""The 8-bit layer where a model has it in the place of `torch.nn.Linear`: results changed in place or
+viewed in another shape, forward-mode differentiation."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
@@ -36,6 +36,26 @@ def test_results_are_changed_in_place(how, op, args, n):
         assert (z is y) == name.endswith("_")
         got.append([z.detach()] + list(torch.autograd.grad(z.float().sum(), leaves)))
     assert all(torch.equal(p, q) for p, q in zip(*got))
+
+
+@pytest.mark.parametrize("n", WIDTHS)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_the_layer_s_results_can_be_viewed_in_any_shape(n, dtype):
+    """As those of the layer it replaces: across the last dimension too."""
+    m = layer(n, dtype=dtype)
+    x = torch.randn(4, 34, 96, device=DEV).to(dtype).requires_grad_(True)
+    y = m(x)
+    assert y.is_contiguous() and y.shape == (4, 34, n)
+    flat = y.view(-1)
+    a = torch.autograd.grad(flat.float().square().sum(), [x, m.weight])
+    y = m(x)
+    b = torch.autograd.grad(y.float().square().sum(), [x, m.weight])
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    assert torch.equal(m(x).view(2, -1), _ps().fp8_linear(x, m.weight, m.bias).reshape(2, -1))
+    with torch.no_grad():
+        assert m(x[0]).view(-1).shape == (34 * n,)
+    m.contiguous = False    # rows on 16-byte boundaries
+    assert torch.equal(m(x), y) and m(x).stride(1) * m(x).element_size() % 16 == 0
 
 
 @pytest.mark.parametrize("which", [0, 1, 2])
