@@ -44,6 +44,7 @@ class _DeviceScaler:
                 "patrickstar_b200 loss scalers keep their state on a CUDA device; no device found")
         self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         self._state = torch.zeros(C.sizeof(ScalerState), dtype=torch.uint8, device=self.device)
+        self.device = self._state.device    # with its number: "cuda" is the current device
         # int32 overflow flag, OR-ed into by the scan kernels
         self._flag = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._host_init = init

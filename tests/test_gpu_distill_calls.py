@@ -1,4 +1,5 @@
-"""Calls of the distillation loss from several threads and under forward-mode differentiation."""
+"""Calls of the distillation loss from several threads, under forward-mode differentiation and with a
+scaler that was given a device without its number."""
 import threading
 
 import pytest
@@ -61,3 +62,18 @@ def test_jvp_is_refused():
     z, idx, teacher = make(4, 333, 5, torch.float32, 1, "drop")
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda t: ps.distillation_loss(t, idx, teacher), (z,), (torch.ones_like(z),))
+
+
+@pytest.mark.parametrize("kind", ["LossScaler", "DynamicLossScaler"])
+def test_a_scaler_on_the_current_device_by_its_type(kind):
+    """`device="cuda"` is the current device."""
+    ps = _ps()
+    z, idx, teacher = make(4, 333, 5, torch.float16, 2, "drop")
+    scaler = getattr(ps, kind)(8.0, device="cuda")
+    assert scaler.device == z.device
+    z.requires_grad_(True)
+    loss = ps.distillation_loss(z, idx, teacher, scaler=scaler)
+    scaler.backward(loss)
+    other = z.detach().clone().requires_grad_(True)
+    (ps.distillation_loss(other, idx, teacher) * 8.0).backward()
+    assert torch.equal(z.grad, other.grad)
