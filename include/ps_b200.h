@@ -628,7 +628,7 @@ typedef struct ps_distill_problem {
     uint64_t ld_logits, ld_indices, ld_teacher;
     uint32_t rows, vocab, k;
     int32_t dtype, index_bytes, teacher_dtype, tail, reduction;
-    float temperature, weight;
+    float temperature, weight; /* temperature: a normal number */
 } ps_distill_problem;
 
 /* Losses of the rows (row_loss, float [rows]) and, unless reduction is NONE,

@@ -36,6 +36,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <cfloat>
 #include <cstring>
 #include <type_traits>
 
@@ -947,7 +948,8 @@ int check_problem(const ps_distill_problem* q, const float* inv_n)
     if (q->index_bytes != 4 && q->index_bytes != 8) return PS_ERR_INVALID;
     if (q->tail != PS_TAIL_DROP && q->tail != PS_TAIL_BUCKET) return PS_ERR_INVALID;
     if (q->reduction < PS_REDUCE_NONE || q->reduction > PS_REDUCE_MEAN) return PS_ERR_INVALID;
-    if (!(q->temperature > 0.f) || !(q->temperature < INFINITY) || !(q->weight < INFINITY) || !(q->weight > -INFINITY))
+    // below the normal numbers log2(e) / temperature is not finite any more
+    if (!(q->temperature >= FLT_MIN) || !(q->temperature < INFINITY) || !(q->weight < INFINITY) || !(q->weight > -INFINITY))
         return PS_ERR_INVALID;
     if (q->rows == 0) return PS_OK;
     if (q->vocab == 0 || q->k == 0) return PS_ERR_INVALID;

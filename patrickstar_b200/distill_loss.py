@@ -18,6 +18,7 @@ from .block_fp8 import _DTYPES, _autograd_sees
 from .streams import current_device, raw_stream
 
 _TAILS = {"drop": PS_TAIL_DROP, "bucket": PS_TAIL_BUCKET}
+_SMALLEST, _LARGEST = torch.finfo(torch.float32).tiny, torch.finfo(torch.float32).max    # what the C struct holds
 _REDUCTIONS = {"none": PS_REDUCE_NONE, "sum": PS_REDUCE_SUM, "mean": PS_REDUCE_MEAN}
 
 
@@ -129,10 +130,11 @@ def distillation_loss(logits, indices, teacher, *, temperature=1.0, tail="drop",
         raise ValueError("distillation_loss: tail must be drop or bucket; got %r" % (tail,))
     if reduction not in _REDUCTIONS:
         raise ValueError("distillation_loss: reduction must be none, sum or mean; got %r" % (reduction,))
-    if not (temperature > 0 and math.isfinite(temperature)):
-        raise ValueError("distillation_loss: temperature must be positive and finite; got %r" % (temperature,))
-    if not math.isfinite(weight):
-        raise ValueError("distillation_loss: weight must be finite; got %r" % (weight,))
+    if not _SMALLEST <= temperature <= _LARGEST:
+        raise ValueError("distillation_loss: temperature must be positive, finite and normal in 32 bits; got %r"
+                         % (temperature,))
+    if not abs(weight) <= _LARGEST:
+        raise ValueError("distillation_loss: weight must be finite in 32 bits; got %r" % (weight,))
     if logits.dim() < 1 or indices.shape != teacher.shape or indices.shape[:-1] != logits.shape[:-1] \
             or indices.dim() != logits.dim():
         raise ValueError("distillation_loss: logits [..., vocab], indices [..., k] and teacher [..., k] do not fit: "

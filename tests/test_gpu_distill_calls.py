@@ -77,3 +77,15 @@ def test_a_scaler_on_the_current_device_by_its_type(kind):
     other = z.detach().clone().requires_grad_(True)
     (ps.distillation_loss(other, idx, teacher) * 8.0).backward()
     assert torch.equal(z.grad, other.grad)
+
+
+def test_temperatures_at_the_ends():
+    """1 / T has to be a number of 32 bits."""
+    ps = _ps()
+    z, idx, teacher = make(4, 333, 5, torch.float32, 3, "drop")
+    for t in (1e-39, 1e-46, 1e39):
+        with pytest.raises(ValueError):
+            ps.distillation_loss(z, idx, teacher, temperature=t)
+    with pytest.raises(ValueError):
+        ps.distillation_loss(z, idx, teacher, weight=1e39)
+    assert torch.isfinite(ps.distillation_loss(z, idx, teacher, temperature=1e-30))
