@@ -1,5 +1,5 @@
-"""Calls of the distillation loss from several threads, under forward-mode differentiation and with a
-scaler that was given a device without its number."""
+"""Calls of the distillation loss from several threads, by its module, under forward-mode differentiation and with
+a scaler that was given a device without its number."""
 import threading
 
 import pytest
@@ -89,3 +89,19 @@ def test_temperatures_at_the_ends():
     with pytest.raises(ValueError):
         ps.distillation_loss(z, idx, teacher, weight=1e39)
     assert torch.isfinite(ps.distillation_loss(z, idx, teacher, temperature=1e-30))
+
+
+def test_the_module_is_the_function():
+    ps = _ps()
+    z, idx, teacher = make(12, 700, 6, torch.bfloat16, 4, "bucket")
+    mask = torch.arange(12, device=DEV) % 3 != 0
+    scaler = ps.LossScaler(32.0)
+    kw = dict(temperature=2.0, tail="bucket", reduction="sum", weight=0.5, scaler=scaler)
+    module = ps.DistillationLoss(**kw)
+    for m in (None, mask):
+        a, b = z.clone().requires_grad_(True), z.clone().requires_grad_(True)
+        la, lb = module(a, idx, teacher, m), ps.distillation_loss(b, idx, teacher, mask=m, **kw)
+        assert torch.equal(la, lb)
+        scaler.backward(la)
+        scaler.backward(lb)
+        assert torch.equal(a.grad, b.grad)

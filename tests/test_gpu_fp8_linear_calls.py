@@ -1,10 +1,11 @@
 """The 8-bit layer where a model has it in the place of `torch.nn.Linear`: results changed in place or
-viewed in another shape, forward-mode differentiation."""
+viewed in another shape, forward-mode differentiation, operands of different types,
+kept weights."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
 
-from test_gpu_block_fp8 import DEV, _ps, linear_case
+from test_gpu_block_fp8 import DEV, _ps, linear_case, product_bound, rounded
 
 pytestmark = pytest.mark.gpu
 WIDTHS = [1, 2, 13, 130, 2305]
@@ -80,3 +81,97 @@ def test_jvp_is_refused():
     x, w, b, _ = (t.to(DEV) for t in linear_case(20, 64, 48, torch.float32, 1))
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda t: ps.fp8_linear(t, w, b), (x,), (torch.ones_like(x),))
+
+
+@pytest.mark.parametrize("kinds", [("float16", "float32", "bfloat16"), ("bfloat16", "float16", "float32"),
+                                   ("float32", "bfloat16", "float16")])
+def test_input_weight_and_bias_of_different_types(kinds):
+    ps = _ps()
+    tx, tw, tb = (getattr(torch, k) for k in kinds)
+    x, w, b, dy = linear_case(130, 257, 129, torch.float32, 5)
+    x, w, b, dy = x.to(tx), w.to(tw), b.to(tb), dy.to(tx)
+    leaves = [t.to(DEV).requires_grad_(True) for t in (x, w, b)]
+    y = ps.fp8_linear(*leaves)
+    grads = torch.autograd.grad(y, leaves, dy.to(DEV))
+    assert (y.dtype,) + tuple(g.dtype for g in grads) == (tx, tx, tw, tb)
+    xr, xc, wt = rounded(x, "row", "e4m3"), rounded(x, "col", "e4m3"), rounded(w, "tile", "e4m3")
+    dr, dc = rounded(dy, "row", "e4m3"), rounded(dy, "col", "e4m3")
+    for got, p, q, length, extra in ((y, xr, wt, 257, b.double()), (grads[0], dr, wt.t(), 129, None),
+                                     (grads[1], dc.t(), xc.t(), 130, None)):
+        want = p @ q.t()
+        bound = product_bound(p, q, length, got.dtype, want)
+        if extra is not None:    # one more addition, of the bias, in 32 bits
+            want = want + extra
+            bound = bound + 2.0 ** -24 * want.abs() + torch.finfo(got.dtype).eps / 2 * want.abs()
+        assert ((got.detach().cpu().double() - want).abs() <= bound).all()
+    want = dy.double().sum(0)    # runs of 128 rows in 32 bits, the runs in 64, two roundings
+    bound = 130 * 2.0 ** -24 * dy.double().abs().sum(0) + torch.finfo(tb).eps / 2 * want.abs()
+    assert ((grads[2].cpu().double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("tokens,k,n", [(1, 64, 48), (130, 257, 129), (300, 130, 1)])
+def test_a_kept_weight_in_either_format_and_under_hooks(tokens, k, n, fmt):
+    """Forward and input gradient from it; under hooks its saved parts come back packed, elsewhere."""
+    ps = _ps()
+    x, w, b, dy = linear_case(tokens, k, n, torch.float16, 6)
+    kept = ps.block_quantize(w.to(DEV), "tile", fmt)
+    wt = rounded(w, "tile", fmt)
+
+    def run():
+        leaf = x.to(DEV).requires_grad_(True)
+        y = ps.fp8_linear(leaf, kept, b.to(DEV))
+        return y.detach(), torch.autograd.grad(y, leaf, dy.to(DEV))[0]
+
+    y, dx = run()
+    xr, dr = rounded(x, "row", "e4m3"), rounded(dy, "row", "e4m3")
+    want = xr @ wt.t()
+    bound = product_bound(xr, wt, k, torch.float16, want) + 2.0 ** -24 * (want + b.double()).abs() + \
+        2.0 ** -11 * (want + b.double()).abs()
+    assert ((y.cpu().double() - want - b.double()).abs() <= bound).all()
+    want = dr @ wt
+    assert ((dx.cpu().double() - want).abs() <= product_bound(dr, wt.t(), n, torch.float16, want)).all()
+    with torch.autograd.graph.save_on_cpu():
+        again = run()
+    assert torch.equal(again[0], y) and torch.equal(again[1], dx)
+
+
+def test_gradients_against_differences_with_the_scales_pinned():
+    """Every block of the input, the weight and the incoming gradient holds an element of full scale (448 2^j), the others
+    are whole numbers up to 7 times 2^j: with the scale 2^j that this element asks for, all of them are values of the format.
+    The layer is then exactly linear in the small elements, and differences of its outputs are its gradients."""
+    ps = _ps()
+    gen = torch.Generator().manual_seed(10)
+
+    def whole(r, c):
+        return torch.randint(-7, 8, (r, c), generator=gen).float()
+
+    x, w, dy = whole(128, 256), whole(128, 256), whole(128, 128)
+    # one element of full scale in each row and column of a tile: its diagonal
+    d = torch.arange(128)
+    for t in (x, w, dy):
+        for j in range(0, t.shape[1], 128):
+            t[d, j + d] = 448.0
+    X, W = x.half().to(DEV).requires_grad_(True), w.half().to(DEV).requires_grad_(True)
+    gx, gw = torch.autograd.grad(ps.fp8_linear(X.float(), W.float()), [X, W], dy.to(DEV))
+
+    def value(xx, ww):
+        # sums of at most 256 products of up to 448 448 are whole numbers below 2^26; in 32 bits those here are exact
+        # when they stay below 2^24, which the assertion on them holds
+        y = ps.fp8_linear(xx.to(DEV), ww.to(DEV)).double().cpu()
+        assert torch.equal(y, xx.double() @ ww.double().t()) and float(y.abs().max()) < 2 ** 24
+        return float((y * dy.double()).sum())
+
+    base = value(x, w)
+    for i, j in ((0, 1), (127, 200), (64, 130)):
+        moved = x.clone()
+        moved[i, j] += 1
+        assert value(moved, w) - base == float((dy.double() @ w.double())[i, j])
+        # the gradient itself is rounded to 16 bits
+        want = float((dy.double() @ w.double())[i, j])
+        assert abs(float(gx[i, j]) - want) <= 2.0 ** -11 * abs(want)
+        moved = w.clone()
+        moved[i, j] += 1
+        want = float((dy.double().t() @ x.double())[i, j])
+        assert value(x, moved) - base == want
+        assert abs(float(gw[i, j]) - want) <= 2.0 ** -11 * abs(want)
