@@ -24,7 +24,7 @@
 // others' pass.  Their gradient is written over the row's after it, so the pass
 // itself knows nothing of them but, for the bucket, one bit per element.
 // 4096 x 131073 bf16: loss alone 6.1 TB/s; 8192 x 50257 fp16, k = 64: loss 155 us
-// (5.3 TB/s), with the gradient 357 us (4.6 TB/s of one read and one write).  HBM-bound: one read, and one write for the
+// (5.3 TB/s), with the gradient 325 us (5.1 TB/s of one read and one write).  HBM-bound: one read, and one write for the
 // gradient; a power of two per element each pass.
 #include "ps_b200.h"
 
@@ -46,8 +46,8 @@ constexpr int kMaxThreads = 320;   // 256 of the pass
 constexpr int kLongThreads = 576;  // 512 of the pass, for the longest rows
 constexpr uint32_t kMaxSlots = 4;
 constexpr int kCtas = 3;  // of the largest kind on an SM: 64 registers a thread
-// Bytes of rows in work, of 126 MB of L2.  8192 x 50257 fp16 with gradient: 373 us with 64 MB, 460 us with 32 MB (two
-// CTAs an SM), 377 us with 128 MB; 4096 x 50257 fp32 318, 434 and 371 us.
+// Bytes of rows in work, of 126 MB of L2.  8192 x 50257 fp16 with gradient: 325 us with 64 MB, 386 us with 32 MB (two
+// CTAs an SM), 359 us with 128 MB; with the bucket 383, 475 and 383 us.
 constexpr uint64_t kRowsInL2 = 64ull << 20;
 constexpr uint32_t kMostSmem = 224 * 1024;  // of a CTA: what the layout below may take, beside 3 KB that are static
 constexpr int kUnroll = 4;  // vectors of a chunk for each thread of the pass
@@ -887,21 +887,19 @@ int launch(const DistillArgs& a, cudaStream_t st)
     if (sms < 0) return sms;
     // Threads for a row by its size: four vectors a thread and chunk, four chunks.  Small CTAs, since each brings a
     // warp for listed entries and rows' own latencies overlap (8192 x 50257 fp16, loss: 158 us with 128 threads,
-    // 167 us with 256).  With the gradient, where L2 limits the rows in work, 256 threads do better (385 -> 357 us with
-    // 64 entries; 4096 x 70000 bf16 302 -> 240 us) if a row is long for its entries (128 of them: 455 -> 570 us).  512
-    // threads for the longest rows, of which L2 keeps two an SM for the second pass, and where there is no more than one
-    // row for an SM.
+    // 167 us with 256; with the gradient and 8, 64 or 128 entries 308, 329 and 388 us, not 321, 343 and 448 us; with the
+    // bucket and 64 entries 385 us, not 404 us; 4096 x 70000 bf16 222 us, not 230 us).  512 threads for the longest rows,
+    // of which L2 keeps two an SM for the second pass, and where there is no more than one row for an SM.
     const uint64_t bytes = (uint64_t)a.vocab * sizeof(T);
     const bool few = a.rows <= (uint32_t)sms;
     const bool bits = kBucket && (kWhat & kLoss), seen = kWhat & kGrad;
     Layout lay;
-    const bool wide = kWhat == (kLoss | kGrad) && !kBucket && bytes >= 1280 * (uint64_t)a.k;
     if (bytes <= 16 * 1024)
         lay.shift = 6;
-    else if (!few && bytes <= (wide ? 48 : 160) * 1024)
+    else if (!few && bytes <= 160 * 1024)
         lay.shift = 7;
     else
-        lay.shift = bytes <= 32 * 1024 || (!few && bytes <= 160 * 1024) ? 8 : 9;
+        lay.shift = bytes <= 32 * 1024 ? 8 : 9;
     size_t smem;
     for (;; --lay.shift) {
         lay.threads = 1u << lay.shift;
