@@ -769,10 +769,12 @@ distill_kernel(const DistillArgs a, const Layout lay)
 #pragma unroll
                     for (int d = 16; d; d >>= 1) m_in = fmaxf(m_in, __shfl_xor_sync(0xffffffffu, m_in, d));
                     in = warp_sum(in * bring(from, m_in));
-                    M = fmaxf(M_out, m_in);
-                    const Origin o(M, c);
-                    const float rest = out * Origin(M_out, c).factor(o, c);
-                    if (m_in != -INFINITY) in *= ex2(o.exponent(m_in, c));
+                    // both relative to M_out, unless a listed element is far above it: one approximate power less
+                    const Origin others(M_out, c);
+                    float rest = out;
+                    if (M_out == -INFINITY ? m_in > -INFINITY : others.exponent(m_in, c) > 16.f)
+                        M = m_in, rest *= others.factor(Origin(M, c), c);
+                    if (m_in != -INFINITY) in *= ex2(Origin(M, c).exponent(m_in, c));
                     Z = rest + in;
                     inside = (float)slot.mass / Z;
                     outside = (float)((slot.mass * (double)(rest / Z) - slot.rest) / (double)out);
