@@ -229,7 +229,8 @@ def block_matmul(a, b, a_dim=None, b_dim=None, bias=None, out_dtype=torch.float1
     ``b_dim`` of ``b`` (each by default the one its blocks lie along; 1 for "tile" blocks).
 
     Returns ``[outer size of a, outer size of b]`` in ``out_dtype`` (float16, bfloat16 or float32),
-    accumulated in 32 bits and rounded once, after ``bias`` (one value for each column) was added.
+    accumulated in 32 bits and rounded once, after ``bias`` (one value for each column) was added.  No
+    gradient flows through, to ``bias`` either.
     Rows of the result start on 16-byte boundaries: where a row is not a multiple of 16 bytes the result
     is not contiguous.
     """
@@ -368,8 +369,8 @@ def fp8_linear(x, weight, bias=None, grad_fmt="e4m3", contiguous=False):
     result and of the gradient of ``x`` start on 16-byte boundaries: where N (or K) is not a multiple of
     16 bytes they are not contiguous, but for the result if ``contiguous`` asks for it.  ``weight`` may
     also be a ``BlockQuantized`` with "tile" blocks, quantized once and kept; it has no gradient then.
-    Between forward and backward the quantized ``x`` and ``weight`` are kept (one byte an element), not
-    the originals.  A second derivative and forward-mode derivatives are refused.
+    Between forward and backward the quantized ``x`` and ``weight`` are kept (one byte an element; that of
+    ``weight`` comes on top of the parameter itself), not the originals.  A second derivative and forward-mode derivatives are refused.
     """
     _check_float(x, "fp8_linear: x")
     if x.dim() < 1:

@@ -592,7 +592,8 @@ int encode_operand(const ps_block_operand* o, uint64_t outer, uint64_t k, uint32
 
 uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 
-// CTAs that share a tile of 128 x 128 along k: as many as fill the SMs, with four k blocks each at least.
+// CTAs that share a tile of 128 x 128 along k: as many as fill the SMs, doubled while each has four k blocks: two
+// blocks each at least.
 uint32_t splits_of(uint64_t tiles, uint32_t n_kb, int sms)
 {
     uint32_t splits = 1;
